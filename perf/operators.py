@@ -493,7 +493,8 @@ def exact(case, seed):
                     mass = max(mass - rest[x], 0.0)
                     rest[x] = 0.0
                 else:
-                    less = np.maximum(rest - q, 0.0)
+                    # what is left of the target's mass, beside a draft of the same mass
+                    less = np.maximum(rest - mass * q, 0.0)
                     rest, mass = (less, less.sum()) if less.sum() > 0 else (rest, mass)
             if found is None:
                 break
