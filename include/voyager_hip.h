@@ -677,6 +677,128 @@ int vh_conv_pack_weight(const void* w, int32_t dtype, const vh_conv_geom* geom, 
 /* dst [n, c, p] = src [n, p, c] (bf16, fp16 or fp32). */
 int vh_nhwc_to_nchw(const void* src, int32_t dtype, int64_t n, int64_t p, int64_t c, void* dst, vh_stream_t stream);
 
+/* ------------------------------------------------- a step with drafted tokens
+ * Operators of a serving step that verifies several tokens of a sequence at
+ * once, beside the reference's own (it has none of them): rotary positions, a
+ * cache of keys and values in pages, attention of a tree of tokens over it,
+ * and the choice among drafted tokens. */
+
+/* Rotary positions.  q [batch, tokens, heads, dim] and k [.., kv_heads, dim]
+ * (either may have no heads), channels dense, other strides in elements; the
+ * outputs are contiguous.  The first `rotary` channels of a head turn by
+ * pos * turns[j] turns, j the pair: channels (j, j + rotary / 2), or (2 j,
+ * 2 j + 1) where interleaved; `factor` multiplies them; the rest are copied.
+ * pos: integers of pos_bits (32 or 64), strides in elements (0: shared).
+ * turns: rotary / 2 float64 in device memory.  inverse turns back: the
+ * gradient.  dim even, at most 512. */
+int vh_rope(const void* q, void* q_out, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, void* k_out,
+            int64_t k_sb, int64_t k_st, int64_t k_sh, int32_t dtype, int64_t batch, int64_t tokens, int32_t heads,
+            int32_t kv_heads, int32_t dim, int32_t rotary, int32_t interleaved, const void* pos, int32_t pos_bits,
+            int64_t pos_sb, int64_t pos_st, const double* turns, float factor, int32_t inverse, vh_stream_t stream);
+
+/* A cache in pages: slot s is row s % page of page s / page.  k, v:
+ * [pages, kv_heads, page, dim] of codes (E4M3 bytes, or int8 codes + 128) or
+ * 16-bit values; k_scale, v_scale: [pages, kv_heads, page], a float32 scale a
+ * row (unused for 16-bit values).  dim a multiple of 8.  Kernels never clear
+ * `flag`: they OR VH_CACHE_ERR_* into it where an index is out of range, and
+ * leave out what it would have named. */
+#define VH_CACHE_E4M3 0
+#define VH_CACHE_INT8 1
+#define VH_CACHE_F16 2
+#define VH_CACHE_BF16 3
+#define VH_CACHE_ERR_SLOT 1    /* a slot past the cache */
+#define VH_CACHE_ERR_PAGE 2    /* a page of a table, or a node of a path, that is not there */
+#define VH_CACHE_ERR_CONTEXT 4 /* a sequence longer than its pages */
+#define VH_CACHE_ERR_PARENT 8  /* a node whose parent is not before it */
+typedef struct vh_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t* flag;
+  int64_t slots, pages;
+  int32_t page, kv_heads, dim, fmt;
+} vh_cache;
+
+/* Writes n tokens' rows (k, v: [n, kv_heads, dim] in dtype, channels dense,
+ * strides of token and head in elements) into their slots, quantized:
+ * scale = amax / most, code = round(x * (most / amax)), most 448 or 127, amax
+ * at least 2^-100; a row with an infinity or NaN reads back as NaN.  Tokens
+ * with a negative slot are left out.  Slots must differ. */
+int vh_paged_write(const vh_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                   int64_t v_sh, int32_t dtype, const int64_t* slots, int64_t n, vh_stream_t stream);
+
+/* Reads n tokens back: code * scale rounded to dtype, contiguous
+ * [n, kv_heads, dim]; zeros where the slot is negative. */
+int vh_paged_read(const vh_cache* cache, void* k, void* v, int32_t dtype, const int64_t* slots, int64_t n,
+                  vh_stream_t stream);
+
+/* Moves the rows of kept nodes together: of sequence b, the row at position
+ * context[b] + path[b][i] to context[b] + i, for 1 <= i < count[b], codes and
+ * scales as they are.  table [batch, table_pages]: a sequence's pages; path
+ * [batch, nodes] rises.  In place. */
+int vh_paged_keep(const vh_cache* cache, const int32_t* table, int64_t table_st, int32_t table_pages,
+                  const int32_t* context, const int32_t* path, int64_t path_st, const int32_t* count, int64_t batch,
+                  int32_t nodes, vh_stream_t stream);
+
+/* The ancestors of each node of a tree (itself among them) as bits:
+ * masks [batch, nodes, (nodes + 63) / 64], from parents [batch, nodes], -1 for
+ * the first node.  Another node whose parent is negative pads its tree: it has
+ * no ancestors, itself included, and sees nothing.  A node whose parent is not
+ * before it is taken as padding, and VH_CACHE_ERR_PARENT set.  At most
+ * VH_TREE_MAX_NODES nodes. */
+#define VH_TREE_MAX_NODES 1024
+int vh_tree_masks(const int32_t* parents, int64_t batch, int32_t nodes, uint64_t* masks, int32_t* flag,
+                  vh_stream_t stream);
+
+/* Attention of `nodes` tokens of each sequence over the cache: q [batch,
+ * nodes, heads, dim] (dtype bfloat16 or float16, that of a 16-bit cache;
+ * channels dense, strides in elements) over the context[b] positions before
+ * them and, of the nodes, which lie at positions context[b] + n, those in its
+ * mask; with masks NULL, those up to itself.  o: contiguous, of q's dtype;
+ * lse (or NULL): [batch, nodes, heads] float32, the logarithm of the sum of
+ * exponentials.  A row that sees nothing gives 0 and -inf.  dim 64, 128 or
+ * 256, page a multiple of 16, heads a multiple of the cache's.  work: 16-byte
+ * aligned device memory of vh_tree_attention_workspace_bytes(desc) bytes.
+ * chunk: keys a workgroup takes, a multiple of 128, or 0 to let the library
+ * choose. */
+typedef struct vh_tree_desc {
+  vh_cache cache;
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  const int32_t* table;
+  int64_t table_st;
+  const int32_t* context;
+  const uint64_t* masks;
+  void* o;
+  float* lse;
+  void* work;
+  int64_t work_bytes;
+  float scale; /* of the scores, positive */
+  int32_t dtype, batch, nodes, heads, table_pages, chunk;
+} vh_tree_desc;
+int vh_tree_attention(const vh_tree_desc* desc, vh_stream_t stream);
+int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);
+
+/* The choice among drafted tokens.  target [batch, nodes, vocab] float32: the
+ * target's probabilities after each node; draft: those of the draft model, or
+ * NULL where each node's children were chosen, not sampled; tokens [batch,
+ * nodes]: each node's token (the first's is not read); u [batch, nodes], r
+ * [batch]: numbers in [0, 1).  From the first node on, a node's children are
+ * tried in order: with rest = the target's row and mass = 1, child n of token
+ * x is taken if u_n * mass * draft(x) < rest(x); else rest = max(rest - mass *
+ * draft, 0) and mass = its sum (a rest of nothing is left as it was).  With no
+ * draft, draft(x) counts as 1, rest(x) becomes 0 and mass loses it.  Where no
+ * child is taken the last token is the first index at which the running sum
+ * of rest passes r times the whole.  Sums are float64, in a fixed order.
+ * told [batch, nodes]: the tokens taken and then the last, -1 after them;
+ * path [batch, nodes]: the first node and those taken, -1 after them; count
+ * [batch]: how many.  A token outside the vocabulary is never taken.  work:
+ * vh_verify_workspace_bytes(batch, vocab) bytes, 16-byte aligned. */
+int vh_verify(const float* target, int64_t target_sb, int64_t target_sn, const float* draft, int64_t draft_sb,
+              int64_t draft_sn, const int32_t* parents, const int64_t* tokens, const float* u, const float* r,
+              int64_t batch, int32_t nodes, int64_t vocab, int64_t* told, int32_t* path, int32_t* count, void* work,
+              int64_t work_bytes, vh_stream_t stream);
+int64_t vh_verify_workspace_bytes(int64_t batch, int64_t vocab);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,207 @@
+// Trees of tokens: the ancestors of their nodes, and the entry point of their
+// attention, with the kernel that joins its splits.
+#include "vh_tree_attention.h"
+
+namespace tree {
+template <>
+int launch<64>(const Args& a, int nt, hipStream_t s);
+template <>
+int launch<128>(const Args& a, int nt, hipStream_t s);
+template <>
+int launch<256>(const Args& a, int nt, hipStream_t s);
+}  // namespace tree
+
+namespace {
+
+using tree::Args;
+using tree::f32x4;
+
+constexpr int MASK_THREADS = 256;
+constexpr int MAX_NODES = VH_TREE_MAX_NODES;
+constexpr int MAX_SPLITS = 256;
+
+// One workgroup a tree, one thread a word of a node's mask: it walks up from
+// the node and sets the bits that fall into its word.  Parents come before
+// their children, so every step goes down in number and the walk ends.
+__global__ void __launch_bounds__(MASK_THREADS) k_tree_masks(const int32_t* parents, int nodes, int words, uint64_t* masks,
+                                                             int32_t* flag) {
+  __shared__ int32_t s_parent[MAX_NODES];
+  const int32_t* p = parents + (int64_t)blockIdx.x * nodes;
+  uint64_t* out = masks + (int64_t)blockIdx.x * nodes * words;
+  for (int n = threadIdx.x; n < nodes; n += MASK_THREADS) s_parent[n] = p[n];
+  __syncthreads();
+  bool bad = s_parent[0] >= 0;
+  for (int i = threadIdx.x; i < nodes * words; i += MASK_THREADS) {
+    const int w = i % words;
+    uint64_t mask = 0ull;
+    int n = i / words;
+    while (n > 0) {
+      if (n >> 6 == w) mask |= 1ull << (n & 63);
+      const int up = s_parent[n];
+      bad |= up >= n;
+      n = up < n ? up : -1;
+    }
+    if (n == 0 && w == 0) mask |= 1ull;
+    out[i] = n == 0 ? mask : 0ull;  // a node that pads, or under one that does
+  }
+  if (bad) atomicOr(flag, VH_CACHE_ERR_PARENT);
+}
+
+// The splits of a row joined: their maxima give each split's weight.  D / 4
+// lanes a row; a row reads only the splits that its keys reach.
+template <int D>
+__global__ void __launch_bounds__(256) k_tree_merge(Args a) {
+  constexpr int LANES = D / 4;
+  const int64_t id = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int c = threadIdx.x % LANES * 4;
+  const int pairs = a.batch * a.c.kv_heads;
+  if (id >= (int64_t)pairs * a.rows) return;
+  const int pair = (int)(id / a.rows), row = (int)(id - (int64_t)pair * a.rows);
+  const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
+  const int total = tree::visible(a, a.context[b], row / a.block_rows * a.block_rows);
+  const int splits = (total + a.chunk - 1) / a.chunk;
+  const int64_t at = (int64_t)pair * a.splits * a.rows + row;
+  float M = -__builtin_inff();
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, a.part_ml[2 * (at + (int64_t)s * a.rows)]);
+  float L = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < splits; ++s) {
+    const int64_t p = at + (int64_t)s * a.rows;
+    const float2 ml = *(const float2*)(a.part_ml + 2 * p);
+    const float w = ml.x == -__builtin_inff() ? 1.0f : tree::exp2_fast(ml.x - M);
+    L += ml.y * w;
+    o += *(const f32x4*)(a.part_o + p * D + c) * w;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees nothing is zero
+  const int node = (int)fast_div((uint32_t)row, a.group_div);
+  const int64_t out = ((int64_t)b * a.nodes + node) * a.heads + h * a.group + row - node * a.group;
+  if (a.lse && c == 0) a.lse[out] = L == 0.0f ? -__builtin_inff() : (M + log2f(L)) * tree::LN2;
+  o *= inv;
+  *(uint2*)((uint16_t*)a.o + out * D + c) =
+      a.q_bf16 ? make_uint2(tree::pack2<CACHE_BF16>(o[0], o[1]), tree::pack2<CACHE_BF16>(o[2], o[3]))
+               : make_uint2(tree::pack2<CACHE_F16>(o[0], o[1]), tree::pack2<CACHE_F16>(o[2], o[3]));
+}
+
+struct Plan {
+  int nt, row_blocks, chunk, splits;
+  int64_t part;  // rows of partial results
+};
+
+// The shape of the launch.  Rows of a wave: as few tiles of 16 as hold them,
+// to four (two for heads of 256), where the accumulators fill the registers.
+Plan plan_of(const vh_tree_desc* d) {
+  Plan p;
+  const int64_t rows = (int64_t)d->nodes * (d->heads / d->cache.kv_heads);
+  p.nt = rows <= 16 ? 1 : rows <= 32 || d->cache.dim > 128 ? 2 : 4;
+  p.row_blocks = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
+  const int64_t keys = (int64_t)d->table_pages * d->cache.page;
+  const int64_t pairs = (int64_t)d->batch * d->cache.kv_heads;
+  const int64_t least = tree::WAVES * tree::STEP;
+  int64_t chunk = d->chunk;
+  if (chunk == 0) {
+    // as many workgroups as four for each of the 256 CUs, if a wave still has a step of its own
+    const int64_t blocks = pairs * p.row_blocks;
+    chunk = keys * blocks / 1024;
+  }
+  chunk = (chunk + least - 1) / least * least;
+  if (chunk < least) chunk = least;
+  while ((keys + chunk - 1) / chunk > MAX_SPLITS) chunk += least;
+  p.chunk = (int)chunk;
+  p.splits = (int)((keys + chunk - 1) / chunk);
+  p.part = p.splits > 1 ? pairs * p.splits * rows : 0;
+  return p;
+}
+
+int desc_check(const vh_tree_desc* d, const char* what) {
+  VH_REQUIRE(d, "%s: null descriptor", what);
+  const vh_cache& c = d->cache;
+  if (int e = vh_cache_check(&c, what)) return e;
+  VH_REQUIRE(d->dtype == VH_BF16 || d->dtype == VH_F16, "%s: queries must be bfloat16 or float16", what);
+  VH_REQUIRE(c.fmt != CACHE_F16 || d->dtype == VH_F16, "%s: float16 queries for a float16 cache", what);
+  VH_REQUIRE(c.fmt != CACHE_BF16 || d->dtype == VH_BF16, "%s: bfloat16 queries for a bfloat16 cache", what);
+  VH_REQUIRE(c.dim == 64 || c.dim == 128 || c.dim == 256, "%s: heads of 64, 128 or 256 (got %d)", what, c.dim);
+  VH_REQUIRE(c.page % 16 == 0, "%s: pages of a multiple of 16 tokens (got %d)", what, c.page);
+  VH_REQUIRE(d->batch >= 0 && d->nodes >= 0 && d->table_pages >= 0, "%s: negative size", what);
+  VH_REQUIRE(d->heads > 0 && d->heads % c.kv_heads == 0, "%s: query heads must be a multiple of the cache's", what);
+  VH_REQUIRE((int64_t)d->nodes * (d->heads / c.kv_heads) < (1 << 24), "%s: too many rows", what);
+  VH_REQUIRE((int64_t)d->table_pages * c.page < (1ll << 31) - 4096, "%s: too many pages", what);
+  VH_REQUIRE((int64_t)d->batch * c.kv_heads < (1 << 20), "%s: too many sequences", what);
+  VH_REQUIRE(!d->masks || d->nodes <= MAX_NODES, "%s: at most %d nodes", what, MAX_NODES);
+  VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
+  VH_REQUIRE(d->chunk >= 0, "%s: bad chunk", what);
+  return VH_OK;
+}
+
+}  // namespace
+
+extern "C" int vh_tree_masks(const int32_t* parents, int64_t batch, int32_t nodes, uint64_t* masks, int32_t* flag,
+                             vh_stream_t stream) {
+  VH_REQUIRE(batch >= 0 && batch < (1ll << 31) && nodes >= 0 && nodes <= MAX_NODES,
+             "vh_tree_masks: at most %d nodes (got %d)", MAX_NODES, nodes);
+  if (batch == 0 || nodes == 0) return VH_OK;
+  VH_REQUIRE(parents && masks && flag, "vh_tree_masks: null argument");
+  hipLaunchKernelGGL(k_tree_masks, dim3((unsigned)batch), dim3(MASK_THREADS), 0, vh::as_stream(stream), parents, nodes,
+                     (nodes + 63) / 64, masks, flag);
+  return vh::check_launch("vh_tree_masks");
+}
+
+extern "C" int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* d) {
+  if (desc_check(d, "vh_tree_attention_workspace_bytes")) return -1;
+  if (d->batch == 0 || d->nodes == 0) return 0;
+  return plan_of(d).part * (int64_t)sizeof(float) * (d->cache.dim + 2);
+}
+
+extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
+  if (int e = desc_check(d, "vh_tree_attention")) return e;
+  if (d->batch == 0 || d->nodes == 0) return VH_OK;
+  VH_REQUIRE(d->q && d->context && d->o && (d->table || d->table_pages == 0), "vh_tree_attention: null argument");
+  VH_REQUIRE((uintptr_t)d->o % 16 == 0, "vh_tree_attention: misaligned output");
+  const Plan p = plan_of(d);
+  const int64_t need = p.part * (int64_t)sizeof(float) * (d->cache.dim + 2);
+  VH_REQUIRE(need == 0 || (d->work && d->work_bytes >= need && (uintptr_t)d->work % 16 == 0),
+             "vh_tree_attention: needs %lld bytes of aligned workspace", (long long)need);
+  const int group = d->heads / d->cache.kv_heads;
+  Args a{};
+  a.c = d->cache;
+  a.q = d->q;
+  a.q_sb = d->q_sb;
+  a.q_st = d->q_st;
+  a.q_sh = d->q_sh;
+  a.table = d->table;
+  a.table_st = d->table_st;
+  a.context = d->context;
+  a.masks = d->masks;
+  a.o = d->o;
+  a.lse = d->lse;
+  a.part_o = (float*)d->work;
+  a.part_ml = a.part_o + p.part * d->cache.dim;
+  a.group_div = make_fast_div((uint32_t)group);
+  a.page_div = make_fast_div((uint32_t)(d->cache.page / 16));
+  a.scale = d->scale * tree::LOG2E;
+  a.q_bf16 = d->dtype == VH_BF16;
+  a.q_wide = (uintptr_t)d->q % 16 == 0 && d->q_sb % 8 == 0 && d->q_st % 8 == 0 && d->q_sh % 8 == 0;
+  a.words = (d->nodes + 63) / 64;
+  a.batch = d->batch;
+  a.nodes = d->nodes;
+  a.heads = d->heads;
+  a.group = group;
+  a.rows = d->nodes * group;
+  a.row_blocks = p.row_blocks;
+  a.block_rows = 16 * p.nt;
+  a.table_pages = d->table_pages;
+  a.chunk = p.chunk;
+  a.splits = p.splits > 0 ? p.splits : 1;
+  VH_REQUIRE(((int64_t)a.splits * a.batch * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31),
+             "vh_tree_attention: too many workgroups");
+  hipStream_t s = vh::as_stream(stream);
+  const int rc = d->cache.dim == 64 ? tree::launch<64>(a, p.nt, s)
+                 : d->cache.dim == 128 ? tree::launch<128>(a, p.nt, s)
+                                       : tree::launch<256>(a, p.nt, s);
+  if (rc != VH_OK || a.splits == 1) return rc;
+  const int64_t lanes = (int64_t)a.batch * a.c.kv_heads * a.rows * (d->cache.dim / 4);
+  const dim3 grid((unsigned)((lanes + 255) / 256));
+  if (d->cache.dim == 64) hipLaunchKernelGGL(k_tree_merge<64>, grid, dim3(256), 0, s, a);
+  else if (d->cache.dim == 128) hipLaunchKernelGGL(k_tree_merge<128>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_tree_merge<256>, grid, dim3(256), 0, s, a);
+  return vh::check_launch("vh_tree_attention");
+}

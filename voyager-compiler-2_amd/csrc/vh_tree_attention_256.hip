@@ -1,0 +1,9 @@
+// Attention of a tree of tokens over a paged cache, heads of 256.
+#include "vh_tree_attention.h"
+
+namespace tree {
+template <>
+int launch<256>(const Args& a, int nt, hipStream_t s) {
+  return launch_d<256>(a, nt, s);
+}
+}  // namespace tree

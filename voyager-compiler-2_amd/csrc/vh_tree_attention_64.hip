@@ -1,0 +1,9 @@
+// Attention of a tree of tokens over a paged cache, heads of 64.
+#include "vh_tree_attention.h"
+
+namespace tree {
+template <>
+int launch<64>(const Args& a, int nt, hipStream_t s) {
+  return launch_d<64>(a, nt, s);
+}
+}  // namespace tree

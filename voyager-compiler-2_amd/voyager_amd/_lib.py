@@ -73,6 +73,18 @@ class Param(ctypes.Structure):
     ]
 
 
+class Cache(ctypes.Structure):
+    """``vh_cache``: keys and values in pages."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("flag", ctypes.c_void_p),
+        ("slots", ctypes.c_int64), ("pages", ctypes.c_int64),
+        ("page", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("fmt", ctypes.c_int32),
+    ]
+
+
 class Codebook(ctypes.Structure):
     """``vh_codebook``: codebook tables under a region grid."""
 
@@ -179,6 +191,18 @@ _SIGNATURES = {
     "vh_slice_csr": ([_P, _I32, _P, _P, _I64, _I64, _I32, _I64, _I64, _I64, _P, _P, _P, _P], _I32),
     "vh_spmm_csr": ([_P, _I32, _P, _P, _I64, _I64, _I64, _P, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _P],
                     _I32),
+    # a step with drafted tokens
+    "vh_rope": ([_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I64, _I64, _I32, _I32, _I32, _I32, _I32,
+                 _P, _I32, _I64, _I64, _P, _F32, _I32, _P], _I32),
+    "vh_paged_write": ([ctypes.POINTER(Cache), _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _P], _I32),
+    "vh_paged_read": ([ctypes.POINTER(Cache), _P, _P, _I32, _P, _I64, _P], _I32),
+    "vh_paged_keep": ([ctypes.POINTER(Cache), _P, _I64, _I32, _P, _P, _I64, _P, _I64, _I32, _P], _I32),
+    "vh_tree_masks": ([_P, _I64, _I32, _P, _P, _P], _I32),
+    # vh_tree_attention takes a vh_tree_desc*; voyager_amd.speculative.TreeDesc mirrors it.
+    "vh_tree_attention": ([_P, _P], _I32),
+    "vh_tree_attention_workspace_bytes": ([_P], _I64),
+    "vh_verify": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I32, _I64, _P, _P, _P, _P, _I64, _P], _I32),
+    "vh_verify_workspace_bytes": ([_I64, _I64], _I64),
 }
 
 DECODE_ERR_FP16_RANGE = 1
@@ -186,6 +210,9 @@ DECODE_ERR_WEIGHT_RANGE = 2
 DECODE_ERR_KV_CODE = 4
 DECODE_ERR_KV_FULL = 8
 DECODE_ERR_KV_STATE = 16
+CACHE_E4M3, CACHE_INT8, CACHE_F16, CACHE_BF16 = range(4)
+CACHE_ERR_SLOT, CACHE_ERR_PAGE, CACHE_ERR_CONTEXT, CACHE_ERR_PARENT = 1, 2, 4, 8
+TREE_MAX_NODES = 1024
 KIVI_RES_CAP = 128
 FILTER_NOALLOC_SCRATCH_BYTES = 8 << 20
 GEMV_STORE, GEMV_RESIDUAL, GEMV_SWIGLU = 0, 1, 2

@@ -1,0 +1,171 @@
+"""A step that verifies drafted tokens: a tree of them attends to a sequence's
+cache at once, and given random numbers say which are kept.
+
+* :class:`Tree`: the drafted tokens of each sequence as a tree;
+* :func:`tree_attention`: attention of its nodes over the paged cache (one
+  node, or a chain of prompt tokens, is a tree as well);
+* :func:`verify`: the drafted tokens against the target's probabilities.
+
+Kept rows are then moved together by :meth:`paged.PagedCache.keep`.  Nothing
+synchronises and every launch goes on torch's current stream.
+"""
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check, load, stream_on
+from .paged import CacheFlag, PagedCache, _int32, _rows
+
+MAX_NODES = _lib.TREE_MAX_NODES
+
+
+class TreeDesc(ctypes.Structure):
+    """``vh_tree_desc``."""
+
+    _fields_ = [
+        ("cache", _lib.Cache),
+        ("q", ctypes.c_void_p), ("q_sb", ctypes.c_int64), ("q_st", ctypes.c_int64), ("q_sh", ctypes.c_int64),
+        ("table", ctypes.c_void_p), ("table_st", ctypes.c_int64),
+        ("context", ctypes.c_void_p), ("masks", ctypes.c_void_p),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("nodes", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32), ("chunk", ctypes.c_int32),
+    ]
+
+
+class Tree:
+    """Trees of tokens, one a sequence.  ``parents [batch, nodes]`` (int32, on
+    the GPU): the node each node follows, which comes before it, and -1 for the
+    first, the sequence's last kept token.  Another node with a negative parent
+    pads its tree: it sees nothing and is never taken, nor is one under it.
+    At most 1024 nodes.  Parents on the GPU are not read on the host: a
+    node whose parent is not before it is taken as padding, and :meth:`check`
+    raises."""
+
+    def __init__(self, parents: torch.Tensor):
+        if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_cuda:
+            raise ValueError(f"Tree: parents must be int32 [batch, nodes] on the GPU (got {parents.dtype} "
+                             f"{list(parents.shape)} on {parents.device})")
+        self.batch, self.nodes = parents.shape
+        if not 1 <= self.nodes <= MAX_NODES:
+            raise ValueError(f"Tree: 1 to {MAX_NODES} nodes (got {self.nodes})")
+        self.parents = parents.contiguous()
+        self.device = parents.device
+        self.flag = CacheFlag(parents.device)
+        #: bit m of word m // 64: node m is on the way from the root to the node (itself included)
+        self.masks = torch.empty(self.batch, self.nodes, -(-self.nodes // 64), dtype=torch.int64, device=parents.device)
+        st = load().vh_tree_masks(self.parents.data_ptr(), self.batch, self.nodes, self.masks.data_ptr(),
+                                  self.flag.t.data_ptr(), stream_on(parents.device))
+        check(st, "vh_tree_masks")
+
+    def check(self) -> None:
+        """Synchronising: raise if a node's parent is not before it."""
+        self.flag.check("Tree")
+
+
+def tree_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, context: torch.Tensor,
+                   tree: Optional[Tree] = None, *, scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of ``q [batch, nodes, heads, dim]`` (the cache's dtype) over
+    each sequence's ``context [batch]`` (int32) cached positions and its tree's
+    nodes, whose keys and values have been written at positions ``context +
+    n``; ``table [batch, pages]`` (int32) names a sequence's pages in order and
+    has room for both.  A node sees the context, itself and the nodes on its
+    way from the root; without a ``tree``, all nodes before it (a prompt, or
+    one token).  ``heads`` is a multiple of the cache's.  ``scale`` defaults to
+    ``dim ** -0.5``.
+
+    Returns the output, contiguous, of q's dtype, and with ``return_lse`` also
+    the logarithm of each row's sum of exponentials (float32 ``[batch, nodes,
+    heads]``).  Rows that see nothing give 0 and -inf.  Heads of 64, 128 or 256
+    channels, pages of a multiple of 16 tokens.  No gradient: it reads a cache."""
+    if q.dim() != 4 or q.shape[3] != cache.dim or q.dtype != cache.dtype or q.device != cache.device:
+        raise ValueError(f"tree_attention: q must be {cache.dtype} [batch, nodes, heads, {cache.dim}] on {cache.device} "
+                         f"(got {q.dtype} {list(q.shape)} on {q.device})")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("tree_attention: passes no gradient; call it under torch.no_grad()")
+    b, t, heads, dim = q.shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"tree_attention: {heads} query heads over {cache.kv_heads} of the cache")
+    _int32(context, (b,), cache.device, "tree_attention: context")
+    _int32(table, (b, table.shape[-1]), cache.device, "tree_attention: table")
+    if tree is not None and (tree.batch != b or tree.nodes != t or tree.device != cache.device):
+        raise ValueError(f"tree_attention: a tree of [{tree.batch}, {tree.nodes}] on {tree.device} for queries [{b}, {t}]")
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    table, context = _rows(table), _rows(context)
+    o = torch.empty(b, t, heads, dim, dtype=q.dtype, device=q.device)
+    lse = torch.empty(b, t, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    sb, st, sh, _ = q.stride()
+    d = TreeDesc(cache.c, q.data_ptr(), sb, st, sh, table.data_ptr(), table.stride(0), context.data_ptr(),
+                 None if tree is None else tree.masks.data_ptr(), o.data_ptr(), None if lse is None else lse.data_ptr(),
+                 None, 0, dim ** -0.5 if scale is None else float(scale), cache._dtype_code, b, t, heads,
+                 table.shape[1], 0)
+    ref = ctypes.byref(d)
+    lib = load()
+    need = lib.vh_tree_attention_workspace_bytes(ref)
+    if need > 0:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        d.work, d.work_bytes = work.data_ptr(), need
+    rc = lib.vh_tree_attention(ref, stream_on(q.device))
+    if rc:
+        check(rc, "vh_tree_attention")
+    return (o, lse) if return_lse else o
+
+
+def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tensor, r: torch.Tensor,
+           draft: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The drafted ``tokens [batch, nodes]`` (int64; the first node's is the
+    last kept token and is not read) against ``target [batch, nodes, vocab]``
+    (float32), the target's probabilities after each node.
+
+    From the first node on, a node's children are tried in order: child n of
+    token x is taken if ``u[n] * mass * draft(x) < rest(x)``, where rest begins
+    as the target's row and mass as 1; if not, ``rest = max(rest - mass *
+    draft, 0)`` and mass is its sum.  ``draft [batch, nodes, vocab]``: the draft
+    model's probabilities after each node, from which its children were sampled;
+    None: the children were chosen (a draft's best tokens), so draft(x) is 1 for
+    the child's own token and rest loses it.  Where no child is taken, the last
+    token is drawn from rest by ``r``: the first index at which its running sum
+    passes r times the whole.  The tokens then follow the target's distribution
+    for ``u [batch, nodes]`` and ``r [batch]`` uniform in [0, 1) (float32).
+
+    Returns ``told [batch, nodes]`` (int64: the tokens taken, then the last; -1
+    after them), ``path [batch, nodes]`` (int32: the first node and those taken;
+    -1 after them) and ``count [batch]`` (int32: how many of each)."""
+    b, t = tree.batch, tree.nodes
+    dev = tree.device
+    for name, x in (("target", target), ("draft", draft)):
+        if x is None:
+            continue
+        if x.dim() != 3 or x.shape[:2] != (b, t) or x.shape != target.shape or x.dtype != torch.float32 or x.device != dev:
+            raise ValueError(f"verify: {name} must be float32 [{b}, {t}, vocab] on {dev} (got {x.dtype} {list(x.shape)} on "
+                             f"{x.device})")
+    if target.shape[2] == 0:
+        raise ValueError("verify: an empty vocabulary")
+    for name, x, shape, dtype in (("tokens", tokens, (b, t), torch.int64), ("u", u, (b, t), torch.float32),
+                                  ("r", r, (b,), torch.float32)):
+        if x.dtype != dtype or x.shape != shape or x.device != dev:
+            raise ValueError(f"verify: {name} must be {dtype} {list(shape)} on {dev} (got {x.dtype} {list(x.shape)} on "
+                             f"{x.device})")
+    target = _rows(target)
+    draft = None if draft is None else _rows(draft)
+    tokens, u, r = tokens.contiguous(), u.contiguous(), r.contiguous()
+    told = torch.empty(b, t, dtype=torch.int64, device=dev)
+    path = torch.empty(b, t, dtype=torch.int32, device=dev)
+    count = torch.empty(b, dtype=torch.int32, device=dev)
+    lib = load()
+    need = lib.vh_verify_workspace_bytes(b, target.shape[2])
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    ds = (0, 0) if draft is None else draft.stride()
+    st = lib.vh_verify(target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(),
+                       ds[0], ds[1], tree.parents.data_ptr(), tokens.data_ptr(), u.data_ptr(), r.data_ptr(), b, t,
+                       target.shape[2], told.data_ptr(), path.data_ptr(), count.data_ptr(), work.data_ptr(),
+                       work.numel(), stream_on(dev))
+    if st:
+        check(st, "vh_verify")
+    return told, path, count
