@@ -47,12 +47,16 @@ __global__ void __launch_bounds__(MASK_THREADS) k_tree_masks(const int32_t* pare
   if (bad) atomicOr(flag, VH_CACHE_ERR_PARENT);
 }
 
-// The splits of a row joined: their maxima give each split's weight.  D / 4
-// lanes a row; a row reads only the splits that its keys reach.
-template <int D>
+// The splits of a row joined: D / 4 lanes hold the row's channels, `GROUPS`
+// of them take turns along the splits, and a row reads only the splits that
+// its keys reach.
+template <int D, int GROUPS>
 __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
-  constexpr int LANES = D / 4;
-  const int64_t id = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = D / 4, ROWS = 256 / (LANES * GROUPS);
+  __shared__ f32x4 s_o[GROUPS > 1 ? 256 : 1];
+  __shared__ float2 s_ml[GROUPS > 1 ? GROUPS : 1];
+  const int group = GROUPS > 1 ? threadIdx.x / LANES : 0;
+  const int64_t id = (int64_t)blockIdx.x * ROWS + (GROUPS > 1 ? 0 : threadIdx.x / LANES);
   const int c = threadIdx.x % LANES * 4;
   const int pairs = a.batch * a.c.kv_heads;
   if (id >= (int64_t)pairs * a.rows) return;
@@ -61,16 +65,51 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
   const int total = tree::visible(a, a.context[b], row / a.block_rows * a.block_rows);
   const int splits = (total + a.chunk - 1) / a.chunk;
   const int64_t at = (int64_t)pair * a.splits * a.rows + row;
-  float M = -__builtin_inff();
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, a.part_ml[2 * (at + (int64_t)s * a.rows)]);
-  float L = 0.0f;
+  float M = -__builtin_inff(), L = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < splits; ++s) {
-    const int64_t p = at + (int64_t)s * a.rows;
-    const float2 ml = *(const float2*)(a.part_ml + 2 * p);
-    const float w = ml.x == -__builtin_inff() ? 1.0f : tree::exp2_fast(ml.x - M);
-    L += ml.y * w;
-    o += *(const f32x4*)(a.part_o + p * D + c) * w;
+  // four splits at a time, so that their reads overlap
+  for (int s0 = group; s0 < splits; s0 += 4 * GROUPS) {
+    float2 ml[4];
+    f32x4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + k * GROUPS;
+      const int64_t p = at + (int64_t)(s < splits ? s : s0) * a.rows;
+      ml[k] = *(const float2*)(a.part_ml + 2 * p);
+      x[k] = *(const f32x4*)(a.part_o + p * D + c);
+      if (s >= splits) {
+        ml[k] = make_float2(-__builtin_inff(), 0.0f);
+        x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    }
+    const float to = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M);
+    const float keep = M == -__builtin_inff() ? 1.0f : tree::exp2_fast(M - to);
+    M = to;
+    L *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = ml[k].x == -__builtin_inff() ? 1.0f : tree::exp2_fast(ml[k].x - M);
+      L += ml[k].y * w;
+      o += x[k] * w;
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    s_o[threadIdx.x] = o;
+    if (c == 0) s_ml[group] = make_float2(M, L);
+    __syncthreads();
+    if (group > 0) return;
+    M = -__builtin_inff();
+    L = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) M = fmaxf(M, s_ml[k].x);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      const float w = s_ml[k].x == -__builtin_inff() ? 1.0f : tree::exp2_fast(s_ml[k].x - M);
+      L += s_ml[k].y * w;
+      o += s_o[k * LANES + threadIdx.x] * w;
+    }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees nothing is zero
   const int node = (int)fast_div((uint32_t)row, a.group_div);
@@ -82,17 +121,26 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
                : make_uint2(tree::pack2<CACHE_F16>(o[0], o[1]), tree::pack2<CACHE_F16>(o[2], o[3]));
 }
 
+// Many splits: a workgroup a row.  Few: as many rows as fit one.
+template <int D>
+void merge(const Args& a, hipStream_t s) {
+  constexpr int ALL = 1024 / D;  // groups of lanes in a workgroup
+  const int64_t rows = (int64_t)a.batch * a.c.kv_heads * a.rows;
+  if (a.splits > 4) hipLaunchKernelGGL((k_tree_merge<D, ALL>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_tree_merge<D, 1>), dim3((unsigned)((rows + ALL - 1) / ALL)), dim3(256), 0, s, a);
+}
+
 struct Plan {
   int nt, row_blocks, chunk, splits;
   int64_t part;  // rows of partial results
 };
 
-// The shape of the launch.  Rows of a wave: as few tiles of 16 as hold them,
-// to four (two for heads of 256), where the accumulators fill the registers.
+// The shape of the launch.  Rows of a wave: 16, or 32 where there are more and
+// their accumulators leave two waves a SIMD (heads of 64 and 128).
 Plan plan_of(const vh_tree_desc* d) {
   Plan p;
   const int64_t rows = (int64_t)d->nodes * (d->heads / d->cache.kv_heads);
-  p.nt = rows <= 16 ? 1 : rows <= 32 || d->cache.dim > 128 ? 2 : 4;
+  p.nt = rows <= 16 || d->cache.dim > 128 ? 1 : 2;
   p.row_blocks = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
   const int64_t keys = (int64_t)d->table_pages * d->cache.page;
   const int64_t pairs = (int64_t)d->batch * d->cache.kv_heads;
@@ -191,17 +239,16 @@ extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
   a.table_pages = d->table_pages;
   a.chunk = p.chunk;
   a.splits = p.splits > 0 ? p.splits : 1;
-  VH_REQUIRE(((int64_t)a.splits * a.batch * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31),
+  VH_REQUIRE(((int64_t)a.splits * a.batch * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31) &&
+                 (int64_t)a.batch * a.c.kv_heads * a.rows < (1ll << 31),
              "vh_tree_attention: too many workgroups");
   hipStream_t s = vh::as_stream(stream);
   const int rc = d->cache.dim == 64 ? tree::launch<64>(a, p.nt, s)
                  : d->cache.dim == 128 ? tree::launch<128>(a, p.nt, s)
                                        : tree::launch<256>(a, p.nt, s);
   if (rc != VH_OK || a.splits == 1) return rc;
-  const int64_t lanes = (int64_t)a.batch * a.c.kv_heads * a.rows * (d->cache.dim / 4);
-  const dim3 grid((unsigned)((lanes + 255) / 256));
-  if (d->cache.dim == 64) hipLaunchKernelGGL(k_tree_merge<64>, grid, dim3(256), 0, s, a);
-  else if (d->cache.dim == 128) hipLaunchKernelGGL(k_tree_merge<128>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(k_tree_merge<256>, grid, dim3(256), 0, s, a);
+  if (d->cache.dim == 64) merge<64>(a, s);
+  else if (d->cache.dim == 128) merge<128>(a, s);
+  else merge<256>(a, s);
   return vh::check_launch("vh_tree_attention");
 }

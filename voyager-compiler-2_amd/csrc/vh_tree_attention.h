@@ -114,17 +114,43 @@ VH_DEV uint32_t nonfinite(uint32_t w) {
   return ((w & e) == e ? 0xffffu : 0u) | (((w >> 16) & e) == e ? 0xffff0000u : 0u);
 }
 
+// Over the four lanes that hold a row, 16 apart, by register swaps: rows of
+// 16 lanes, then halves of the wave.
 VH_DEV float max_rows(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const uint32_t u = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 VH_DEV float sum_rows(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  const uint32_t u = __float_as_uint(v);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The other side of a branch that scales the accumulators: no instructions,
+// but a definition of its own, so that both sides keep them in place (without
+// it the compiler copies all of them before each such branch).
+template <int CT, int NT>
+VH_DEV void stay(f32x4 (&acc)[CT][NT]) {
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(acc[c][nt]));
+}
+
+// Waves of a SIMD that the registers are shared out for: two at least, so that
+// accumulators stay where vector instructions reach them (under 256 registers
+// a wave), three where a wave's 16 rows of 8-bit keys leave room.
+constexpr int waves_of(int d, int fmt, int nt) {
+  return nt > 1 || d > 128 ? 2 : fmt == CACHE_E4M3 || fmt == CACHE_INT8 || d == 64 ? 3 : 2;
 }
 
 template <int D, int FMT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
+__global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args a) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
   constexpr int ESZ = BYTE ? 1 : 2;
   constexpr int KS = D / 32;                        // matrix instructions along D
@@ -151,7 +177,8 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
   const int begin = split * a.chunk;
   if (begin >= total && a.splits > 1) return;
   const int end = begin + a.chunk < total ? begin + a.chunk : total;
-  const int32_t* table = a.table + (int64_t)b * a.table_st;
+  // read through the scalar cache: its waits are apart from those for keys and values
+  const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.table + (int64_t)b * a.table_st);
 
   // the queries, as the B operand: column r is a row, k the lane's share of D
   uint4 Q[NT][KS];
@@ -217,51 +244,68 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
   uint4 kr[2][KQ];
   uint32_t vr[2][4][VB][VW];
   f32x4 ks[2], vs[2];
-  int live[2];  // keys of each tile that exist
+  // A lane's part of a tile's rows: keys at r, channels from 16 g bytes on;
+  // values at 4 g + i, channels from r CPL on.
+  const uint32_t k_lane = (uint32_t)r * (D * ESZ) + g * 16, v_lane = (uint32_t)(4 * g) * (D * ESZ) + r * (CPL * ESZ);
 
-  for (int key0 = begin + wave * STEP; key0 < end; key0 += WAVES * STEP) {
+  // Where a step's two tiles lie, and how many of their keys exist.
+  struct Step {
     int64_t row[2];
+    int live[2];
+  };
+  const int64_t page_rows = (int64_t)a.c.kv_heads * a.c.page, head_rows = (int64_t)h * a.c.page;
+  const uint32_t pages = (uint32_t)a.c.pages;
+  auto find = [&](int key0) __attribute__((always_inline)) {
+    Step st;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = key0 + 16 * t;
-      live[t] = end - key < 0 ? 0 : end - key < 16 ? end - key : 16;
-      const uint32_t tile = (uint32_t)(live[t] ? key : key0) >> 4;
+      const int left = end - (key0 + 16 * t);
+      const uint32_t tile = ((uint32_t)key0 >> 4) + (left > 0 ? t : 0);
       const uint32_t pg = fast_div(tile, a.page_div);
-      int id = __builtin_amdgcn_readfirstlane(table[pg]);
-      if (id < 0 || id >= a.c.pages) {  // nothing there is seen
-        bad_page = true;
-        id = 0;
-        live[t] = 0;
-      }
-      row[t] = ((int64_t)id * a.c.kv_heads + h) * a.c.page + (tile * 16 - pg * (uint32_t)a.c.page);
+      const int id = table[pg];
+      const bool there = (uint32_t)id < pages;  // if not, nothing of it is seen
+      bad_page |= !there;
+      st.live[t] = !there || left < 0 ? 0 : left < 16 ? left : 16;
+      st.row[t] = (there ? id : 0) * page_rows + head_rows + (tile * 16 - pg * (uint32_t)a.c.page);
     }
+    return st;
+  };
+  auto load_k = [&](const Step& st) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* kp = (const uint8_t*)a.c.k + (row[t] + r) * (D * ESZ) + g * 16;
+      const uint8_t* kp = (const uint8_t*)a.c.k + st.row[t] * (D * ESZ);
 #pragma unroll
-      for (int j = 0; j < KQ; ++j) kr[t][j] = *(const uint4*)(kp + 64 * j);
-      if constexpr (BYTE) {
-        ks[t] = *(const f32x4*)(a.c.k_scale + row[t] + 4 * g);
-        vs[t] = *(const f32x4*)(a.c.v_scale + row[t] + 4 * g);
-      }
+      for (int j = 0; j < KQ; ++j) kr[t][j] = *(const uint4*)(kp + k_lane + 64 * j);
+      if constexpr (BYTE) ks[t] = *(const f32x4*)(a.c.k_scale + st.row[t] + 4 * g);
+    }
+  };
+  auto load_v = [&](const Step& st) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* vp = (const uint8_t*)a.c.v + (row[t] + 4 * g + i) * (D * ESZ) + r * (CPL * ESZ);
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* vp = (const uint8_t*)a.c.v + st.row[t] * (D * ESZ);
+      if constexpr (BYTE) vs[t] = *(const f32x4*)(a.c.v_scale + st.row[t] + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int w = 0; w < VB; ++w) {
+          const uint8_t* at = vp + v_lane + i * (D * ESZ) + w * (16 * CPL * ESZ);
           if constexpr (VW == 4) {
-            const uint4 x = *(const uint4*)(vp + 256 * w);
+            const uint4 x = *(const uint4*)at;
             vr[t][i][w][0] = x.x; vr[t][i][w][1] = x.y; vr[t][i][w][2] = x.z; vr[t][i][w][3] = x.w;
           } else if constexpr (VW == 2) {
-            const uint2 x = *(const uint2*)(vp + 128 * w);
+            const uint2 x = *(const uint2*)at;
             vr[t][i][w][0] = x.x; vr[t][i][w][1] = x.y;
           } else {
-            vr[t][i][w][0] = *(const uint32_t*)(vp + 64 * w);
+            vr[t][i][w][0] = *(const uint32_t*)at;
           }
         }
-      }
     }
+  };
 
+  // One step of 32 keys; `st` is it, `next` the one whose keys and values are
+  // asked for as soon as this step's registers are free.
+  auto step = [&](auto is_masked, int key0, const Step& st, const Step& next) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(is_masked)::value;
     // scores: S[t][nt][i] of key 16 t + 4 g + i and row 16 nt + r
     f32x4 S[2][NT];
 #pragma unroll
@@ -293,9 +337,11 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
         for (int nt = 0; nt < NT; ++nt) S[t][nt] *= ks[t];
       }
     }
-    const bool masked = key0 + STEP > ctx || live[0] + live[1] < STEP;
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(next);
+    __builtin_amdgcn_sched_barrier(0);
     uint32_t seen[NT];  // the lane's keys (bit 4 t + i) that its row sees
-    if (masked) {
+    if constexpr (MASKED) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         seen[nt] = 0u;
@@ -304,13 +350,13 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at = 4 * g + i, n = key0 + 16 * t + at - ctx;  // n: the key's node, if it is one
-            bool ok = at < live[t];
+            bool ok = at < st.live[t];
             if (ok && n >= 0) {
               if (a.masks) ok = n < a.nodes && (a.masks[((int64_t)b * a.nodes + node[nt]) * a.words + (n >> 6)] >> (n & 63) & 1);
               else ok = n <= node[nt];
             }
-            if (ok) seen[nt] |= 1u << (4 * t + i);
-            else S[t][nt][i] = -__builtin_inff();
+            seen[nt] |= ok ? 1u << (4 * t + i) : 0u;
+            S[t][nt][i] = ok ? S[t][nt][i] : -__builtin_inff();
           }
       }
     }
@@ -321,11 +367,11 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
     bool grow = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float v = -__builtin_inff();
+      float v = fmaxf(S[0][nt][0], S[0][nt][1]);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v = fmaxf(v, S[t][nt][i]);
+        for (int i = t ? 0 : 2; i < 4; i += 2) v = fmaxf(fmaxf(v, S[t][nt][i]), S[t][nt][i + 1]);
       mx[nt] = max_rows(v) * fac[nt];
       grow |= mx[nt] > m[nt] + 8.0f;
     }
@@ -339,6 +385,8 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[c][nt] *= alpha;
       }
+    } else {
+      stay(acc);
     }
     f32x4 vn[2];
     if constexpr (BYTE) {
@@ -346,19 +394,21 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, vs[t][i]);
+        for (int i = 0; i < 4; i += 2) top = fmaxf(fmaxf(top, vs[t][i]), vs[t][i + 1]);
       top = fminf(max_rows(top), 0x1p125f);  // the next power of two stays finite
       top = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(top)));
       if (top > T) {
         const float to = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
-        const float down = T / to;
+        const float down = T * __uint_as_float(0x7f000000u - __float_as_uint(to));  // T / to, both powers of two
         T = to;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < CT; ++c) acc[c][nt] *= down;
+      } else {
+        stay(acc);
       }
-      const float inv = 1.0f / T;
+      const float inv = __uint_as_float(0x7f000000u - __float_as_uint(T));  // 1 / T
 #pragma unroll
       for (int t = 0; t < 2; ++t) vn[t] = vs[t] * inv;
     }
@@ -378,7 +428,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
           if constexpr (BYTE) {
             p0 *= vn[t][i];
             p1 *= vn[t][i + 1];
-            if (masked) {  // a scale there may be anything
+            if constexpr (MASKED) {  // a scale there may be anything
               p0 = seen[nt] >> (4 * t + i) & 1 ? p0 : 0.0f;
               p1 = seen[nt] >> (4 * t + i + 1) & 1 ? p1 : 0.0f;
             }
@@ -388,7 +438,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
             const f32x2 hi = unpack2<FMT>(w[2 * t + i / 2]);
             u[2 * t + i / 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
           }
-          if constexpr (!BYTE) {
+          if constexpr (!BYTE && MASKED) {
             S[t][nt][i] = p0;
             S[t][nt][i + 1] = p1;
           }
@@ -399,42 +449,40 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
 
     // Values that are not finite would reach rows that do not see them as 0 *
     // inf: in steps with a mask they are taken out and added to the rows that do.
-    if constexpr (!BYTE) {
-      if (masked) {
-        uint32_t any = 0u;
+    if constexpr (!BYTE && MASKED) {
+      uint32_t any = 0u;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int w = 0; w < VB; ++w)
+          for (int w = 0; w < VB; ++w)
 #pragma unroll
-              for (int d = 0; d < VW; ++d) {
-                const uint32_t bits = nonfinite<FMT>(vr[t][i][w][d]);
-                any |= bits;
-                vr[t][i][w][d] &= ~bits;
-              }
-        if (__any(any != 0u)) {
-          for (int k = 0; k < STEP; ++k) {
-            const int t = k >> 4, at = k & 15;
-            const uint16_t* v = (const uint16_t*)a.c.v + ((t ? row[1] : row[0]) + at) * D;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float mine = 0.0f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if ((at & 3) == i) mine = t ? S[1][nt][i] : S[0][nt][i];
-              const int from = (at >> 2) * 16 + r;
-              const float p = __shfl(mine, from);
-              const bool ok = (uint32_t)__shfl((int)seen[nt], from) >> (4 * t + (at & 3)) & 1;
-#pragma unroll
-              for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint32_t x = v[(c / CPL) * 16 * CPL + (4 * g + i) * CPL + c % CPL];
-                  if (ok && nonfinite<FMT>(x) & 0xffffu) acc[c][nt][i] += p * unpack2<FMT>(x)[0];
-                }
+            for (int d = 0; d < VW; ++d) {
+              const uint32_t bits = nonfinite<FMT>(vr[t][i][w][d]);
+              any |= bits;
+              vr[t][i][w][d] &= ~bits;
             }
+      if (__any(any != 0u)) {
+        for (int k = 0; k < STEP; ++k) {
+          const int t = k >> 4, at = k & 15;
+          const uint16_t* v = (const uint16_t*)a.c.v + ((t ? st.row[1] : st.row[0]) + at) * D;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((at & 3) == i) mine = t ? S[1][nt][i] : S[0][nt][i];
+            const int from = (at >> 2) * 16 + r;
+            const float p = __shfl(mine, from);
+            const bool ok = (uint32_t)__shfl((int)seen[nt], from) >> (4 * t + (at & 3)) & 1;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t x = v[(c / CPL) * 16 * CPL + (4 * g + i) * CPL + c % CPL];
+                if (ok && nonfinite<FMT>(x) & 0xffffu) acc[c][nt][i] += p * unpack2<FMT>(x)[0];
+              }
           }
         }
       }
@@ -444,55 +492,69 @@ __global__ void __launch_bounds__(WAVES * 64) k_tree(Args a) {
 #pragma unroll
     for (int w = 0; w < VB; ++w)
 #pragma unroll
-      for (int d = 0; d < VW; ++d) {
-        if constexpr (BYTE) {
-          uint32_t x[2][4];  // per tile and channel of the dword: four keys, a byte each
+      for (int d = 0; d < VW; ++d)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint32_t r0 = vr[t][0][w][d], r1 = vr[t][1][w][d], r2 = vr[t][2][w][d], r3 = vr[t][3][w][d];
-            const uint32_t p0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), p1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-            const uint32_t p2 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), p3 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-            x[t][0] = __builtin_amdgcn_perm(p2, p0, 0x05040100u);
-            x[t][1] = __builtin_amdgcn_perm(p2, p0, 0x07060302u);
-            x[t][2] = __builtin_amdgcn_perm(p3, p1, 0x05040100u);
-            x[t][3] = __builtin_amdgcn_perm(p3, p1, 0x07060302u);
-          }
+        for (int e = 0; e < 4 / ESZ; ++e) {
+          uint4 A;
+          if constexpr (FMT == CACHE_E4M3) {
+            // four keys' bytes of a channel side by side, as the converter takes them
+            uint32_t x[2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 A;
-            if constexpr (FMT == CACHE_E4M3) {
-              A = make_uint4(e4m3_pair(x[0][e], false), e4m3_pair(x[0][e], true), e4m3_pair(x[1][e], false),
-                             e4m3_pair(x[1][e], true));
-            } else {
-              A = make_uint4(int8_pair(__builtin_amdgcn_perm(0u, x[0][e], 0x0c010c00u)),
-                             int8_pair(__builtin_amdgcn_perm(0u, x[0][e], 0x0c030c02u)),
-                             int8_pair(__builtin_amdgcn_perm(0u, x[1][e], 0x0c010c00u)),
-                             int8_pair(__builtin_amdgcn_perm(0u, x[1][e], 0x0c030c02u)));
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t s2 = e < 2 ? 0x05010400u : 0x07030602u;
+              const uint32_t lo = __builtin_amdgcn_perm(vr[t][1][w][d], vr[t][0][w][d], s2);
+              const uint32_t hi = __builtin_amdgcn_perm(vr[t][3][w][d], vr[t][2][w][d], s2);
+              x[t] = __builtin_amdgcn_perm(hi, lo, e & 1 ? 0x07060302u : 0x05040100u);
             }
-            const int c = w * CPL + 4 * d + e;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[c][nt] = mfma<FMT>(A, P[nt], acc[c][nt]);
-              if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
+            A = make_uint4(e4m3_pair(x[0], false), e4m3_pair(x[0], true), e4m3_pair(x[1], false), e4m3_pair(x[1], true));
+          } else if constexpr (FMT == CACHE_INT8) {
+            const uint32_t sel = 0x0c040c00u + e * 0x00010001u;  // byte e of two keys
+            A = make_uint4(int8_pair(__builtin_amdgcn_perm(vr[0][1][w][d], vr[0][0][w][d], sel)),
+                           int8_pair(__builtin_amdgcn_perm(vr[0][3][w][d], vr[0][2][w][d], sel)),
+                           int8_pair(__builtin_amdgcn_perm(vr[1][1][w][d], vr[1][0][w][d], sel)),
+                           int8_pair(__builtin_amdgcn_perm(vr[1][3][w][d], vr[1][2][w][d], sel)));
+          } else {
             const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-            const uint4 A = make_uint4(__builtin_amdgcn_perm(vr[0][1][w][d], vr[0][0][w][d], sel),
-                                       __builtin_amdgcn_perm(vr[0][3][w][d], vr[0][2][w][d], sel),
-                                       __builtin_amdgcn_perm(vr[1][1][w][d], vr[1][0][w][d], sel),
-                                       __builtin_amdgcn_perm(vr[1][3][w][d], vr[1][2][w][d], sel));
-            const int c = w * CPL + 2 * d + e;
+            A = make_uint4(__builtin_amdgcn_perm(vr[0][1][w][d], vr[0][0][w][d], sel),
+                           __builtin_amdgcn_perm(vr[0][3][w][d], vr[0][2][w][d], sel),
+                           __builtin_amdgcn_perm(vr[1][1][w][d], vr[1][0][w][d], sel),
+                           __builtin_amdgcn_perm(vr[1][3][w][d], vr[1][2][w][d], sel));
+          }
+          const int c = w * CPL + (4 / ESZ) * d + e;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[c][nt] = mfma<FMT>(A, P[nt], acc[c][nt]);
-              if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            acc[c][nt] = mfma<FMT>(A, P[nt], acc[c][nt]);
+            if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
           }
         }
-      }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(next);
+  };
+
+  int key0 = begin + wave * STEP;
+  if (key0 < end) {
+    Step st = find(key0);
+    load_k(st);
+    load_v(st);
+    // Steps that every row sees, then the rest: two loops, so that neither's
+    // loads are moved ahead of the other's use of the registers.  After the
+    // last step it is asked for again, and not waited for.
+    const int whole = end < ctx ? end : ctx;
+    auto turn = [&](auto is_masked) __attribute__((always_inline)) {
+      const Step next = find(key0 + WAVES * STEP < end ? key0 + WAVES * STEP : key0);
+      step(is_masked, key0, st, next);
+      st = next;
+      key0 += WAVES * STEP;
+    };
+    auto plain = [&]() { return key0 + STEP <= whole && st.live[0] + st.live[1] == STEP; };
+    if (plain()) {
+      do turn(std::false_type());
+      while (plain());
+    }
+    if (key0 < end) {
+      do turn(std::true_type());
+      while (key0 < end);
+    }
   }
   if (bad_page && lane == 0) atomicOr(a.c.flag, VH_CACHE_ERR_PAGE);
 
@@ -614,8 +676,7 @@ int launch_d(const Args& a, int nt, hipStream_t s) {
   const int64_t combos = (int64_t)a.splits * a.batch * a.c.kv_heads;
   const dim3 grid((unsigned)((combos + 7) / 8 * 8 * a.row_blocks));
   if (nt == 1) launch_nt<D, 1>(a, grid, s);
-  else if (nt == 2) launch_nt<D, 2>(a, grid, s);
-  else if constexpr (D <= 128) launch_nt<D, 4>(a, grid, s);
+  else if constexpr (D <= 128) launch_nt<D, 2>(a, grid, s);
   return vh::check_launch("vh_tree_attention");
 }
 

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int WALK_THREADS = 1024;
+constexpr int PICK_THREADS = 1024;
 constexpr int PIECE = 4096;
 constexpr int MAX_PIECES = 1024;
 constexpr int MAX_NODES = VH_TREE_MAX_NODES;
@@ -47,19 +48,23 @@ struct VerifyArgs {
   double2* sums;  // [batch, pieces]: of the rest, and of the rest before the last rejection
 };
 
-struct Nodes {
-  int32_t parent[MAX_NODES];  // -1: not a child
-  int32_t token[MAX_NODES];   // -1: outside the vocabulary
-  float p[MAX_NODES], q[MAX_NODES];
+struct Nodes {  // in LDS; up to a multiple of four, the rest no children
+  alignas(16) int32_t parent[MAX_NODES];  // -1: not a child
+  alignas(16) int32_t token[MAX_NODES];   // -1: outside the vocabulary
+  alignas(16) float p[MAX_NODES];
+  float q[MAX_NODES], u[MAX_NODES];
   int32_t next[MAX_NODES];    // the child taken
 };
 
 template <bool DRAFT>
 VH_DEV void load_nodes(const VerifyArgs& a, int64_t b, Nodes& s, int threads) {
-  for (int n = threadIdx.x; n < a.nodes; n += threads) {
-    int up = a.parents[b * a.nodes + n];
-    const int64_t x = a.tokens[b * a.nodes + n];
-    if (n == 0 || up < 0 || up >= n) up = -1;
+  for (int n = threadIdx.x; n < (a.nodes + 3) / 4 * 4; n += threads) {
+    const bool real = n > 0 && n < a.nodes;
+    const int64_t at = b * a.nodes + (real ? n : 0);
+    int up = a.parents[at];
+    const int64_t x = a.tokens[at];
+    s.u[n] = a.u[at];
+    if (!real || up < 0 || up >= n) up = -1;
     const bool in = up >= 0 && x >= 0 && x < a.vocab;
     s.parent[n] = up;
     s.token[n] = in ? (int32_t)x : -1;
@@ -86,23 +91,17 @@ VH_DEV void tell_none(const VerifyArgs& a, int64_t b, int count, int threads) {
   if (threadIdx.x == 0) a.count[b] = count;
 }
 
-// Sums over the workgroup in a fixed order; every thread gets them.
+// The sum over the workgroup in a fixed order; every thread gets it.
 template <int N>
-VH_DEV double2 block_sum(double2 v, double2* s_part) {
+VH_DEV double block_sum(double v, double* s_part) {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    v.x += __shfl_xor(v.x, d);
-    v.y += __shfl_xor(v.y, d);
-  }
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
   __syncthreads();
-  double2 t = s_part[0];
+  double t = s_part[0];
 #pragma unroll
-  for (int w = 1; w < N / 64; ++w) {
-    t.x += s_part[w].x;
-    t.y += s_part[w].y;
-  }
+  for (int w = 1; w < N / 64; ++w) t += s_part[w];
   return t;
 }
 
@@ -111,7 +110,7 @@ VH_DEV double2 block_sum(double2 v, double2* s_part) {
 // second sibling is tried: a chain needs none.
 __global__ void __launch_bounds__(WALK_THREADS) k_verify_walk(VerifyArgs a) {
   __shared__ Nodes s;
-  __shared__ double2 s_part[WALK_THREADS / 64];
+  __shared__ double s_part[WALK_THREADS / 64];
   const int64_t b = blockIdx.x;
   load_nodes<true>(a, b, s, WALK_THREADS);
   int cur = 0, count = 1;
@@ -124,16 +123,17 @@ __global__ void __launch_bounds__(WALK_THREADS) k_verify_walk(VerifyArgs a) {
       const float* p = a.target + b * a.target_sb + cur * a.target_sn;
       const float* q = a.draft + b * a.draft_sb + cur * a.draft_sn;
       const double more = c + mass;
-      double2 v = {0.0, 0.0};
-      for (int64_t x = threadIdx.x; x < a.vocab; x += WALK_THREADS) v.x += fmax((double)p[x] - more * (double)q[x], 0.0);
-      const double left = block_sum<WALK_THREADS>(v, s_part).x;
+      double v = 0.0;
+#pragma unroll 8
+      for (int64_t x = threadIdx.x; x < a.vocab; x += WALK_THREADS) v += fmax((double)p[x] - more * (double)q[x], 0.0);
+      const double left = block_sum<WALK_THREADS>(v, s_part);
       if (left > 0.0) {
         c = more;
         mass = left;
       }
     }
     const double q = s.q[n], rest = fmax((double)s.p[n] - c * q, 0.0);
-    if ((double)a.u[b * a.nodes + n] * mass * q < rest) {
+    if ((double)s.u[n] * mass * q < rest) {
       if (threadIdx.x == 0) tell(a, b, s, count, n);
       ++count;
       cur = n;
@@ -155,19 +155,29 @@ VH_DEV int walk_chosen(const VerifyArgs& a, int64_t b, Nodes& s, bool teller) {
   load_nodes<false>(a, b, s, THREADS);
   for (int n = threadIdx.x; n < a.nodes; n += THREADS) {
     const int up = s.parent[n], x = s.token[n];
-    if (up < 0 || x < 0) continue;
     bool again = false;
-    for (int k = 1; k < n; ++k) again |= s.parent[k] == up && s.token[k] == x;
+#pragma unroll 4
+    for (int k = 0; k < n; k += 4) {
+      const int4 ups = *(const int4*)&s.parent[k], xs = *(const int4*)&s.token[k];
+      again |= (ups.x == up && xs.x == x) || (ups.y == up && xs.y == x && k + 1 < n) ||
+               (ups.z == up && xs.z == x && k + 2 < n) || (ups.w == up && xs.w == x && k + 3 < n);
+    }
     if (again) s.p[n] = 0.0f;  // an earlier sibling's token: nothing is left of it
   }
   __syncthreads();
   for (int n = threadIdx.x; n < a.nodes; n += THREADS) {
     const int up = s.parent[n];
-    if (up < 0) continue;
     double mass = 1.0;
-    for (int k = 1; k < n; ++k)
-      if (s.parent[k] == up) mass = fmax(mass - (double)s.p[k], 0.0);
-    if ((double)a.u[b * a.nodes + n] * mass < (double)s.p[n]) atomicMin(&s.next[up], n);
+#pragma unroll 4
+    for (int k = 0; k < n; k += 4) {
+      const int4 ups = *(const int4*)&s.parent[k];
+      const float4 ps = *(const float4*)&s.p[k];
+      mass = fmax(mass - (ups.x == up ? (double)ps.x : 0.0), 0.0);
+      mass = fmax(mass - (ups.y == up && k + 1 < n ? (double)ps.y : 0.0), 0.0);
+      mass = fmax(mass - (ups.z == up && k + 2 < n ? (double)ps.z : 0.0), 0.0);
+      mass = fmax(mass - (ups.w == up && k + 3 < n ? (double)ps.w : 0.0), 0.0);
+    }
+    if (up >= 0 && (double)s.u[n] * mass < (double)s.p[n]) atomicMin(&s.next[up], n);
   }
   __syncthreads();
   int cur = 0, count = 1;
@@ -191,27 +201,21 @@ struct Rest {
   const float *p, *q;
   const uint32_t* gone;
   double c, c_before;
-  __device__ __forceinline__ double2 operator()(int64_t first, int i) const {
-    const double x = p[first + i];
+  // entry first + i, 0 from entry n on (read at the last: a read under a
+  // condition would be waited for before the next)
+  __device__ __forceinline__ double2 operator()(int64_t first, int i, int n) const {
+    const int at = i < n ? i : n - 1;
+    const float x0 = p[first + at];
+    const double x = i < n ? x0 : 0.0f;
     if constexpr (DRAFT) {
-      const double y = q[first + i];
+      const float y0 = q[first + at];
+      const double y = i < n ? y0 : 0.0f;
       return double2{c > 0.0 ? fmax(x - c * y, 0.0) : x, c_before > 0.0 ? fmax(x - c_before * y, 0.0) : x};
     } else {
       return double2{gone[i >> 5] >> (i & 31) & 1 ? 0.0 : x, 0.0};
     }
   }
 };
-
-// Marks the tokens of `last`'s children that fall into the piece.
-VH_DEV void mark_gone(const VerifyArgs& a, int64_t b, int last, int64_t first, uint32_t* gone) {
-  for (int i = threadIdx.x; i < PIECE / 32; i += THREADS) gone[i] = 0u;
-  __syncthreads();
-  for (int n = threadIdx.x; n < a.nodes; n += THREADS) {
-    const int64_t x = a.tokens[b * a.nodes + n] - first;
-    if (n > last && a.parents[b * a.nodes + n] == last && x >= 0 && x < PIECE) atomicOr(&gone[x >> 5], 1u << (x & 31));
-  }
-  __syncthreads();
-}
 
 template <bool DRAFT>
 VH_DEV Rest<DRAFT> rest_of(const VerifyArgs& a, int64_t b, int last, const uint32_t* gone, const Row& row) {
@@ -223,7 +227,7 @@ template <bool DRAFT>
 __global__ void __launch_bounds__(THREADS) k_verify_sums(VerifyArgs a) {
   __shared__ Nodes s;
   __shared__ uint32_t s_gone[PIECE / 32];
-  __shared__ double2 s_part[THREADS / 64];
+  __shared__ double s_part[THREADS / 64];
   const int64_t b = blockIdx.y, first = (int64_t)blockIdx.x * PIECE;
   Row row{0, 0, 0.0, 0.0};
   int last;
@@ -232,106 +236,142 @@ __global__ void __launch_bounds__(THREADS) k_verify_sums(VerifyArgs a) {
     last = row.last;
   } else {
     last = walk_chosen(a, b, s, blockIdx.x == 0);
-    mark_gone(a, b, last, first, s_gone);
+    for (int i = threadIdx.x; i < PIECE / 32; i += THREADS) s_gone[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.nodes; i += THREADS) {
+      const int64_t x = s.token[i] - first;
+      if (s.parent[i] == last && x >= 0 && x < PIECE) atomicOr(&s_gone[x >> 5], 1u << (x & 31));
+    }
+    __syncthreads();
   }
   const Rest<DRAFT> rest = rest_of<DRAFT>(a, b, last, s_gone, row);
   const int n = (int)(a.vocab - first < PIECE ? a.vocab - first : PIECE);
   double2 v = {0.0, 0.0};
-#pragma unroll 16
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const double2 x = rest(first, i);
+#pragma unroll
+  for (int k = 0; k < PIECE / THREADS; ++k) {
+    const double2 x = rest(first, k * THREADS + threadIdx.x, n);
     v.x += x.x;
     v.y += x.y;
   }
-  v = block_sum<THREADS>(v, s_part);
+  v.x = block_sum<THREADS>(v.x, s_part);
+  if constexpr (DRAFT) v.y = block_sum<THREADS>(v.y, s_part);
   if (threadIdx.x == 0) a.sums[b * a.pieces + blockIdx.x] = v;
 }
 
-template <bool DRAFT>
-__global__ void __launch_bounds__(THREADS) k_verify_pick(VerifyArgs a) {
-  __shared__ double s_sum[MAX_PIECES];
-  __shared__ double s_w[PIECE];
-  __shared__ double s_wave[THREADS / 64];
-  __shared__ uint32_t s_gone[PIECE / 32];
-  __shared__ int s_first, s_last;
-  const int64_t b = blockIdx.x;
-  const Row row = a.rows[b];
-  bool before = false;  // the last rejection left nothing: the rest is as it was
-  if constexpr (DRAFT) {
-    double all = 0.0;
-    for (int i = 0; i < a.pieces; ++i) all += a.sums[b * a.pieces + i].x;
-    before = !(all > 0.0);
-  }
-  for (int i = threadIdx.x; i < a.pieces; i += THREADS) {
-    const double2 v = a.sums[b * a.pieces + i];
-    s_sum[i] = before ? v.y : v.x;
-  }
-  if (threadIdx.x == 0) {
-    s_first = PIECE;
-    s_last = -1;
+// The sum of the threads up to this one, and of all.
+VH_DEV double block_scan(double v, double* s_wave, double& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const double y = __shfl_up(v, d);
+    if (lane >= d) v += y;
   }
   __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < a.pieces; ++i) total += s_sum[i];
-  const double bar = (double)a.r[b] * total;
-  // the piece in which the running sum passes the bar, or the last with anything in it
-  int piece = -1;
-  double base = 0.0, run = 0.0;
-  for (int i = 0; i < a.pieces; ++i) {
-    const double v = s_sum[i];
-    if (v > 0.0) {
-      piece = i;
-      base = run;
-    }
-    run += v;
-    if (run > bar) break;
+  if (lane == 63) s_wave[wave] = v;
+  __syncthreads();
+  double before = 0.0;
+  all = 0.0;
+#pragma unroll
+  for (int w = 0; w < PICK_THREADS / 64; ++w) {
+    if (w == wave) before = all;
+    all += s_wave[w];
   }
+  return before + v;
+}
+
+// The first thread of the workgroup whose `hit` is true, or else the last
+// whose `any` is, or else -1; s_pick has two places a wave.
+VH_DEV int pick(bool hit, bool any, int* s_pick) {
+  constexpr int W = PICK_THREADS / 64;
+  const uint64_t h = __ballot(hit), y = __ballot(any);
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    s_pick[wave] = h ? wave * 64 + __ffsll((unsigned long long)h) - 1 : PICK_THREADS;
+    s_pick[W + wave] = y ? wave * 64 + 63 - __clzll((long long)y) : -1;
+  }
+  __syncthreads();
+  int first = PICK_THREADS, last = -1;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    first = min(first, s_pick[w]);
+    last = max(last, s_pick[W + w]);
+  }
+  return first < PICK_THREADS ? first : last;
+}
+
+// One thread a piece finds the piece, then one thread four entries the entry.
+template <bool DRAFT>
+__global__ void __launch_bounds__(PICK_THREADS) k_verify_pick(VerifyArgs a) {
+  static_assert(MAX_PIECES <= PICK_THREADS && PIECE == 4 * PICK_THREADS, "one thread a piece, or four entries");
+  __shared__ double s_wave[PICK_THREADS / 64];
+  __shared__ double s_base;
+  __shared__ uint32_t s_gone[PIECE / 32];
+  __shared__ int s_pick[2 * PICK_THREADS / 64];
+  const int64_t b = blockIdx.x;
+  const Row row = a.rows[b];
+  const double r = a.r[b];
+  const bool held = threadIdx.x < a.pieces;
+  const double2 sums = held ? a.sums[b * a.pieces + threadIdx.x] : double2{0.0, 0.0};
+  // the tokens of the last node's children
+  int64_t gone[MAX_NODES / PICK_THREADS];
+  if constexpr (!DRAFT) {
+#pragma unroll
+    for (int k = 0; k < MAX_NODES / PICK_THREADS; ++k) {
+      const int n = k * PICK_THREADS + threadIdx.x;
+      gone[k] = n < a.nodes && n > row.last && a.parents[b * a.nodes + n] == row.last ? a.tokens[b * a.nodes + n] : -1;
+    }
+    for (int i = threadIdx.x; i < PIECE / 32; i += PICK_THREADS) s_gone[i] = 0u;
+  }
+  double total, v = sums.x;
+  double upto = block_scan(v, s_wave, total);
+  bool before = false;
+  if (DRAFT && !(total > 0.0)) {  // the last rejection left nothing: the rest is as it was
+    before = true;
+    v = sums.y;
+    upto = block_scan(v, s_wave, total);
+  }
+  const double bar = r * total;
   int64_t* out = a.told + b * a.nodes + row.count - 1;
+  // the piece in which the running sum passes the bar, or the last with anything in it
+  const int piece = pick(v > 0.0 && upto > bar, v > 0.0, s_pick);
   if (piece < 0 || total != total) {  // no distribution: the end of it, or its start where it holds a NaN
     if (threadIdx.x == 0) *out = total != total ? 0 : a.vocab - 1;
     return;
   }
+  if (threadIdx.x == piece) s_base = upto - v;
   const int64_t first = (int64_t)piece * PIECE;
   const int n = (int)(a.vocab - first < PIECE ? a.vocab - first : PIECE);
-  if constexpr (!DRAFT) mark_gone(a, b, row.last, first, s_gone);
-  const Rest<DRAFT> rest = rest_of<DRAFT>(a, b, row.last, s_gone, row);
-#pragma unroll 16
-  for (int i = threadIdx.x; i < PIECE; i += THREADS) {
-    const double2 x = i < n ? rest(first, i) : double2{0.0, 0.0};
-    s_w[i] = before ? x.y : x.x;
-  }
-  __syncthreads();
-  constexpr int PER = PIECE / THREADS;
-  double mine = 0.0;
+  if constexpr (!DRAFT) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) mine += s_w[threadIdx.x * PER + i];
-  // the sums of the threads before this one
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double up = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double y = __shfl_up(up, d);
-    if (lane >= d) up += y;
-  }
-  if (lane == 63) s_wave[wave] = up;
-  __syncthreads();
-  double at = base + (up - mine);
-  for (int w = 0; w < wave; ++w) at += s_wave[w];
-  int hit = PIECE, any = -1;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const double w = s_w[threadIdx.x * PER + i];
-    at += w;
-    if (w > 0.0) {
-      any = threadIdx.x * PER + i;
-      if (at > bar && hit == PIECE) hit = any;
+    for (int k = 0; k < MAX_NODES / PICK_THREADS; ++k) {
+      const int64_t x = gone[k] - first;
+      if (gone[k] >= 0 && x >= 0 && x < PIECE) atomicOr(&s_gone[x >> 5], 1u << (x & 31));
     }
   }
-  if (hit < PIECE) atomicMin(&s_first, hit);
-  if (any >= 0) atomicMax(&s_last, any);
   __syncthreads();
-  // none where a rounding put the piece's own sum on the other side of the bar
-  if (threadIdx.x == 0) *out = first + (s_first < PIECE ? s_first : s_last);
+  const Rest<DRAFT> rest = rest_of<DRAFT>(a, b, row.last, s_gone, row);
+  double w[4], mine = 0.0, whole;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double2 x = rest(first, threadIdx.x * 4 + i, n);
+    w[i] = before ? x.y : x.x;
+    mine += w[i];
+  }
+  const double base = s_base;
+  double at = base + (block_scan(mine, s_wave, whole) - mine);
+  int hit = 4, any = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    at += w[i];
+    if (w[i] > 0.0) {
+      any = i;
+      if (at > bar && hit == 4) hit = i;
+    }
+  }
+  // none where a rounding put the piece's own sum on the other side of the bar: the last of all
+  const int at_thread = pick(hit < 4, any >= 0, s_pick);
+  if (threadIdx.x == at_thread) *out = first + threadIdx.x * 4 + (hit < 4 ? hit : any);
 }
 
 int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -363,10 +403,10 @@ extern "C" int vh_verify(const float* target, int64_t target_sb, int64_t target_
   if (draft) {
     hipLaunchKernelGGL(k_verify_walk, rows, dim3(WALK_THREADS), 0, s, a);
     hipLaunchKernelGGL(k_verify_sums<true>, pieces, dim3(THREADS), 0, s, a);
-    hipLaunchKernelGGL(k_verify_pick<true>, rows, dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(k_verify_pick<true>, rows, dim3(PICK_THREADS), 0, s, a);
   } else {
     hipLaunchKernelGGL(k_verify_sums<false>, pieces, dim3(THREADS), 0, s, a);
-    hipLaunchKernelGGL(k_verify_pick<false>, rows, dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(k_verify_pick<false>, rows, dim3(PICK_THREADS), 0, s, a);
   }
   return vh::check_launch("vh_verify");
 }
