@@ -758,8 +758,8 @@ int vh_tree_masks(const int32_t* parents, int64_t batch, int32_t nodes, uint64_t
  * exponentials.  A row that sees nothing gives 0 and -inf.  dim 64, 128 or
  * 256, page a multiple of 16, heads a multiple of the cache's.  work: 16-byte
  * aligned device memory of vh_tree_attention_workspace_bytes(desc) bytes.
- * chunk: keys a workgroup takes, a multiple of 128, or 0 to let the library
- * choose. */
+ * The keys of all sequences are shared out, by their number as the device reads
+ * it, to about `workgroups` workgroups (0: the library chooses). */
 typedef struct vh_tree_desc {
   vh_cache cache;
   const void* q;
@@ -773,7 +773,7 @@ typedef struct vh_tree_desc {
   void* work;
   int64_t work_bytes;
   float scale; /* of the scores, positive */
-  int32_t dtype, batch, nodes, heads, table_pages, chunk;
+  int32_t dtype, batch, nodes, heads, table_pages, workgroups;
 } vh_tree_desc;
 int vh_tree_attention(const vh_tree_desc* desc, vh_stream_t stream);
 int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);

@@ -172,14 +172,14 @@ def test_cache_entries_of_nothing():
 def _desc(**kw):
     p = 1 << 20
     a = dict(cache=_cache(), q=p, q_sb=256, q_st=256, q_sh=64, table=p, table_st=4, context=p, masks=p, o=p, lse=p,
-             work=p, work_bytes=1 << 40, scale=0.125, dtype=_lib.VH_BF16, batch=2, nodes=3, heads=4, table_pages=4, chunk=0)
+             work=p, work_bytes=1 << 40, scale=0.125, dtype=_lib.VH_BF16, batch=2, nodes=3, heads=4, table_pages=4, workgroups=0)
     a.update(kw)
     return speculative.TreeDesc(**a)
 
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=_lib.VH_F32), dict(heads=3), dict(heads=0), dict(batch=-1), dict(nodes=-1), dict(nodes=1025),
-    dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(chunk=-1), dict(q=None),
+    dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(workgroups=-1), dict(q=None),
     dict(context=None), dict(table=None), dict(o=None), dict(o=(1 << 20) + 4), dict(work_bytes=8, table_pages=4096),
     dict(work=None, table_pages=4096), dict(work=(1 << 20) + 4, table_pages=4096),
     dict(cache=_cache(page=8, pages=8)), dict(cache=_cache(page=24, slots=96)), dict(cache=_cache(dim=72)),
@@ -201,8 +201,11 @@ def test_attention_workspace():
     need = lambda **kw: _lib.load().vh_tree_attention_workspace_bytes(ctypes.byref(_desc(**kw)))
     assert need(batch=0) == 0 and need(nodes=0) == 0
     assert need(table_pages=4) == 0  # 64 positions: one split
-    # a long table is split, and the partial results stay a small part of the cache it reads
-    assert 0 < need(table_pages=4096) <= 256 * 2 * 2 * 6 * 66 * 4
+    assert need(table_pages=4096, workgroups=1) == 0
+    # a long table is split: as many parts as workgroups, and one more a sequence
+    assert need(table_pages=4096, workgroups=64) == (64 // 2 + 2) * 2 * 6 * 66 * 4
+    # and does not grow with what the table might hold
+    assert need(table_pages=4096) == need(table_pages=1 << 20)
     assert need(table_pages=0) == 0
 
 

@@ -4,11 +4,11 @@
 
 namespace tree {
 template <>
-int launch<64>(const Args& a, int nt, hipStream_t s);
+int launch<64>(const Args& a, bool wide, int n, hipStream_t s);
 template <>
-int launch<128>(const Args& a, int nt, hipStream_t s);
+int launch<128>(const Args& a, bool wide, int n, hipStream_t s);
 template <>
-int launch<256>(const Args& a, int nt, hipStream_t s);
+int launch<256>(const Args& a, bool wide, int n, hipStream_t s);
 }  // namespace tree
 
 namespace {
@@ -18,7 +18,6 @@ using tree::f32x4;
 
 constexpr int MASK_THREADS = 256;
 constexpr int MAX_NODES = VH_TREE_MAX_NODES;
-constexpr int MAX_SPLITS = 256;
 
 // One workgroup a tree, one thread a word of a node's mask: it walks up from
 // the node and sets the bits that fall into its word.  Parents come before
@@ -47,9 +46,33 @@ __global__ void __launch_bounds__(MASK_THREADS) k_tree_masks(const int32_t* pare
   if (bad) atomicOr(flag, VH_CACHE_ERR_PARENT);
 }
 
+// The number of a sequence's splits and of those before them.  Every lane of
+// a wave calls it together, each with a sequence of its own.
+struct Splits {
+  uint32_t before, n;
+};
+VH_DEV Splits splits_before(const Args& a, int b) {
+  Splits s{0u, 1u};
+  const uint32_t chunk = tree::chunk_of(a);
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const uint32_t n = b0 + lane < a.batch ? tree::splits_of(tree::pieces(a, b0 + lane), chunk) : 0u;
+    uint32_t upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t y = (uint32_t)__shfl_up((int)upto, d);
+      upto += lane >= d ? y : 0u;
+    }
+    const int at = b - b0 < 0 ? 0 : b - b0 > 63 ? 63 : b - b0;
+    const uint32_t mine = (uint32_t)__shfl((int)n, at), sum = (uint32_t)__shfl((int)upto, at);
+    if (b >= b0 + 64) s.before += sum;
+    else if (b >= b0) s = Splits{s.before + sum - mine, mine};
+  }
+  return s;
+}
+
 // The splits of a row joined: D / 4 lanes hold the row's channels, `GROUPS`
-// of them take turns along the splits, and a row reads only the splits that
-// its keys reach.
+// of them take turns along the splits.
 template <int D, int GROUPS>
 __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
   constexpr int LANES = D / 4, ROWS = 256 / (LANES * GROUPS);
@@ -59,12 +82,13 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
   const int64_t id = (int64_t)blockIdx.x * ROWS + (GROUPS > 1 ? 0 : threadIdx.x / LANES);
   const int c = threadIdx.x % LANES * 4;
   const int pairs = a.batch * a.c.kv_heads;
-  if (id >= (int64_t)pairs * a.rows) return;
-  const int pair = (int)(id / a.rows), row = (int)(id - (int64_t)pair * a.rows);
+  const bool in = id < (int64_t)pairs * a.rows;  // a wave's lanes go on together: they share out the sequences
+  const int pair = in ? (int)(id / a.rows) : 0, row = in ? (int)(id - (int64_t)pair * a.rows) : 0;
   const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
-  const int total = tree::visible(a, a.context[b], row / a.block_rows * a.block_rows);
-  const int splits = (total + a.chunk - 1) / a.chunk;
-  const int64_t at = (int64_t)pair * a.splits * a.rows + row;
+  const Splits sp = splits_before(a, b);
+  const int splits = (int)sp.n;
+  const int64_t step = (int64_t)a.c.kv_heads * a.rows, at = ((int64_t)sp.before * a.c.kv_heads + h) * a.rows + row;
+  if (!in) return;
   float M = -__builtin_inff(), L = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   // four splits at a time, so that their reads overlap
@@ -74,7 +98,7 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int s = s0 + k * GROUPS;
-      const int64_t p = at + (int64_t)(s < splits ? s : s0) * a.rows;
+      const int64_t p = at + (s < splits ? s : s0) * step;
       ml[k] = *(const float2*)(a.part_ml + 2 * p);
       x[k] = *(const f32x4*)(a.part_o + p * D + c);
       if (s >= splits) {
@@ -121,42 +145,55 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
                : make_uint2(tree::pack2<CACHE_F16>(o[0], o[1]), tree::pack2<CACHE_F16>(o[2], o[3]));
 }
 
-// Many splits: a workgroup a row.  Few: as many rows as fit one.
+// Many splits a sequence and few rows: a workgroup a row.  Else as many rows as
+// fit one.
 template <int D>
 void merge(const Args& a, hipStream_t s) {
   constexpr int ALL = 1024 / D;  // groups of lanes in a workgroup
   const int64_t rows = (int64_t)a.batch * a.c.kv_heads * a.rows;
-  if (a.splits > 4) hipLaunchKernelGGL((k_tree_merge<D, ALL>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  if (a.units >= 8 * (uint32_t)a.batch && rows <= 4096) hipLaunchKernelGGL((k_tree_merge<D, ALL>), dim3((unsigned)rows), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_tree_merge<D, 1>), dim3((unsigned)((rows + ALL - 1) / ALL)), dim3(256), 0, s, a);
 }
 
 struct Plan {
-  int nt, row_blocks, chunk, splits;
+  bool wide;
+  int n, block_rows, row_blocks;  // n: tiles of 16 rows a wave, or waves of rows
+  uint32_t share, units;
   int64_t part;  // rows of partial results
 };
 
-// The shape of the launch.  Rows of a wave: 16, or 32 where there are more and
-// their accumulators leave two waves a SIMD (heads of 64 and 128).
+// The shape of the launch.  Up to 32 rows of a key head (16 of heads of 256)
+// a wave holds them all and takes its own keys; more share converted keys.
 Plan plan_of(const vh_tree_desc* d) {
   Plan p;
   const int64_t rows = (int64_t)d->nodes * (d->heads / d->cache.kv_heads);
-  p.nt = rows <= 16 || d->cache.dim > 128 ? 1 : 2;
-  p.row_blocks = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
-  const int64_t keys = (int64_t)d->table_pages * d->cache.page;
-  const int64_t pairs = (int64_t)d->batch * d->cache.kv_heads;
-  const int64_t least = tree::WAVES * tree::STEP;
-  int64_t chunk = d->chunk;
-  if (chunk == 0) {
-    // as many workgroups as four for each of the 256 CUs, if a wave still has a step of its own
-    const int64_t blocks = pairs * p.row_blocks;
-    chunk = keys * blocks / 1024;
+  const bool small = d->cache.dim <= 128;
+  p.wide = rows > (small ? 32 : 16);
+  if (p.wide) {
+    p.n = small && rows <= 64 ? 2 : 4;
+    p.block_rows = 16 * (small ? 2 : 1) * p.n;
+  } else {
+    p.n = small && rows > 16 ? 2 : 1;
+    p.block_rows = 16 * p.n;
   }
-  chunk = (chunk + least - 1) / least * least;
-  if (chunk < least) chunk = least;
-  while ((keys + chunk - 1) / chunk > MAX_SPLITS) chunk += least;
-  p.chunk = (int)chunk;
-  p.splits = (int)((keys + chunk - 1) / chunk);
-  p.part = p.splits > 1 ? pairs * p.splits * rows : 0;
+  p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
+  const int64_t keys = (int64_t)d->table_pages * d->cache.page;
+  const int64_t most = (keys + tree::PIECE - 1) / tree::PIECE;  // splits of a sequence, a piece each
+  const int64_t blocks = (int64_t)d->cache.kv_heads * p.row_blocks;
+  // Two workgroups a CU hold their registers where rows are many, and each more
+  // share costs its rows' partial results twice; single tokens' keys fill the
+  // card best at six, whose results are few.  (8 trees of 64 over 4096: 83 us at
+  // 1024, 69 at 512, 89 at 256; 32 tokens over 8192: 91 us at 512, 83 at 1536.)
+  const int64_t slots = d->workgroups > 0 ? d->workgroups : p.wide ? 512 : 1536;
+  int64_t share = slots / blocks;
+  if (share < 1) share = 1;
+  if (share > most * d->batch) share = most * d->batch > 0 ? most * d->batch : 1;
+  p.share = (uint32_t)share;
+  // one share: every sequence is one split, and its results are final
+  int64_t units = share == 1 ? d->batch : share + d->batch;
+  if (units > most * d->batch && most > 0) units = most * d->batch;
+  p.units = (uint32_t)units;
+  p.part = units > d->batch ? units * d->cache.kv_heads * rows : 0;
   return p;
 }
 
@@ -176,7 +213,7 @@ int desc_check(const vh_tree_desc* d, const char* what) {
   VH_REQUIRE((int64_t)d->batch * c.kv_heads < (1 << 20), "%s: too many sequences", what);
   VH_REQUIRE(!d->masks || d->nodes <= MAX_NODES, "%s: at most %d nodes", what, MAX_NODES);
   VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
-  VH_REQUIRE(d->chunk >= 0, "%s: bad chunk", what);
+  VH_REQUIRE(d->workgroups >= 0 && d->workgroups <= (1 << 20), "%s: bad number of workgroups", what);
   return VH_OK;
 }
 
@@ -221,8 +258,10 @@ extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
   a.masks = d->masks;
   a.o = d->o;
   a.lse = d->lse;
-  a.part_o = (float*)d->work;
-  a.part_ml = a.part_o + p.part * d->cache.dim;
+  if (p.part > 0) {
+    a.part_o = (float*)d->work;
+    a.part_ml = a.part_o + p.part * d->cache.dim;
+  }
   a.group_div = make_fast_div((uint32_t)group);
   a.page_div = make_fast_div((uint32_t)(d->cache.page / 16));
   a.scale = d->scale * tree::LOG2E;
@@ -235,18 +274,18 @@ extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
   a.group = group;
   a.rows = d->nodes * group;
   a.row_blocks = p.row_blocks;
-  a.block_rows = 16 * p.nt;
+  a.block_rows = p.block_rows;
   a.table_pages = d->table_pages;
-  a.chunk = p.chunk;
-  a.splits = p.splits > 0 ? p.splits : 1;
-  VH_REQUIRE(((int64_t)a.splits * a.batch * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31) &&
+  a.share = p.share;
+  a.units = p.units;
+  VH_REQUIRE(((int64_t)p.units * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31) &&
                  (int64_t)a.batch * a.c.kv_heads * a.rows < (1ll << 31),
              "vh_tree_attention: too many workgroups");
   hipStream_t s = vh::as_stream(stream);
-  const int rc = d->cache.dim == 64 ? tree::launch<64>(a, p.nt, s)
-                 : d->cache.dim == 128 ? tree::launch<128>(a, p.nt, s)
-                                       : tree::launch<256>(a, p.nt, s);
-  if (rc != VH_OK || a.splits == 1) return rc;
+  const int rc = d->cache.dim == 64 ? tree::launch<64>(a, p.wide, p.n, s)
+                 : d->cache.dim == 128 ? tree::launch<128>(a, p.wide, p.n, s)
+                                       : tree::launch<256>(a, p.wide, p.n, s);
+  if (rc != VH_OK || p.part == 0) return rc;
   if (d->cache.dim == 64) merge<64>(a, s);
   else if (d->cache.dim == 128) merge<128>(a, s);
   else merge<256>(a, s);

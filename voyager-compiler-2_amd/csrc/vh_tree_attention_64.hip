@@ -3,7 +3,7 @@
 
 namespace tree {
 template <>
-int launch<64>(const Args& a, int nt, hipStream_t s) {
-  return launch_d<64>(a, nt, s);
+int launch<64>(const Args& a, bool wide, int n, hipStream_t s) {
+  return launch_d<64>(a, wide, n, s);
 }
 }  // namespace tree

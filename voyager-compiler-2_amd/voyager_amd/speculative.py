@@ -34,7 +34,7 @@ class TreeDesc(ctypes.Structure):
         ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64),
         ("scale", ctypes.c_float),
         ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("nodes", ctypes.c_int32), ("heads", ctypes.c_int32),
-        ("table_pages", ctypes.c_int32), ("chunk", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32), ("workgroups", ctypes.c_int32),
     ]
 
 
