@@ -691,10 +691,22 @@ int vh_nhwc_to_nchw(const void* src, int32_t dtype, int64_t n, int64_t p, int64_
  * pos: integers of pos_bits (32 or 64), strides in elements (0: shared).
  * turns: rotary / 2 float64 in device memory.  inverse turns back: the
  * gradient.  dim even, at most 512. */
-int vh_rope(const void* q, void* q_out, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, void* k_out,
-            int64_t k_sb, int64_t k_st, int64_t k_sh, int32_t dtype, int64_t batch, int64_t tokens, int32_t heads,
-            int32_t kv_heads, int32_t dim, int32_t rotary, int32_t interleaved, const void* pos, int32_t pos_bits,
-            int64_t pos_sb, int64_t pos_st, const double* turns, float factor, int32_t inverse, vh_stream_t stream);
+typedef struct vh_rope_desc {
+  const void* q;
+  void* q_out;
+  int64_t q_sb, q_st, q_sh;
+  const void* k;
+  void* k_out;
+  int64_t k_sb, k_st, k_sh;
+  const void* pos;
+  int64_t pos_sb, pos_st;
+  int64_t batch, tokens;
+  int32_t heads, kv_heads, dtype, pos_bits;
+  int32_t inverse, dim, rotary, interleaved;
+  float factor;
+  const double* turns;
+} vh_rope_desc;
+int vh_rope(const vh_rope_desc* desc, vh_stream_t stream);
 
 /* A cache in pages: slot s is row s % page of page s / page.  k, v:
  * [pages, kv_heads, page, dim] of codes (E4M3 bytes, or int8 codes + 128) or
@@ -757,7 +769,8 @@ int vh_tree_masks(const int32_t* parents, int64_t batch, int32_t nodes, uint64_t
  * lse (or NULL): [batch, nodes, heads] float32, the logarithm of the sum of
  * exponentials.  A row that sees nothing gives 0 and -inf.  dim 64, 128 or
  * 256, page a multiple of 16, heads a multiple of the cache's.  work: 16-byte
- * aligned device memory of vh_tree_attention_workspace_bytes(desc) bytes.
+ * aligned device memory of vh_tree_attention_workspace_bytes(desc) bytes
+ * (which goes by the sizes alone).
  * The keys of all sequences are shared out, by their number as the device reads
  * it, to about `workgroups` workgroups (0: the library chooses). */
 typedef struct vh_tree_desc {
@@ -770,12 +783,10 @@ typedef struct vh_tree_desc {
   const uint64_t* masks;
   void* o;
   float* lse;
-  void* work;
-  int64_t work_bytes;
   float scale; /* of the scores, positive */
   int32_t dtype, batch, nodes, heads, table_pages, workgroups;
 } vh_tree_desc;
-int vh_tree_attention(const vh_tree_desc* desc, vh_stream_t stream);
+int vh_tree_attention(const vh_tree_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
 int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);
 
 /* The choice among drafted tokens.  target [batch, nodes, vocab] float32: the
@@ -793,10 +804,19 @@ int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);
  * path [batch, nodes]: the first node and those taken, -1 after them; count
  * [batch]: how many.  A token outside the vocabulary is never taken.  work:
  * vh_verify_workspace_bytes(batch, vocab) bytes, 16-byte aligned. */
-int vh_verify(const float* target, int64_t target_sb, int64_t target_sn, const float* draft, int64_t draft_sb,
-              int64_t draft_sn, const int32_t* parents, const int64_t* tokens, const float* u, const float* r,
-              int64_t batch, int32_t nodes, int64_t vocab, int64_t* told, int32_t* path, int32_t* count, void* work,
-              int64_t work_bytes, vh_stream_t stream);
+typedef struct vh_verify_desc {
+  const float* target;
+  int64_t target_sb, target_sn; /* strides of sequence and node, in elements */
+  const float* draft;
+  int64_t draft_sb, draft_sn;
+  const int32_t* parents;
+  const int64_t* tokens;
+  const float *u, *r;
+  int64_t batch, nodes, vocab;
+  int64_t* told;
+  int32_t *path, *count;
+} vh_verify_desc;
+int vh_verify(const vh_verify_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
 int64_t vh_verify_workspace_bytes(int64_t batch, int64_t vocab);
 
 #ifdef __cplusplus

@@ -4,6 +4,8 @@ entries (which check before they launch), and workspace sizes."""
 
 import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -83,12 +85,38 @@ def test_rotary_arguments_refused():
 def _rope(**kw):
     a = dict(q=1 << 20, heads=4, dim=64, rotary=64, dtype=_lib.VH_F32, pos=1 << 20, bits=64, turns=1 << 20, batch=1)
     a.update(kw)
-    return _lib.load().vh_rope(a["q"], a["q"], 0, 0, 0, None, None, 0, 0, 0, a["dtype"], a["batch"], 3, a["heads"], 0,
-                               a["dim"], a["rotary"], 0, a["pos"], a["bits"], 0, 1, a["turns"], 1.0, 0, None)
+    d = rotary.ROPE.pack(a["q"], a["q"], 0, 0, 0, 0, 0, 0, 0, 0, a["pos"], 0, 1, a["batch"], 3, a["heads"], 0, a["dtype"],
+                         a["bits"], 0) + rotary._ROPE_REST.pack(a["dim"], a["rotary"], 0, 1.0, a["turns"])
+    return _lib.load().vh_rope(d, None)
+
+
+def test_descriptors_are_as_long_as_the_header_says():
+    """The packed descriptors against the structures' sizes: pointers and
+    int64 of 8 bytes, int32 and float of 4, each at its own alignment."""
+    text = open(os.path.join(os.path.dirname(__file__), "..", "include", "voyager_hip.h")).read()
+
+    def size(name):
+        at, most = 0, 8
+        for line in re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1).split(";"):
+            line = re.sub(r"/\*.*?\*/", "", line, flags=re.S).strip()
+            if not line:
+                continue
+            for i in range(line.count(",") + 1):
+                if line.startswith("vh_cache "):
+                    n, a = ctypes.sizeof(_lib.Cache), 8
+                else:
+                    n = a = 8 if "*" in line or "int64_t" in line else 4
+                at = -(-at // a) * a + n
+        return -(-at // most) * most
+
+    assert size("vh_cache") == ctypes.sizeof(_lib.Cache)
+    assert size("vh_rope_desc") == rotary.ROPE.size + rotary._ROPE_REST.size
+    assert size("vh_tree_desc") == ctypes.sizeof(_lib.Cache) + speculative.TREE.size
+    assert size("vh_verify_desc") == speculative.VERIFY.size
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=_lib.VH_U8), dict(dim=63, rotary=2), dict(dim=514), dict(rotary=66),
-                                dict(rotary=0), dict(bits=16), dict(q=None), dict(pos=None), dict(turns=None),
+                                dict(rotary=0), dict(bits=16), dict(q=0), dict(pos=0), dict(turns=0),
                                 dict(batch=-1)])
 def test_rope_entry_refuses(kw):
     assert _rope(**kw) == 1
@@ -172,33 +200,37 @@ def test_cache_entries_of_nothing():
 def _desc(**kw):
     p = 1 << 20
     a = dict(cache=_cache(), q=p, q_sb=256, q_st=256, q_sh=64, table=p, table_st=4, context=p, masks=p, o=p, lse=p,
-             work=p, work_bytes=1 << 40, scale=0.125, dtype=_lib.VH_BF16, batch=2, nodes=3, heads=4, table_pages=4, workgroups=0)
+             scale=0.125, dtype=_lib.VH_BF16, batch=2, nodes=3, heads=4, table_pages=4, workgroups=0)
     a.update(kw)
-    return speculative.TreeDesc(**a)
+    return bytes(a.pop("cache")) + speculative.TREE.pack(*a.values())
+
+
+def _attention(work=1 << 20, work_bytes=1 << 40, **kw):
+    return _lib.load().vh_tree_attention(_desc(**kw), work, work_bytes, None)
 
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=_lib.VH_F32), dict(heads=3), dict(heads=0), dict(batch=-1), dict(nodes=-1), dict(nodes=1025),
-    dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(workgroups=-1), dict(q=None),
-    dict(context=None), dict(table=None), dict(o=None), dict(o=(1 << 20) + 4), dict(work_bytes=8, table_pages=4096),
+    dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(workgroups=-1), dict(q=0),
+    dict(context=0), dict(table=0), dict(o=0), dict(o=(1 << 20) + 4), dict(work_bytes=8, table_pages=4096),
     dict(work=None, table_pages=4096), dict(work=(1 << 20) + 4, table_pages=4096),
     dict(cache=_cache(page=8, pages=8)), dict(cache=_cache(page=24, slots=96)), dict(cache=_cache(dim=72)),
     dict(cache=_cache(fmt=_lib.CACHE_F16)), dict(cache=_cache(fmt=_lib.CACHE_BF16), dtype=_lib.VH_F16)])
 def test_attention_entry_refuses(kw):
     lib = _lib.load()
-    assert lib.vh_tree_attention(ctypes.byref(_desc(**kw)), None) == 1
+    assert _attention(**kw) == 1
     assert lib.vh_last_error().startswith(b"vh_tree_attention")
 
 
 @pytest.mark.parametrize("kw", BAD_CACHES)
 def test_attention_entry_refuses_caches(kw):
     lib = _lib.load()
-    d = ctypes.byref(_desc(cache=_cache(**kw)))
-    assert lib.vh_tree_attention(d, None) == 1 and lib.vh_tree_attention_workspace_bytes(d) == -1
+    d = _desc(cache=_cache(**kw))
+    assert _attention(cache=_cache(**kw)) == 1 and lib.vh_tree_attention_workspace_bytes(d) == -1
 
 
 def test_attention_workspace():
-    need = lambda **kw: _lib.load().vh_tree_attention_workspace_bytes(ctypes.byref(_desc(**kw)))
+    need = lambda **kw: _lib.load().vh_tree_attention_workspace_bytes(_desc(**kw))
     assert need(batch=0) == 0 and need(nodes=0) == 0
     assert need(table_pages=4) == 0  # 64 positions: one split
     assert need(table_pages=4096, workgroups=1) == 0
@@ -210,7 +242,7 @@ def test_attention_workspace():
 
 
 def test_attention_of_nothing():
-    assert _lib.load().vh_tree_attention(ctypes.byref(_desc(batch=0, q=None)), None) == 0
+    assert _attention(batch=0, q=0, work=None, work_bytes=0) == 0
 
 
 def test_attention_arguments_refused():
@@ -243,16 +275,15 @@ def test_tree_refuses():
 # ---------------------------------------------------------------- verify
 def _verify(**kw):
     p = 1 << 20
-    a = dict(target=p, parents=p, tokens=p, u=p, r=p, batch=2, nodes=4, vocab=1000, told=p, path=p, count=p, work=p,
-             work_bytes=1 << 30)
+    a = dict(target=p, target_sb=4000, target_sn=1000, draft=0, draft_sb=0, draft_sn=0, parents=p, tokens=p, u=p, r=p,
+             batch=2, nodes=4, vocab=1000, told=p, path=p, count=p)
+    work, work_bytes = kw.pop("work", p), kw.pop("work_bytes", 1 << 30)
     a.update(kw)
-    return _lib.load().vh_verify(a["target"], 4000, 1000, None, 0, 0, a["parents"], a["tokens"], a["u"], a["r"],
-                                 a["batch"], a["nodes"], a["vocab"], a["told"], a["path"], a["count"], a["work"],
-                                 a["work_bytes"], None)
+    return _lib.load().vh_verify(speculative.VERIFY.pack(*a.values()), work, work_bytes, None)
 
 
-@pytest.mark.parametrize("kw", [dict(target=None), dict(parents=None), dict(tokens=None), dict(u=None), dict(r=None),
-                                dict(told=None), dict(path=None), dict(count=None), dict(work=None), dict(work_bytes=8),
+@pytest.mark.parametrize("kw", [dict(target=0), dict(parents=0), dict(tokens=0), dict(u=0), dict(r=0),
+                                dict(told=0), dict(path=0), dict(count=0), dict(work=None), dict(work_bytes=8),
                                 dict(work=(1 << 20) + 4), dict(batch=-1), dict(batch=65536), dict(nodes=0),
                                 dict(nodes=1025), dict(vocab=0), dict(vocab=(1 << 22) + 1)])
 def test_verify_entry_refuses(kw):

@@ -187,29 +187,29 @@ void rope_dispatch(RopeArgs& a, bool interleaved, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int vh_rope(const void* q, void* q_out, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, void* k_out,
-                       int64_t k_sb, int64_t k_st, int64_t k_sh, int32_t dtype, int64_t batch, int64_t tokens,
-                       int32_t heads, int32_t kv_heads, int32_t dim, int32_t rotary, int32_t interleaved,
-                       const void* pos, int32_t pos_bits, int64_t pos_sb, int64_t pos_st, const double* turns,
-                       float factor, int32_t inverse, vh_stream_t stream) {
-  VH_REQUIRE(vh::is_float_dtype(dtype), "vh_rope: dtype must be bfloat16, float16 or float32");
-  VH_REQUIRE(batch >= 0 && tokens >= 0 && heads >= 0 && kv_heads >= 0, "vh_rope: negative size");
-  VH_REQUIRE(dim > 0 && dim <= ROPE_MAX_DIM && dim % 2 == 0, "vh_rope: dim must be even and at most %d (got %d)",
-             ROPE_MAX_DIM, dim);
-  VH_REQUIRE(rotary > 0 && rotary <= dim && rotary % 2 == 0, "vh_rope: the rotated part must be even and at most dim");
-  VH_REQUIRE(pos_bits == 32 || pos_bits == 64, "vh_rope: positions of 32 or 64 bits");
-  const int64_t rows = batch * tokens;
-  if (rows == 0 || heads + kv_heads == 0) return VH_OK;
-  VH_REQUIRE(rows < (1ll << 31) && (int64_t)heads + kv_heads < (1 << 20), "vh_rope: too many rows or heads");
-  VH_REQUIRE((heads == 0 || (q && q_out)) && (kv_heads == 0 || (k && k_out)) && pos && turns, "vh_rope: null argument");
-  RopeArgs a{{heads ? q : k, heads ? q_out : k_out, heads ? q_sb : k_sb, heads ? q_st : k_st, heads ? q_sh : k_sh},
-             {kv_heads ? k : q, kv_heads ? k_out : q_out, kv_heads ? k_sb : q_sb, kv_heads ? k_st : q_st,
-              kv_heads ? k_sh : q_sh},
-             pos, pos_sb, pos_st, turns, tokens, rows, make_fast_div((uint32_t)(heads + kv_heads)), heads, kv_heads, dim,
-             rotary, 0, pos_bits == 64, factor, inverse ? -1.0f : 1.0f};
+extern "C" int vh_rope(const vh_rope_desc* d, vh_stream_t stream) {
+  VH_REQUIRE(d, "vh_rope: null descriptor");
+  VH_REQUIRE(vh::is_float_dtype(d->dtype), "vh_rope: dtype must be bfloat16, float16 or float32");
+  VH_REQUIRE(d->batch >= 0 && d->tokens >= 0 && d->heads >= 0 && d->kv_heads >= 0, "vh_rope: negative size");
+  VH_REQUIRE(d->dim > 0 && d->dim <= ROPE_MAX_DIM && d->dim % 2 == 0, "vh_rope: dim must be even and at most %d (got %d)",
+             ROPE_MAX_DIM, d->dim);
+  VH_REQUIRE(d->rotary > 0 && d->rotary <= d->dim && d->rotary % 2 == 0,
+             "vh_rope: the rotated part must be even and at most dim");
+  VH_REQUIRE(d->pos_bits == 32 || d->pos_bits == 64, "vh_rope: positions of 32 or 64 bits");
+  VH_REQUIRE(d->batch < (1ll << 31) && d->tokens < (1ll << 31), "vh_rope: too many rows");
+  const int64_t rows = d->batch * d->tokens;
+  if (rows == 0 || d->heads + (int64_t)d->kv_heads == 0) return VH_OK;
+  VH_REQUIRE(rows < (1ll << 31) && (int64_t)d->heads + d->kv_heads < (1 << 20), "vh_rope: too many rows or heads");
+  VH_REQUIRE((d->heads == 0 || (d->q && d->q_out)) && (d->kv_heads == 0 || (d->k && d->k_out)) && d->pos && d->turns,
+             "vh_rope: null argument");
+  const RopeTensor q{d->q, d->q_out, d->q_sb, d->q_st, d->q_sh}, k{d->k, d->k_out, d->k_sb, d->k_st, d->k_sh};
+  // a tensor without heads is never read: the other one's stands for it
+  RopeArgs a{d->heads ? q : k, d->kv_heads ? k : q, d->pos, d->pos_sb, d->pos_st, d->turns, d->tokens, rows,
+             make_fast_div((uint32_t)(d->heads + d->kv_heads)), d->heads, d->kv_heads, d->dim, d->rotary, 0,
+             d->pos_bits == 64, d->factor, d->inverse ? -1.0f : 1.0f};
   hipStream_t s = vh::as_stream(stream);
-  if (dtype == VH_BF16) rope_dispatch<__bf16>(a, interleaved != 0, s);
-  else if (dtype == VH_F16) rope_dispatch<_Float16>(a, interleaved != 0, s);
-  else rope_dispatch<float>(a, interleaved != 0, s);
+  if (d->dtype == VH_BF16) rope_dispatch<__bf16>(a, d->interleaved != 0, s);
+  else if (d->dtype == VH_F16) rope_dispatch<_Float16>(a, d->interleaved != 0, s);
+  else rope_dispatch<float>(a, d->interleaved != 0, s);
   return vh::check_launch("vh_rope");
 }

@@ -236,14 +236,14 @@ extern "C" int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* d) {
   return plan_of(d).part * (int64_t)sizeof(float) * (d->cache.dim + 2);
 }
 
-extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
+extern "C" int vh_tree_attention(const vh_tree_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
   if (int e = desc_check(d, "vh_tree_attention")) return e;
   if (d->batch == 0 || d->nodes == 0) return VH_OK;
   VH_REQUIRE(d->q && d->context && d->o && (d->table || d->table_pages == 0), "vh_tree_attention: null argument");
   VH_REQUIRE((uintptr_t)d->o % 16 == 0, "vh_tree_attention: misaligned output");
   const Plan p = plan_of(d);
   const int64_t need = p.part * (int64_t)sizeof(float) * (d->cache.dim + 2);
-  VH_REQUIRE(need == 0 || (d->work && d->work_bytes >= need && (uintptr_t)d->work % 16 == 0),
+  VH_REQUIRE(need == 0 || (work && work_bytes >= need && (uintptr_t)work % 16 == 0),
              "vh_tree_attention: needs %lld bytes of aligned workspace", (long long)need);
   const int group = d->heads / d->cache.kv_heads;
   Args a{};
@@ -259,7 +259,7 @@ extern "C" int vh_tree_attention(const vh_tree_desc* d, vh_stream_t stream) {
   a.o = d->o;
   a.lse = d->lse;
   if (p.part > 0) {
-    a.part_o = (float*)d->work;
+    a.part_o = (float*)work;
     a.part_ml = a.part_o + p.part * d->cache.dim;
   }
   a.group_div = make_fast_div((uint32_t)group);

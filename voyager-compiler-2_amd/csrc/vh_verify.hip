@@ -383,24 +383,24 @@ extern "C" int64_t vh_verify_workspace_bytes(int64_t batch, int64_t vocab) {
   return align16(batch * (int64_t)sizeof(Row)) + batch * ((vocab + PIECE - 1) / PIECE) * (int64_t)sizeof(double2);
 }
 
-extern "C" int vh_verify(const float* target, int64_t target_sb, int64_t target_sn, const float* draft, int64_t draft_sb,
-                         int64_t draft_sn, const int32_t* parents, const int64_t* tokens, const float* u, const float* r,
-                         int64_t batch, int32_t nodes, int64_t vocab, int64_t* told, int32_t* path, int32_t* count,
-                         void* work, int64_t work_bytes, vh_stream_t stream) {
-  VH_REQUIRE(batch >= 0 && batch < 65536, "vh_verify: at most 65535 sequences");
-  VH_REQUIRE(nodes >= 1 && nodes <= MAX_NODES, "vh_verify: 1 to %d nodes (got %d)", MAX_NODES, nodes);
-  VH_REQUIRE(vocab >= 1 && vocab <= (int64_t)PIECE * MAX_PIECES, "vh_verify: a vocabulary of 1 to %lld",
+extern "C" int vh_verify(const vh_verify_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
+  VH_REQUIRE(d, "vh_verify: null descriptor");
+  VH_REQUIRE(d->batch >= 0 && d->batch < 65536, "vh_verify: at most 65535 sequences");
+  VH_REQUIRE(d->nodes >= 1 && d->nodes <= MAX_NODES, "vh_verify: 1 to %d nodes (got %lld)", MAX_NODES, (long long)d->nodes);
+  VH_REQUIRE(d->vocab >= 1 && d->vocab <= (int64_t)PIECE * MAX_PIECES, "vh_verify: a vocabulary of 1 to %lld",
              (long long)PIECE * MAX_PIECES);
-  if (batch == 0) return VH_OK;
-  VH_REQUIRE(target && parents && tokens && u && r && told && path && count, "vh_verify: null argument");
-  VH_REQUIRE(work && (uintptr_t)work % 16 == 0 && work_bytes >= vh_verify_workspace_bytes(batch, vocab),
-             "vh_verify: needs %lld bytes of aligned workspace", (long long)vh_verify_workspace_bytes(batch, vocab));
-  VerifyArgs a{target, draft, target_sb, target_sn, draft_sb, draft_sn, parents, tokens, u, r, nodes,
-               (int)((vocab + PIECE - 1) / PIECE), vocab, told, path, count, (Row*)work,
-               (double2*)((char*)work + align16(batch * (int64_t)sizeof(Row)))};
+  if (d->batch == 0) return VH_OK;
+  VH_REQUIRE(d->target && d->parents && d->tokens && d->u && d->r && d->told && d->path && d->count,
+             "vh_verify: null argument");
+  const int64_t need = vh_verify_workspace_bytes(d->batch, d->vocab);
+  VH_REQUIRE(work && (uintptr_t)work % 16 == 0 && work_bytes >= need, "vh_verify: needs %lld bytes of aligned workspace",
+             (long long)need);
+  VerifyArgs a{d->target, d->draft, d->target_sb, d->target_sn, d->draft_sb, d->draft_sn, d->parents, d->tokens, d->u, d->r,
+               (int)d->nodes, (int)((d->vocab + PIECE - 1) / PIECE), d->vocab, d->told, d->path, d->count, (Row*)work,
+               (double2*)((char*)work + align16(d->batch * (int64_t)sizeof(Row)))};
   hipStream_t s = vh::as_stream(stream);
-  const dim3 rows((unsigned)batch), pieces((unsigned)a.pieces, (unsigned)batch);
-  if (draft) {
+  const dim3 rows((unsigned)d->batch), pieces((unsigned)a.pieces, (unsigned)d->batch);
+  if (d->draft) {
     hipLaunchKernelGGL(k_verify_walk, rows, dim3(WALK_THREADS), 0, s, a);
     hipLaunchKernelGGL(k_verify_sums<true>, pieces, dim3(THREADS), 0, s, a);
     hipLaunchKernelGGL(k_verify_pick<true>, rows, dim3(PICK_THREADS), 0, s, a);

@@ -192,16 +192,17 @@ _SIGNATURES = {
     "vh_spmm_csr": ([_P, _I32, _P, _P, _I64, _I64, _I64, _P, _I32, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _P],
                     _I32),
     # a step with drafted tokens
-    "vh_rope": ([_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I32, _I64, _I64, _I32, _I32, _I32, _I32, _I32,
-                 _P, _I32, _I64, _I64, _P, _F32, _I32, _P], _I32),
+    # vh_rope, vh_tree_attention and vh_verify take a descriptor's bytes: rotary.ROPE, speculative.TREE
+    # and speculative.VERIFY pack vh_rope_desc, vh_tree_desc and vh_verify_desc (a ctypes structure
+    # of as many fields costs 3 us of a call)
+    "vh_rope": ([_P, _P], _I32),
     "vh_paged_write": ([ctypes.POINTER(Cache), _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _P], _I32),
     "vh_paged_read": ([ctypes.POINTER(Cache), _P, _P, _I32, _P, _I64, _P], _I32),
     "vh_paged_keep": ([ctypes.POINTER(Cache), _P, _I64, _I32, _P, _P, _I64, _P, _I64, _I32, _P], _I32),
     "vh_tree_masks": ([_P, _I64, _I32, _P, _P, _P], _I32),
-    # vh_tree_attention takes a vh_tree_desc*; voyager_amd.speculative.TreeDesc mirrors it.
-    "vh_tree_attention": ([_P, _P], _I32),
+    "vh_tree_attention": ([_P, _P, _I64, _P], _I32),
     "vh_tree_attention_workspace_bytes": ([_P], _I64),
-    "vh_verify": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I32, _I64, _P, _P, _P, _P, _I64, _P], _I32),
+    "vh_verify": ([_P, _P, _I64, _P], _I32),
     "vh_verify_workspace_bytes": ([_I64, _I64], _I64),
 }
 

@@ -46,7 +46,7 @@ class CacheFlag:
 
 
 def _int32(t: torch.Tensor, shape: Tuple[int, ...], device, what: str) -> None:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+    if t.shape != shape or t.dtype is not torch.int32 or t.device != device:
         raise ValueError(f"{what} must be int32 {list(shape)} on {device} (got {t.dtype} {list(t.shape)} on {t.device})")
 
 
@@ -86,6 +86,8 @@ class PagedCache:
         self.c = _lib.Cache(self.k.data_ptr(), self.v.data_ptr(), ptr(self.k_scale), ptr(self.v_scale),
                             self.flag.t.data_ptr(), pages * page, pages, page, kv_heads, dim, code)
         self._c = ctypes.byref(self.c)
+        self._bytes = bytes(self.c)
+        self._work = {}  # tree_attention's workspace, by its sizes
         self._dtype_code = dtype_code(dtype)
 
     def check(self) -> None:
@@ -93,7 +95,7 @@ class PagedCache:
         self.flag.check("PagedCache")
 
     def _slots(self, slots: torch.Tensor) -> int:
-        if slots.dtype != torch.int64 or slots.dim() != 1 or slots.device != self.device:
+        if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.device != self.device:
             raise ValueError(f"PagedCache: slots must be int64 [tokens] on {self.device} (got {slots.dtype} "
                              f"{list(slots.shape)} on {slots.device})")
         return slots.shape[0]
@@ -103,20 +105,24 @@ class PagedCache:
         [tokens]`` (int64, all different; negative: a token that pads, left
         out).  Views with dense channels are read in place."""
         n = self._slots(slots)
-        if k.requires_grad or v.requires_grad:
-            if torch.is_grad_enabled():
-                raise RuntimeError("PagedCache.write: the cache passes no gradient; write under torch.no_grad()")
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            raise RuntimeError("PagedCache.write: the cache passes no gradient; write under torch.no_grad()")
+        shape = (n, self.kv_heads, self.dim)
         for name, t in (("k", k), ("v", v)):
-            if t.dtype != self.dtype or t.device != self.device or t.shape != (n, self.kv_heads, self.dim):
+            if t.shape != shape or t.dtype is not self.dtype or t.device != self.device:
                 raise ValueError(f"PagedCache.write: {name} must be {self.dtype} [{n}, {self.kv_heads}, {self.dim}] on "
                                  f"{self.device} (got {t.dtype} {list(t.shape)} on {t.device})")
-        if k.stride(2) != 1:
+        k_st, k_sh, k_sc = k.stride()
+        if k_sc != 1:
             k = k.contiguous()
-        if v.stride(2) != 1:
+            k_st, k_sh, _ = k.stride()
+        v_st, v_sh, v_sc = v.stride()
+        if v_sc != 1:
             v = v.contiguous()
+            v_st, v_sh, _ = v.stride()
         slots = slots.contiguous()
-        st = load().vh_paged_write(self._c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                   v.stride(1), self._dtype_code, slots.data_ptr(), n, stream_on(self.device))
+        st = load().vh_paged_write(self._c, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, self._dtype_code,
+                                   slots.data_ptr(), n, stream_on(self.device))
         if st:
             check(st, "vh_paged_write")
 

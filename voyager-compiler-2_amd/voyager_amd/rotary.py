@@ -10,13 +10,18 @@ chain's roundings.
 """
 
 import math
+import struct
 from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import check, dtype_code, load, ptr, stream_on
+from ._lib import check, dtype_code, load, stream_on
 
 MAX_DIM = 512
+#: ``vh_rope_desc``: up to ``inverse``, which a call gives, and the rest, which the embedding does
+ROPE = struct.Struct("@QQqqqQQqqqQqqqqiiiii")
+_ROPE_REST = struct.Struct("=iiif4xQ")
+_NONE = (0, 0, 0, 0, 0, 0)
 
 _SCALING = {"linear": (), "ntk": (), "bands": ("low", "high", "trained"), "yarn": ("low", "high", "trained")}
 
@@ -85,6 +90,8 @@ class Rotary:
         self.dim, self.rotary_dim, self.interleaved = dim, rotary_dim, bool(interleaved)
         f, self.factor = frequencies(rotary_dim, theta, scaling)
         self.turns = (f / (2 * math.pi)).to(device)  # per position: the kernel drops whole turns in float64
+        self._rest = _ROPE_REST.pack(dim, rotary_dim, 1 if interleaved else 0, self.factor, self.turns.data_ptr())
+        self._checked = None
 
     def __call__(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor):
         """``q [batch, tokens, heads, dim]`` and ``k [batch, tokens, kv_heads,
@@ -92,7 +99,11 @@ class Rotary:
         ``[tokens]`` (int32 or int64), contiguous, of the inputs' dtype
         (bfloat16, float16 or float32).  Views with dense channels are read in
         place.  Differentiable in q and k, any number of times."""
-        self._check(q, k, positions)
+        given = (None if q is None else (q.shape, q.dtype, q.device), None if k is None else (k.shape, k.dtype, k.device),
+                 positions.shape, positions.dtype, positions.device)
+        if given != self._checked:  # a step's sizes are mostly those of the step before
+            self._check(q, k, positions)
+            self._checked = given
         if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
             return _Turn.apply(q, k, positions, self, False)
         return self._turn(q, k, positions, False)
@@ -119,23 +130,29 @@ class Rotary:
                              f"{list(x.shape[:2])})")
 
     def _turn(self, q, k, positions, inverse: bool):
-        def given(t):
-            if t is None:
-                return None, None, (0, 0, 0, 0), 0
-            if t.stride(3) != 1:
-                t = t.contiguous()
-            return t, torch.empty(t.shape, dtype=t.dtype, device=t.device), t.stride(), t.shape[2]
-
-        q, qo, qs, nq = given(q)
-        k, ko, ks, nk = given(k)
-        x = q if q is not None else k
+        qo = ko = None
+        qd = kd = _NONE
+        x = k
+        if k is not None:
+            if k.stride(3) != 1:
+                k = k.contiguous()
+            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+            sb, st, sh, _ = k.stride()
+            kd = (k.data_ptr(), ko.data_ptr(), sb, st, sh, k.shape[2])
+        if q is not None:
+            if q.stride(3) != 1:
+                q = q.contiguous()
+            qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+            sb, st, sh, _ = q.stride()
+            qd = (q.data_ptr(), qo.data_ptr(), sb, st, sh, q.shape[2])
+            x = q
+        batch, tokens, _, _ = x.shape
+        ps = positions.stride()
         # one position a token for all sequences: no step from one to the next
-        step = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-        st = load().vh_rope(ptr(q), ptr(qo), qs[0], qs[1], qs[2], ptr(k), ptr(ko), ks[0], ks[1], ks[2],
-                            dtype_code(x.dtype), x.shape[0], x.shape[1], nq, nk, self.dim, self.rotary_dim,
-                            1 if self.interleaved else 0, positions.data_ptr(), 8 * positions.element_size(), step,
-                            positions.stride(-1), self.turns.data_ptr(), self.factor, 1 if inverse else 0,
-                            stream_on(x.device))
+        step = ps[0] if len(ps) == 2 and positions.shape[0] > 1 else 0
+        d = ROPE.pack(*qd[:5], *kd[:5], positions.data_ptr(), step, ps[-1], batch, tokens, qd[5], kd[5], dtype_code(x.dtype),
+                      64 if positions.dtype is torch.int64 else 32, 1 if inverse else 0) + self._rest
+        st = load().vh_rope(d, stream_on(x.device))
         if st:
             check(st, "vh_rope")
         return qo, ko
@@ -161,5 +178,8 @@ class _Turn(torch.autograd.Function):
         if gq is None and gk is None:
             return None, None, None, None, None
         (positions,) = ctx.saved_tensors
-        gq, gk = _Turn.apply(gq, gk, positions, ctx.rotary, not ctx.inverse)
+        if torch.is_grad_enabled():  # the gradient's own graph is wanted
+            gq, gk = _Turn.apply(gq, gk, positions, ctx.rotary, not ctx.inverse)
+        else:
+            gq, gk = ctx.rotary._turn(gq, gk, positions, not ctx.inverse)
         return gq, gk, None, None, None

@@ -10,7 +10,7 @@ Kept rows are then moved together by :meth:`paged.PagedCache.keep`.  Nothing
 synchronises and every launch goes on torch's current stream.
 """
 
-import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -22,20 +22,9 @@ from .paged import CacheFlag, PagedCache, _int32, _rows
 MAX_NODES = _lib.TREE_MAX_NODES
 
 
-class TreeDesc(ctypes.Structure):
-    """``vh_tree_desc``."""
-
-    _fields_ = [
-        ("cache", _lib.Cache),
-        ("q", ctypes.c_void_p), ("q_sb", ctypes.c_int64), ("q_st", ctypes.c_int64), ("q_sh", ctypes.c_int64),
-        ("table", ctypes.c_void_p), ("table_st", ctypes.c_int64),
-        ("context", ctypes.c_void_p), ("masks", ctypes.c_void_p),
-        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-        ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64),
-        ("scale", ctypes.c_float),
-        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("nodes", ctypes.c_int32), ("heads", ctypes.c_int32),
-        ("table_pages", ctypes.c_int32), ("workgroups", ctypes.c_int32),
-    ]
+#: ``vh_tree_desc`` after its cache, and ``vh_verify_desc``
+TREE = struct.Struct("@QqqqQqQQQQfiiiiii4x")
+VERIFY = struct.Struct("@QqqQqqQQQQqqqQQQ")
 
 
 class Tree:
@@ -83,35 +72,44 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, cont
     the logarithm of each row's sum of exponentials (float32 ``[batch, nodes,
     heads]``).  Rows that see nothing give 0 and -inf.  Heads of 64, 128 or 256
     channels, pages of a multiple of 16 tokens.  No gradient: it reads a cache."""
-    if q.dim() != 4 or q.shape[3] != cache.dim or q.dtype != cache.dtype or q.device != cache.device:
-        raise ValueError(f"tree_attention: q must be {cache.dtype} [batch, nodes, heads, {cache.dim}] on {cache.device} "
+    dev = cache.device
+    if q.dim() != 4 or q.shape[3] != cache.dim or q.dtype is not cache.dtype or q.device != dev:
+        raise ValueError(f"tree_attention: q must be {cache.dtype} [batch, nodes, heads, {cache.dim}] on {dev} "
                          f"(got {q.dtype} {list(q.shape)} on {q.device})")
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("tree_attention: passes no gradient; call it under torch.no_grad()")
     b, t, heads, dim = q.shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"tree_attention: {heads} query heads over {cache.kv_heads} of the cache")
-    _int32(context, (b,), cache.device, "tree_attention: context")
-    _int32(table, (b, table.shape[-1]), cache.device, "tree_attention: table")
-    if tree is not None and (tree.batch != b or tree.nodes != t or tree.device != cache.device):
-        raise ValueError(f"tree_attention: a tree of [{tree.batch}, {tree.nodes}] on {tree.device} for queries [{b}, {t}]")
-    if q.stride(3) != 1:
+    _int32(context, (b,), dev, "tree_attention: context")
+    _int32(table, (b, table.shape[-1]), dev, "tree_attention: table")
+    masks = 0
+    if tree is not None:
+        if tree.batch != b or tree.nodes != t or tree.device != dev:
+            raise ValueError(f"tree_attention: a tree of [{tree.batch}, {tree.nodes}] on {tree.device} for queries [{b}, {t}]")
+        masks = tree.masks.data_ptr()
+    sb, st, sh, sc = q.stride()
+    if sc != 1:
         q = q.contiguous()
+        sb, st, sh, _ = q.stride()
     table, context = _rows(table), _rows(context)
-    o = torch.empty(b, t, heads, dim, dtype=q.dtype, device=q.device)
-    lse = torch.empty(b, t, heads, dtype=torch.float32, device=q.device) if return_lse else None
-    sb, st, sh, _ = q.stride()
-    d = TreeDesc(cache.c, q.data_ptr(), sb, st, sh, table.data_ptr(), table.stride(0), context.data_ptr(),
-                 None if tree is None else tree.masks.data_ptr(), o.data_ptr(), None if lse is None else lse.data_ptr(),
-                 None, 0, dim ** -0.5 if scale is None else float(scale), cache._dtype_code, b, t, heads,
-                 table.shape[1], 0)
-    ref = ctypes.byref(d)
+    pages = table.shape[1]
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(b, t, heads, dtype=torch.float32, device=dev) if return_lse else None
+    d = cache._bytes + TREE.pack(q.data_ptr(), sb, st, sh, table.data_ptr(), table.stride(0), context.data_ptr(), masks,
+                                 o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                 dim ** -0.5 if scale is None else scale, cache._dtype_code, b, t, heads, pages, 0)
     lib = load()
-    need = lib.vh_tree_attention_workspace_bytes(ref)
-    if need > 0:
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        d.work, d.work_bytes = work.data_ptr(), need
-    rc = lib.vh_tree_attention(ref, stream_on(q.device))
+    sizes = (b, t, heads, pages)
+    need = cache._work.get(sizes)
+    if need is None:
+        need = lib.vh_tree_attention_workspace_bytes(d)
+        if need >= 0:  # or the call says what is wrong
+            if len(cache._work) >= 4096:
+                cache._work.clear()
+            cache._work[sizes] = need
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    rc = lib.vh_tree_attention(d, None if work is None else work.data_ptr(), need, stream_on(dev))
     if rc:
         check(rc, "vh_tree_attention")
     return (o, lse) if return_lse else o
@@ -137,35 +135,32 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tens
     Returns ``told [batch, nodes]`` (int64: the tokens taken, then the last; -1
     after them), ``path [batch, nodes]`` (int32: the first node and those taken;
     -1 after them) and ``count [batch]`` (int32: how many of each)."""
-    b, t = tree.batch, tree.nodes
-    dev = tree.device
-    for name, x in (("target", target), ("draft", draft)):
-        if x is None:
-            continue
-        if x.dim() != 3 or x.shape[:2] != (b, t) or x.shape != target.shape or x.dtype != torch.float32 or x.device != dev:
-            raise ValueError(f"verify: {name} must be float32 [{b}, {t}, vocab] on {dev} (got {x.dtype} {list(x.shape)} on "
-                             f"{x.device})")
-    if target.shape[2] == 0:
-        raise ValueError("verify: an empty vocabulary")
-    for name, x, shape, dtype in (("tokens", tokens, (b, t), torch.int64), ("u", u, (b, t), torch.float32),
+    b, t, dev = tree.batch, tree.nodes, tree.device
+    vocab = target.shape[-1] if target.dim() == 3 else 0
+    for name, x, shape, dtype in (("target", target, (b, t, vocab), torch.float32), ("draft", draft, (b, t, vocab), torch.float32),
+                                  ("tokens", tokens, (b, t), torch.int64), ("u", u, (b, t), torch.float32),
                                   ("r", r, (b,), torch.float32)):
-        if x.dtype != dtype or x.shape != shape or x.device != dev:
+        if x is not None and (x.shape != shape or x.dtype is not dtype or x.device != dev):
             raise ValueError(f"verify: {name} must be {dtype} {list(shape)} on {dev} (got {x.dtype} {list(x.shape)} on "
                              f"{x.device})")
+    if vocab == 0:
+        raise ValueError("verify: an empty vocabulary")
     target = _rows(target)
-    draft = None if draft is None else _rows(draft)
+    tb, tn, _ = target.stride()
+    q, qb, qn = 0, 0, 0
+    if draft is not None:
+        draft = _rows(draft)
+        q, (qb, qn, _) = draft.data_ptr(), draft.stride()
     tokens, u, r = tokens.contiguous(), u.contiguous(), r.contiguous()
-    told = torch.empty(b, t, dtype=torch.int64, device=dev)
-    path = torch.empty(b, t, dtype=torch.int32, device=dev)
+    told = torch.empty_like(tokens)
+    path = torch.empty_like(tree.parents)
     count = torch.empty(b, dtype=torch.int32, device=dev)
     lib = load()
-    need = lib.vh_verify_workspace_bytes(b, target.shape[2])
-    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    ds = (0, 0) if draft is None else draft.stride()
-    st = lib.vh_verify(target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(),
-                       ds[0], ds[1], tree.parents.data_ptr(), tokens.data_ptr(), u.data_ptr(), r.data_ptr(), b, t,
-                       target.shape[2], told.data_ptr(), path.data_ptr(), count.data_ptr(), work.data_ptr(),
-                       work.numel(), stream_on(dev))
+    need = lib.vh_verify_workspace_bytes(b, vocab)
+    work = torch.empty(need, dtype=torch.uint8, device=dev)
+    st = lib.vh_verify(VERIFY.pack(target.data_ptr(), tb, tn, q, qb, qn, tree.parents.data_ptr(), tokens.data_ptr(),
+                                   u.data_ptr(), r.data_ptr(), b, t, vocab, told.data_ptr(), path.data_ptr(),
+                                   count.data_ptr()), work.data_ptr(), need, stream_on(dev))
     if st:
         check(st, "vh_verify")
     return told, path, count
