@@ -54,6 +54,7 @@ struct Splits {
 VH_DEV Splits splits_before(const Args& a, int b) {
   Splits s{0u, 1u};
   const uint32_t chunk = tree::chunk_of(a);
+  if (a.batch == 1) return Splits{0u, tree::splits_of(tree::pieces(a, 0), chunk)};
   const int lane = threadIdx.x & 63;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const uint32_t n = b0 + lane < a.batch ? tree::splits_of(tree::pieces(a, b0 + lane), chunk) : 0u;

@@ -98,9 +98,13 @@ VH_DEV uint32_t pieces(const Args& a, int b) {
 VH_DEV uint32_t chunk_of(const Args& a) {
   const int lane = threadIdx.x & 63;
   uint32_t all = 0u;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) all += pieces(a, b0 + lane);
+  if (a.batch == 1) {
+    all = pieces(a, 0);
+  } else {
+    for (int b0 = 0; b0 < a.batch; b0 += 64) all += pieces(a, b0 + lane);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) all += (uint32_t)__shfl_xor((int)all, d);
+    for (int d = 1; d < 64; d *= 2) all += (uint32_t)__shfl_xor((int)all, d);
+  }
   all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
   return all == 0u ? 1u : (all + a.share - 1) / a.share;
 }
@@ -113,6 +117,13 @@ struct Span {
 };
 VH_DEV Span span_of(const Args& a, uint32_t unit) {
   Span s{-1, 0u, chunk_of(a)};
+  if (a.batch == 1) {  // the scan over sequences is a microsecond of a lone token's
+    if (unit < splits_of(pieces(a, 0), s.chunk)) {
+      s.b = 0;
+      s.split = unit;
+    }
+    return s;
+  }
   const int lane = threadIdx.x & 63;
   uint32_t before = 0u;
   for (int b0 = 0; b0 < a.batch && s.b < 0; b0 += 64) {
