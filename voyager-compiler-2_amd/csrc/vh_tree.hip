@@ -159,7 +159,7 @@ void merge(const Args& a, hipStream_t s) {
 struct Plan {
   bool wide;
   int n, block_rows, row_blocks;  // n: tiles of 16 rows a wave, or waves of rows
-  uint32_t share, units;
+  uint32_t share, fill, units;
   int64_t part;  // rows of partial results
 };
 
@@ -190,6 +190,8 @@ Plan plan_of(const vh_tree_desc* d) {
   if (share < 1) share = 1;
   if (share > most * d->batch) share = most * d->batch > 0 ? most * d->batch : 1;
   p.share = (uint32_t)share;
+  const int64_t fill = 256 / blocks;
+  p.fill = (uint32_t)(d->workgroups > 0 || fill > share ? share : fill > 1 ? fill : 1);
   // one share: every sequence is one split, and its results are final
   int64_t units = share == 1 ? d->batch : share + d->batch;
   if (units > most * d->batch && most > 0) units = most * d->batch;
@@ -278,6 +280,7 @@ extern "C" int vh_tree_attention(const vh_tree_desc* d, void* work, int64_t work
   a.block_rows = p.block_rows;
   a.table_pages = d->table_pages;
   a.share = p.share;
+  a.fill = p.fill;
   a.units = p.units;
   VH_REQUIRE(((int64_t)p.units * a.c.kv_heads + 7) / 8 * 8 * a.row_blocks < (1ll << 31) &&
                  (int64_t)a.batch * a.c.kv_heads * a.rows < (1ll << 31),

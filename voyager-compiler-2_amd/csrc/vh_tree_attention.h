@@ -73,7 +73,7 @@ struct Args {
   float scale;                 // times log2(e)
   int q_bf16, q_wide, words, batch, nodes, heads, group, rows, row_blocks, block_rows;
   int table_pages;
-  uint32_t share;              // workgroups that a row block's keys are shared out to, of all sequences
+  uint32_t share, fill;        // workgroups that a row block's keys are shared out to at most; that fill the card
   uint32_t units;              // most splits of all sequences together
 };
 
@@ -87,10 +87,13 @@ VH_DEV int visible(const Args& a, int ctx, int row0) {
   return fits(a, ctx) ? ctx + (int)fast_div((uint32_t)(last - 1), a.group_div) + 1 : 0;
 }
 
-// How the sequences fall into splits: `chunk` pieces of PIECE keys each, the
-// least with which all pieces fill no more than `share` splits and a rest a
-// sequence.  Every lane of a wave calls these together; a lane holds a sequence.
-constexpr int PIECE = 128;
+// How the sequences fall into splits of `chunk` pieces of PIECE keys: the least
+// with which all pieces make no more than `share` splits and a rest a sequence,
+// and four where that still makes `fill`, so that a wave has steps to ask ahead
+// in and a split's results are few beside its keys (8 sequences of 8192, heads
+// of 256, two tokens: 44 us at one piece a split, 32 at three).  Every lane of a
+// wave calls these together; a lane holds a sequence.
+constexpr int PIECE = 128, CHUNK = 4;
 VH_DEV uint32_t pieces(const Args& a, int b) {
   const int ctx = b < a.batch ? a.context[b] : -1;
   return fits(a, ctx) && b < a.batch ? ((uint32_t)ctx + a.nodes + PIECE - 1) / PIECE : 0u;
@@ -106,7 +109,9 @@ VH_DEV uint32_t chunk_of(const Args& a) {
     for (int d = 1; d < 64; d *= 2) all += (uint32_t)__shfl_xor((int)all, d);
   }
   all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
-  return all == 0u ? 1u : (all + a.share - 1) / a.share;
+  if (all == 0u) return 1u;
+  const uint32_t least = (all + a.share - 1) / a.share;
+  return least >= CHUNK ? least : max(least, min((uint32_t)CHUNK, (all + a.fill - 1) / a.fill));
 }
 VH_DEV uint32_t splits_of(uint32_t piece, uint32_t chunk) { return piece <= chunk ? 1u : (piece + chunk - 1) / chunk; }
 
@@ -767,10 +772,14 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
         uint4 P[NT], Plo[NT];
         const uint32_t all[NT] = {};
         products(S);
-        if (__any(quick<FMT>(S, ks, vs, fac, m, T, p))) break;
+        const f32x4 k1[2] = {ks[0], ks[1]};
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
+        if (__any(quick<FMT>(S, k1, vs, fac, m, T, p))) {
+          load_k(st);  // once more, seldom
+          break;
+        }
         operands<FMT, SPLIT, false>(p, vs, T, all, l, P, Plo);
         add(P, Plo);
         __builtin_amdgcn_sched_barrier(0);
