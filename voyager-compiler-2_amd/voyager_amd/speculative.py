@@ -46,6 +46,7 @@ class Tree:
         self.parents = parents.contiguous()
         self.device = parents.device
         self.flag = CacheFlag(parents.device)
+        self._checked = None
         #: bit m of word m // 64: node m is on the way from the root to the node (itself included)
         self.masks = torch.empty(self.batch, self.nodes, -(-self.nodes // 64), dtype=torch.int64, device=parents.device)
         st = load().vh_tree_masks(self.parents.data_ptr(), self.batch, self.nodes, self.masks.data_ptr(),
@@ -136,15 +137,20 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tens
     after them), ``path [batch, nodes]`` (int32: the first node and those taken;
     -1 after them) and ``count [batch]`` (int32: how many of each)."""
     b, t, dev = tree.batch, tree.nodes, tree.device
-    vocab = target.shape[-1] if target.dim() == 3 else 0
-    for name, x, shape, dtype in (("target", target, (b, t, vocab), torch.float32), ("draft", draft, (b, t, vocab), torch.float32),
-                                  ("tokens", tokens, (b, t), torch.int64), ("u", u, (b, t), torch.float32),
-                                  ("r", r, (b,), torch.float32)):
-        if x is not None and (x.shape != shape or x.dtype is not dtype or x.device != dev):
-            raise ValueError(f"verify: {name} must be {dtype} {list(shape)} on {dev} (got {x.dtype} {list(x.shape)} on "
-                             f"{x.device})")
-    if vocab == 0:
-        raise ValueError("verify: an empty vocabulary")
+    given = tuple(None if x is None else (x.shape, x.dtype, x.device) for x in (target, tokens, u, r, draft))
+    if given != tree._checked:  # a step's sizes are mostly those of the step before
+        vocab = target.shape[-1] if target.dim() == 3 else 0
+        for name, x, shape, dtype in (("target", target, (b, t, vocab), torch.float32),
+                                      ("draft", draft, (b, t, vocab), torch.float32),
+                                      ("tokens", tokens, (b, t), torch.int64), ("u", u, (b, t), torch.float32),
+                                      ("r", r, (b,), torch.float32)):
+            if x is not None and (x.shape != shape or x.dtype is not dtype or x.device != dev):
+                raise ValueError(f"verify: {name} must be {dtype} {list(shape)} on {dev} (got {x.dtype} {list(x.shape)} on "
+                                 f"{x.device})")
+        if vocab == 0:
+            raise ValueError("verify: an empty vocabulary")
+        tree._checked = given
+    vocab = target.shape[2]
     target = _rows(target)
     tb, tn, _ = target.stride()
     q, qb, qn = 0, 0, 0
@@ -154,7 +160,7 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tens
     tokens, u, r = tokens.contiguous(), u.contiguous(), r.contiguous()
     told = torch.empty_like(tokens)
     path = torch.empty_like(tree.parents)
-    count = torch.empty(b, dtype=torch.int32, device=dev)
+    count = torch.empty_like(r, dtype=torch.int32)
     lib = load()
     need = lib.vh_verify_workspace_bytes(b, vocab)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
