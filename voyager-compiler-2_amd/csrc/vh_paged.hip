@@ -9,7 +9,10 @@
 // reads back as NaN everywhere and no code has to stand for it.
 //
 // Bound by memory: a value is read once in 16 bits and written once in 8, or
-// the reverse.
+// the reverse.  8 heads of 128, E4M3, 32768 tokens in a shuffled order of
+// slots: written in 42-43 us (204 MB, 4.8 TB/s), read back in 30.7 (204 MB,
+// the codes still in the last cache); 4001 tokens, int8, 8.0 and 6.0 us
+// (25 MB each); 8 tokens 3.2 and 3.0 us, one load's and one store's latency.
 #include <hip/hip_runtime.h>
 
 #include "vh_device.h"
@@ -99,7 +102,9 @@ VH_DEV void paged_decode(uint2 c, float scale, float (&x)[8]) {
 // A workgroup takes consecutive tokens of one head; `group` lanes a token (a
 // power of two, so that a row's maximum stays inside it), 8 values a lane, its
 // key and its value.  Heads are the fastest index of the grid: the rows of a
-// token are read by workgroups that run together.
+// token are read by workgroups that run together.  A lane reads 16 bytes and
+// writes 8, so a wave covers whole rows on both sides, and the row's maximum is
+// a few exchanges between neighbours, without LDS.
 template <typename T, int FMT, bool WIDE>
 __global__ void __launch_bounds__(PAGED_THREADS) k_paged_write(PagedArgs a, int group) {
   const int h = blockIdx.x % a.c.kv_heads;

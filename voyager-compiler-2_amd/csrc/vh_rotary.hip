@@ -11,7 +11,11 @@
 // the float64 one by less than 1e-9.  Sine and cosine are taken in float32 of
 // the fraction, once per token and pair, and shared by all heads through LDS.
 //
-// Bound by memory: 4 bytes moved per bfloat16 value, 3 operations.
+// Bound by memory: 4 bytes moved per bfloat16 value, 3 operations.  32 + 8
+// heads of 128 in bfloat16: 8192 tokens (168 MB read and written) 29-33 us,
+// 5.1-5.8 TB/s with part of it in the last cache; a single token 2.5 us, its
+// loads' and the launch's latency.  5001 tokens of 16 + 4 heads of 128 in
+// float32, half of each turned (102 MB): 17.3 us.
 #include <hip/hip_runtime.h>
 
 #include "vh_device.h"
@@ -156,10 +160,12 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a) {
 template <typename T, int VEC>
 void rope_launch(const RopeArgs& a, bool interleaved, hipStream_t s) {
   const int heads = a.nq + a.nk;
-  // Many tokens: four a workgroup share the launch's cost.  Few: one each,
-  // its heads over several workgroups, so that a single token's load and
-  // store are one trip each.
-  if (a.rows >= 1024) {
+  // Many tokens: four a workgroup share the launch's cost, and fill it where
+  // heads are few.  Fewer: one each, its heads over several workgroups, so that
+  // a token's load and store are one trip each.  (us with four and with one;
+  // 32 + 8 heads of 128: 64 tokens 5.6 and 3.1, 1024 6.8 and 5.7, 2048 9.4 and
+  // 9.2, 8192 28.1 and 28.9; 8 + 1 heads: 1024 4.1 and 3.6, 16384 14.8 and 21.6.)
+  if (a.rows >= 2048) {
     const dim3 grid((unsigned)((a.rows + ROPE_TOKENS - 1) / ROPE_TOKENS));
     if (interleaved) hipLaunchKernelGGL((k_rope<T, VEC, true, ROPE_TOKENS>), grid, dim3(ROPE_THREADS), 0, s, a);
     else hipLaunchKernelGGL((k_rope<T, VEC, false, ROPE_TOKENS>), grid, dim3(ROPE_THREADS), 0, s, a);
@@ -171,7 +177,8 @@ void rope_launch(const RopeArgs& a, bool interleaved, hipStream_t s) {
   }
 }
 
-// Whether 16-byte accesses of VEC values are aligned in this tensor.
+// Whether 16-byte accesses of VEC values are aligned in this tensor; if not,
+// values are taken one by one.
 bool rope_aligned(const RopeTensor& t, int vec) {
   return (uintptr_t)t.x % 16 == 0 && (uintptr_t)t.y % 16 == 0 && t.sb % vec == 0 && t.st % vec == 0 && t.sh % vec == 0;
 }

@@ -146,13 +146,17 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
                : make_uint2(tree::pack2<CACHE_F16>(o[0], o[1]), tree::pack2<CACHE_F16>(o[2], o[3]));
 }
 
-// Many splits a sequence and few rows: a workgroup a row.  Else as many rows as
-// fit one.
+// Many splits a sequence and few rows: a workgroup a row, whose groups share the
+// splits.  Else as many rows as fit one: rows alone fill the card then.  (us of
+// attention and joining, by the first and the second: 32 rows of 41 splits 10.6
+// and 14.2, 512 of 72 22.8 and 25.9, 832 of 32 65.6 and 67.0; 4096 of 64 42.8 and 36.6,
+// 16384 of 8 96.4 and 72.7.)  Joining 16384 rows of 8 splits reads 68 MB in
+// 10.2 us, the most of it from the last cache.
 template <int D>
 void merge(const Args& a, hipStream_t s) {
   constexpr int ALL = 1024 / D;  // groups of lanes in a workgroup
   const int64_t rows = (int64_t)a.batch * a.c.kv_heads * a.rows;
-  if (a.units >= 8 * (uint32_t)a.batch && rows <= 4096) hipLaunchKernelGGL((k_tree_merge<D, ALL>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  if (a.units >= 8 * (uint32_t)a.batch && rows <= 1024) hipLaunchKernelGGL((k_tree_merge<D, ALL>), dim3((unsigned)rows), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_tree_merge<D, 1>), dim3((unsigned)((rows + ALL - 1) / ALL)), dim3(256), 0, s, a);
 }
 
@@ -164,7 +168,11 @@ struct Plan {
 };
 
 // The shape of the launch.  Up to 32 rows of a key head (16 of heads of 256)
-// a wave holds them all and takes its own keys; more share converted keys.
+// a wave holds them all and takes its own keys; more share converted keys.  (us
+// by the first and the second, 4 sequences of 8192 over 8 key heads of 128,
+// E4M3: 8 rows 22.9 and 32.5, 32 rows 29.5 and 34.7, 48 rows 43.4 and 35.8; 4
+// heads of 256: 16 rows 24.1 and 32.0, 32 rows 30.8 and 33.1, but with 16
+// sequences 91 and 72, and of 16-bit keys 168 and 113.)
 Plan plan_of(const vh_tree_desc* d) {
   Plan p;
   const int64_t rows = (int64_t)d->nodes * (d->heads / d->cache.kv_heads);
@@ -183,8 +191,8 @@ Plan plan_of(const vh_tree_desc* d) {
   const int64_t blocks = (int64_t)d->cache.kv_heads * p.row_blocks;
   // Two workgroups a CU hold their registers where rows are many, and each more
   // share costs its rows' partial results twice; single tokens' keys fill the
-  // card best at six, whose results are few.  (8 trees of 64 over 4096: 83 us at
-  // 1024, 69 at 512, 89 at 256; 32 tokens over 8192: 91 us at 512, 83 at 1536.)
+  // card best at six, whose results are few.  (8 trees of 64 over 4096: 80 us at
+  // 1024, 67 at 512, 84 at 256; 32 tokens over 8192: 88 us at 512, 84 at 1536.)
   const int64_t slots = d->workgroups > 0 ? d->workgroups : p.wide ? 512 : 1536;
   int64_t share = slots / blocks;
   if (share < 1) share = 1;
