@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
 
 // Many splits a sequence and few rows: a workgroup a row, whose groups share the
 // splits.  Else as many rows as fit one: rows alone fill the card then.  (us of
-// attention and joining, by the first and the second: 32 rows of 41 splits 10.6
-// and 14.2, 512 of 72 22.8 and 25.9, 832 of 32 65.6 and 67.0; 4096 of 64 42.8 and 36.6,
-// 16384 of 8 96.4 and 72.7.)  Joining 16384 rows of 8 splits reads 68 MB in
+// attention and joining, by the first and the second: 32 rows of 32 splits 10.6
+// and 14.2, 512 of 64 22.8 and 25.9, 832 of 32 65.6 and 67.0; 4096 of 8 42.8 and
+// 36.6, 16384 of 4 or 5 96.4 and 72.7.)  Joining these 16384 rows reads 42 MB in
 // 10.2 us, the most of it from the last cache.
 template <int D>
 void merge(const Args& a, hipStream_t s) {
