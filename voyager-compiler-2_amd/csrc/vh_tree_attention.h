@@ -883,9 +883,10 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 //
 // 8 trees of 64 nodes over 1024 to 4096 cached tokens, 8 E4M3 key heads of 128
 // and 32 query heads (56 MB, 24 GFLOP): 50-69 us, 0.34-0.47 PFLOP/s.  The vector
-// instructions bound it (softmax, conversion and operand reads: half of all
-// cycles, the matrix instructions a quarter), with about 15 us before the first
-// product and after the last.  2 of 13 nodes over 8192 to 32768 in float16
+// instructions and LDS bound it (softmax, conversion and operand reads: each
+// half of all cycles, the matrix instructions a third; 0.77 PFLOP/s from one
+// length to the next), with about 18 us before the first product and after the
+// last.  2 of 13 nodes over 8192 to 32768 in float16
 // (218 MB): 46 us, 4.7 TB/s.
 template <int D>
 constexpr int wide_nt() { return D <= 128 ? 2 : 1; }
@@ -1179,6 +1180,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         // The quick form of the softmax, written out so that nothing waits:
         // operands are read AHEAD of their products, and the last step's second
         // products are issued between this step's softmax, two scores at a time.
+        // A step is given up where a lane's sum passes 2^13: its terms are no more.
         constexpr int AHEAD = 4, TN = 2 * SUB;                // TN: 16-key tiles
         constexpr int KF = KS * TN, VF = CT * SUB, HALVES = TN * NT * 2;
         const Stage& in = s_stage[half];
@@ -1186,11 +1188,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         f32x4 S[TN][NT];
         uint32_t w[TN][NT][2], u[TN][NT][2];
         f32x4 ks[2], vs[2];  // of this 16-key tile and the next
-        float sum[NT], top[NT], high = 0.0f;
+        float sum[NT], high = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          sum[nt] = l[nt];
-          top[nt] = 0.0f;
+          sum[nt] = 0.0f;
 #pragma unroll
           for (int t = 0; t < TN; ++t) S[t][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -1216,7 +1217,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           }
           const float f0 = BYTE ? ks[t % 2][i] * fac[nt] : fac[nt], f1 = BYTE ? ks[t % 2][i + 1] * fac[nt] : fac[nt];
           float p0 = exp2_fast(fmaf(S[t][nt][i], f0, -m[nt])), p1 = exp2_fast(fmaf(S[t][nt][i + 1], f1, -m[nt]));
-          top[nt] = fmaxf(fmaxf(top[nt], p0), p1);
           sum[nt] += p0 + p1;
           if constexpr (BYTE) {
             p0 *= vs[t % 2][i];
@@ -1226,7 +1226,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           if constexpr (SPLIT) {
             const f32x2 hi = unpack2<FMT>(w[t][nt][n % 2]);
             u[t][nt][n % 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
+            asm volatile("" : "+v"(u[t][nt][n % 2]));
           }
+          // here, between the products: the compiler would leave them for after the loop's exit
+          asm volatile("" : "+v"(w[t][nt][n % 2]), "+v"(sum[nt]));
         };
         uint4 f[AHEAD];
 #pragma unroll
@@ -1255,7 +1258,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         }
         bool far = BYTE && high > T;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) far |= top[nt] > 0x1p13f || m[nt] == -__builtin_inff();
+        for (int nt = 0; nt < NT; ++nt) far |= sum[nt] > 0x1p13f || m[nt] == -__builtin_inff();
         pending = false;
         if (__any(far)) {
           fed = true;
@@ -1264,7 +1267,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         pending = true;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          l[nt] = sum[nt];
+          l[nt] += sum[nt];
 #pragma unroll
           for (int v = 0; v < SUB; ++v) {
             P[v][nt] = make_uint4(w[2 * v][nt][0], w[2 * v][nt][1], w[2 * v + 1][nt][0], w[2 * v + 1][nt][1]);
