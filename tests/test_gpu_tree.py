@@ -279,3 +279,32 @@ def test_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, exp)), f"replay {i}"
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("t", [2, 20])
+def test_pages_past_32_bits(fmt, t):
+    """The last pages of a cache whose keys alone are over 4 GiB: written,
+    attended to, moved and read as those of a small one are."""
+    kv, d, page, per = 8, 256, 64, 4
+    b = 2
+    count = (1 << 32) // (kv * d * page * (1 if fmt else 2)) + 16
+    g = torch.Generator().manual_seed(15)
+    x = torch.randn(2, b * per * page, kv, d, generator=g).bfloat16().cuda()
+    q = torch.randn(b, t, 16, d, generator=g).bfloat16().cuda()
+    context = torch.tensor([per * page - t, 77], dtype=torch.int32).cuda()
+    tree = speculative.Tree(_parents(b, t, 5).cuda())
+    kept = torch.full((b, t), -1, dtype=torch.int32)
+    kept[:, 0], kept[:, 1] = 0, t - 1
+    results = []
+    for pages in (b * per, count):
+        cache = paged.PagedCache(pages, page, kv, d, fmt=fmt)
+        table = (pages - 1 - torch.arange(b * per)).reshape(b, per)
+        slots = (table[:, :, None] * page + torch.arange(page)).flatten().cuda()
+        table = table.int().cuda()
+        cache.write(x[0], x[1], slots)
+        o, lse = speculative.tree_attention(q, cache, table, context, tree, return_lse=True)
+        cache.keep(table, context, kept.cuda(), torch.full((b,), 2, dtype=torch.int32, device="cuda"))
+        results.append((o, lse, *cache.read(slots)))
+        cache.check()
+    assert all(torch.equal(near, far) for near, far in zip(*results))

@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 // writes half an operand of each).
 //
 // 8 trees of 64 nodes over 1024 to 4096 cached tokens, 8 E4M3 key heads of 128
-// and 32 query heads (56 MB, 24 GFLOP): 50-69 us, 0.34-0.47 PFLOP/s.  The vector
+// and 32 query heads (56 MB, 24 GFLOP): 50-65 us, 0.36-0.47 PFLOP/s.  The vector
 // instructions and LDS bound it (softmax, conversion and operand reads: each
 // half of all cycles, the matrix instructions a third; 0.77 PFLOP/s from one
 // length to the next), with about 18 us before the first product and after the
