@@ -390,66 +390,72 @@ VH_DEV void see(const Args& a, int b, int ctx, int key0, const int (&live)[2], c
 
 // A step's softmax is in two forms.  S: products of key 16 t + 4 g + i and row
 // 16 nt + r; ks, vs: the keys' scales; m, l: a row's maximum and a lane's part
-// of its sum; T: the accumulators' unit, a power of two over the value scales
-// so far.
+// of its sum; top: over codes, the largest probability times value scale that
+// the row has seen.
+//
+// The operand of the second product is p * vs in the unit of its row, a power
+// of two over `top`.  Only keys that the row sees count: what another branch, a
+// node that pads or an old row behind the sequence holds does not move it.
 //
 // In the quick form, for a step that every row sees, nothing moves: the
 // probabilities are taken against the maximum as it is, and the step is given
-// up (true) where one passes 2^13, where a row has no maximum yet, or where a
-// value scale passes T.  It needs no maximum over lanes, and its loop holds no
-// branch that writes the accumulators (with one, the compiler keeps two copies
-// of them).  Float16 holds 2^13 as well as 1, so the maximum seldom moves.
+// up (true) where an operand passes 2^13 or where a row has no maximum yet.  It
+// needs no maximum over lanes, and its loop holds no branch that writes the
+// accumulators (with one, the compiler keeps two copies of them).  Float16 holds
+// 2^13 as well as 1, so the maximum seldom moves.
+constexpr float OPERAND_MOST = 0x1p13f;
+// Bounds on a probability and on a value scale in a row's unit, so that no sum
+// and no product of the quick form passes float32.
+constexpr float QUICK_MOST = 0x1p100f;
+
+VH_DEV float unit_of(float top) {  // the power of two over `top`, 2^-126 at least
+  return __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
+}
+VH_DEV float inverse_unit(float top) { return __uint_as_float(0x7f000000u - __float_as_uint(unit_of(top))); }
+
 template <int FMT, int NT>
 VH_DEV bool quick(const f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&vs)[2], const float (&fac)[NT],
-                  const float (&m)[NT], float T, f32x4 (&p)[2][NT]) {
+                  const float (&m)[NT], const float (&top)[NT], f32x4 (&p)[2][NT]) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
   bool far = false;
+  float high = 0.0f;
+  if constexpr (BYTE) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      high = fmaxf(fmaxf(high, vs[t][0]), vs[t][1]);
+      high = fmaxf(fmaxf(high, vs[t][2]), vs[t][3]);
+    }
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float top = 0.0f;
+    const float inv = BYTE ? inverse_unit(top[nt]) : 1.0f;
+    float most = 0.0f, operand = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[t][nt][i] = exp2_fast(fmaf(S[t][nt][i], BYTE ? ks[t][i] * fac[nt] : fac[nt], -m[nt]));
-      top = fmaxf(fmaxf(top, p[t][nt][0]), p[t][nt][1]);
-      top = fmaxf(fmaxf(top, p[t][nt][2]), p[t][nt][3]);
+      most = fmaxf(fmaxf(most, p[t][nt][0]), p[t][nt][1]);
+      most = fmaxf(fmaxf(most, p[t][nt][2]), p[t][nt][3]);
+      if constexpr (BYTE) {
+        const f32x4 w = vs[t] * inv;
+        operand = fmaxf(fmaxf(operand, p[t][nt][0] * w[0]), p[t][nt][1] * w[1]);
+        operand = fmaxf(fmaxf(operand, p[t][nt][2] * w[2]), p[t][nt][3] * w[3]);
+      }
     }
-    far |= top > 0x1p13f || m[nt] == -__builtin_inff();
-  }
-  if constexpr (BYTE) {
-    float top = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      top = fmaxf(fmaxf(top, vs[t][0]), vs[t][1]);
-      top = fmaxf(fmaxf(top, vs[t][2]), vs[t][3]);
-    }
-    far |= top > T;
+    far |= m[nt] == -__builtin_inff();
+    if constexpr (BYTE) far |= operand > OPERAND_MOST || most > QUICK_MOST || high * inv > QUICK_MOST;
+    else far |= most > OPERAND_MOST;
   }
   return far;
 }
 
-// The other form: any step, U tiles at once, with the maximum and the unit
+// The other form: any step, U tiles at once, with the maxima and the unit
 // moved to where they belong.  seen: the keys that the rows see.  S becomes the
 // probabilities.
 template <int FMT, int U, int CT, int NT>
 VH_DEV void careful(f32x4 (&S)[U][2][NT], const f32x4 (&ks)[U][2], const f32x4 (&vs)[U][2], const float (&fac)[NT],
-                    const uint32_t (&seen)[U][NT], float (&m)[NT], float (&l)[NT], float& T, f32x4 (&acc)[CT][NT]) {
+                    const uint32_t (&seen)[U][NT], float (&m)[NT], float (&l)[NT], float (&top)[NT], f32x4 (&acc)[CT][NT]) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
-  float down = 1.0f;
-  if constexpr (BYTE) {
-    float top = 0.0f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, vs[u][t][i]);
-    top = fminf(max_rows(top), 0x1p125f);  // the next power of two stays finite
-    const float over = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
-    const float to = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(top > T ? over : T)));
-    down = T * __uint_as_float(0x7f000000u - __float_as_uint(to));  // T / to, both powers of two
-    T = to;
-  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float v = -__builtin_inff();
@@ -467,32 +473,38 @@ VH_DEV void careful(f32x4 (&S)[U][2][NT], const f32x4 (&ks)[U][2], const f32x4 (
     const float alpha = m[nt] == -__builtin_inff() ? 0.0f : exp2_fast(m[nt] - to);
     m[nt] = to;
     l[nt] *= alpha;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c][nt] *= alpha * down;
     const float ref = to == -__builtin_inff() ? 0.0f : to;
+    float most = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[u][t][nt][i] = exp2_fast(S[u][t][nt][i] - ref);
+        for (int i = 0; i < 4; ++i) {
+          S[u][t][nt][i] = exp2_fast(S[u][t][nt][i] - ref);
+          // a scale that is not seen may be anything
+          if (BYTE) most = fmaxf(most, seen[u][nt] >> (4 * t + i) & 1 ? S[u][t][nt][i] * vs[u][t][i] : 0.0f);
+        }
+    float down = alpha;
+    if constexpr (BYTE) {
+      const float was = unit_of(top[nt]);
+      top[nt] = fmaxf(top[nt] * alpha, max_rows(most));
+      down = alpha * was * inverse_unit(top[nt]);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c][nt] *= down;
   }
 }
 
 // The probabilities as the B operand of the second product (k = 4 t + i), in
-// two parts where SPLIT, times the value scales in the unit T.
+// two parts where SPLIT, times the value scales in the rows' units.
 template <int FMT, bool SPLIT, bool MASKED, int NT>
-VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], float T, const uint32_t (&seen)[NT], float (&l)[NT],
-                     uint4 (&P)[NT], uint4 (&Plo)[NT]) {
+VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], const float (&top)[NT], const uint32_t (&seen)[NT],
+                     float (&l)[NT], uint4 (&P)[NT], uint4 (&Plo)[NT]) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
-  f32x4 vn[2];
-  if constexpr (BYTE) {
-    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(T));  // 1 / T
-#pragma unroll
-    for (int t = 0; t < 2; ++t) vn[t] = vs[t] * inv;
-  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    const float inv = BYTE ? inverse_unit(top[nt]) : 1.0f;
     uint32_t w[4], u[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -501,11 +513,12 @@ VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], float T, con
         float p0 = p[t][nt][i], p1 = p[t][nt][i + 1];
         l[nt] += p0 + p1;
         if constexpr (BYTE) {
-          p0 *= vn[t][i];
-          p1 *= vn[t][i + 1];
-          if constexpr (MASKED) {  // a scale there may be anything
-            p0 = seen[nt] >> (4 * t + i) & 1 ? p0 : 0.0f;
-            p1 = seen[nt] >> (4 * t + i + 1) & 1 ? p1 : 0.0f;
+          if constexpr (MASKED) {  // the scale last: a large one in the unit of small ones would not be finite
+            p0 = seen[nt] >> (4 * t + i) & 1 ? p0 * vs[t][i] * inv : 0.0f;
+            p1 = seen[nt] >> (4 * t + i + 1) & 1 ? p1 * vs[t][i + 1] * inv : 0.0f;
+          } else {
+            p0 *= vs[t][i] * inv;
+            p1 *= vs[t][i + 1] * inv;
           }
         }
         w[2 * t + i / 2] = pack2<FMT>(p0, p1);
@@ -643,15 +656,14 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
   load_queries(a, b, h, row0, Q, node, [&](int s) { return BYTE ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; });
 
   f32x4 acc[CT][NT];
-  float m[NT], l[NT];
+  float m[NT], l[NT], top[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt] = -__builtin_inff();
-    l[nt] = 0.0f;
+    l[nt] = top[nt] = 0.0f;
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  float T = 0x1p-126f;
   Finder find(a, b, h, begin, end);
 
   uint4 kr[2][KQ];
@@ -749,8 +761,8 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
         uint4 P[NT], Plo[NT];
         products(S[0]);
         see<NT>(a, b, ctx, key0, st.live, node, seen[0]);
-        careful<FMT>(S, k1, v1, fac, seen, m, l, T, acc);
-        operands<FMT, SPLIT, true>(S[0], vs, T, seen[0], l, P, Plo);
+        careful<FMT>(S, k1, v1, fac, seen, m, l, top, acc);
+        operands<FMT, SPLIT, true>(S[0], vs, top, seen[0], l, P, Plo);
         if constexpr (!BYTE) {
           uint32_t any = 0u;
 #pragma unroll
@@ -785,11 +797,11 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
-        if (__any(quick<FMT>(S, k1, vs, fac, m, T, p))) {
+        if (__any(quick<FMT>(S, k1, vs, fac, m, top, p))) {
           load_k(st);  // once more, seldom
           break;
         }
-        operands<FMT, SPLIT, false>(p, vs, T, all, l, P, Plo);
+        operands<FMT, SPLIT, false>(p, vs, top, all, l, P, Plo);
         add(P, Plo);
         __builtin_amdgcn_sched_barrier(0);
         load_v(next);
@@ -822,7 +834,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
       const float mw = s_m[w][16 * nt + r];
       L[nt] += s_l[w][16 * nt + r] * (mw == -__builtin_inff() ? 1.0f : exp2_fast(mw - M[nt]));
     }
-    const float f = (m[nt] == -__builtin_inff() ? 1.0f : exp2_fast(m[nt] - M[nt])) * (BYTE ? T : 1.0f);
+    const float f = (m[nt] == -__builtin_inff() ? 1.0f : exp2_fast(m[nt] - M[nt])) * (BYTE ? unit_of(top[nt]) : 1.0f);
     const bool none = pads(a, b, node[nt]);
     if (none) {
       M[nt] = -__builtin_inff();
@@ -934,15 +946,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   load_queries(a, b, h, row0, Q, node, [&](int s) { return 32 * s + 8 * g; });
 
   f32x4 acc[CT][NT];
-  float m[NT], l[NT];
+  float m[NT], l[NT], top[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt] = -__builtin_inff();
-    l[nt] = 0.0f;
+    l[nt] = top[nt] = 0.0f;
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  float T = 0x1p-126f;
   Finder find(a, b, h, begin, end);
 
   // a thread's part in the conversion
@@ -1144,9 +1155,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           scales(in, tile, ks[u], vs[u]);
           see<NT>(a, b, ctx, key0 + STEP * tile, live[u], node, seen[u]);
         }
-        careful<FMT>(S, ks, vs, fac, seen, m, l, T, acc);
+        careful<FMT>(S, ks, vs, fac, seen, m, l, top, acc);
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) operands<FMT, SPLIT, true>(S[u], vs[u], T, seen[u], l, P[u], Plo[u]);
+        for (int u = 0; u < SUB; ++u) operands<FMT, SPLIT, true>(S[u], vs[u], top, seen[u], l, P[u], Plo[u]);
         if constexpr (!BYTE) {
           if (!is_plain) {
 #pragma unroll
@@ -1180,18 +1191,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         // The quick form of the softmax, written out so that nothing waits:
         // operands are read AHEAD of their products, and the last step's second
         // products are issued between this step's softmax, two scores at a time.
-        // A step is given up where a lane's sum passes 2^13: its terms are no more.
+        // A step is given up as in the other kernel; a lane's sum stands for its terms.
         constexpr int AHEAD = 4, TN = 2 * SUB;                // TN: 16-key tiles
         constexpr int KF = KS * TN, VF = CT * SUB, HALVES = TN * NT * 2;
         const Stage& in = s_stage[half];
         const Stage& old = s_stage[half ^ 1];
         f32x4 S[TN][NT];
         uint32_t w[TN][NT][2], u[TN][NT][2];
-        f32x4 ks[2], vs[2];  // of this 16-key tile and the next
-        float sum[NT], high = 0.0f;
+        f32x4 ks[2], vs[2], vn;  // of this 16-key tile and the next; in the unit of this tile's row
+        float sum[NT], inv[NT], high = 0.0f, operand = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           sum[nt] = 0.0f;
+          inv[nt] = BYTE ? inverse_unit(top[nt]) : 1.0f;
 #pragma unroll
           for (int t = 0; t < TN; ++t) S[t][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -1206,21 +1218,21 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
             vs[t % 2] = in.scale[kw * SUB + t / 2][1][4 * (t % 2) + g];
           }
         };
-        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(T));  // 1 / T
         auto scores2 = [&](int n) __attribute__((always_inline)) {
           const int t = n / (2 * NT), nt = n / 2 % NT, i = n % 2 * 2;
           if (BYTE && n % (2 * NT) == 0) {
             high = fmaxf(fmaxf(high, vs[t % 2][0]), vs[t % 2][1]);
             high = fmaxf(fmaxf(high, vs[t % 2][2]), vs[t % 2][3]);
-            vs[t % 2] *= inv;
             if (t + 1 < TN) scale_at(t + 1);
           }
+          if (BYTE && i == 0) vn = vs[t % 2] * inv[nt];
           const float f0 = BYTE ? ks[t % 2][i] * fac[nt] : fac[nt], f1 = BYTE ? ks[t % 2][i + 1] * fac[nt] : fac[nt];
           float p0 = exp2_fast(fmaf(S[t][nt][i], f0, -m[nt])), p1 = exp2_fast(fmaf(S[t][nt][i + 1], f1, -m[nt]));
           sum[nt] += p0 + p1;
           if constexpr (BYTE) {
-            p0 *= vs[t % 2][i];
-            p1 *= vs[t % 2][i + 1];
+            p0 *= vn[i];
+            p1 *= vn[i + 1];
+            operand = fmaxf(fmaxf(operand, p0), p1);
           }
           w[t][nt][n % 2] = pack2<FMT>(p0, p1);
           if constexpr (SPLIT) {
@@ -1256,9 +1268,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           for (int x = n * HALVES / VF; x < (n + 1) * HALVES / VF; ++x) scores2(x);
           __builtin_amdgcn_sched_barrier(0);
         }
-        bool far = BYTE && high > T;
+        bool far = BYTE && operand > OPERAND_MOST;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) far |= sum[nt] > 0x1p13f || m[nt] == -__builtin_inff();
+        for (int nt = 0; nt < NT; ++nt) {
+          far |= sum[nt] > (BYTE ? QUICK_MOST : OPERAND_MOST) || m[nt] == -__builtin_inff();
+          if constexpr (BYTE) far |= high * inv[nt] > QUICK_MOST;
+        }
         pending = false;
         if (__any(far)) {
           fed = true;
@@ -1302,7 +1317,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s_o[(c * NT + nt) * 64 + lane] = acc[c][nt] * (BYTE ? T : 1.0f);
+        for (int nt = 0; nt < NT; ++nt) s_o[(c * NT + nt) * 64 + lane] = acc[c][nt] * (BYTE ? unit_of(top[nt]) : 1.0f);
     }
     __syncthreads();
     if (kw == 1) return;
@@ -1313,7 +1328,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       const float f1 = m1 == -__builtin_inff() ? 1.0f : exp2_fast(m1 - to);
       M[nt] = to;
       L[nt] = L[nt] * f0 + s_l[rw][16 * nt + r] * f1;
-      const float f = f0 * (BYTE ? T : 1.0f);
+      const float f = f0 * (BYTE ? unit_of(top[nt]) : 1.0f);
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[c][nt] = acc[c][nt] * f + s_o[(c * NT + nt) * 64 + lane] * f1;
     }
@@ -1321,7 +1336,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) acc[c][nt] *= T;
+      for (int c = 0; c < CT; ++c) acc[c][nt] *= unit_of(top[nt]);
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
