@@ -91,7 +91,7 @@ class Case:
             self.cache.v_scale.double().transpose(1, 2).flatten(0, 1)[self.slots] * MOST[self.fmt])
         return out[0], out[1], most
 
-    def exact(self, gone=None):
+    def exact(self, gone=None, floor=2.0**-34):
         """``(o, lse, tolerance of o, tolerance of lse)``; ``gone [b,
         positions]``: positions that are not there.
 
@@ -106,9 +106,9 @@ class Case:
           waves and splits, in units of 2^-24;
         * float16 parts: half of its least value, 2^-25, where the largest
           p * scale of the row lies at 2^9 or more (8-bit caches), or the
-          largest p (float16): keys times 2^-34 of the largest p * amax, or
-          of the largest value seen;
-        * half a step of the result.
+          largest p (float16): keys times ``floor``, 2^-34, of the largest
+          p * amax, or of the largest value seen;
+        * half a step of the result, which has a least size.
         """
         b, t, heads, d = self.q.shape
         group = heads // self.kv
@@ -117,6 +117,7 @@ class Case:
         lse = torch.full((b, t, heads), -math.inf, dtype=torch.float64, device="cuda")
         tol, tlse = torch.zeros_like(o), torch.zeros_like(lse)
         part = 2.0**-16 if self.cache.dtype == torch.bfloat16 and self.fmt is None else 2.0**-22
+        step = torch.finfo(self.dtype).smallest_normal * torch.finfo(self.dtype).eps
         for i in range(b):
             n = int(self.context[i]) + t
             see = torch.ones(t, n, dtype=torch.bool, device="cuda")
@@ -143,8 +144,8 @@ class Case:
                 score = (d + 6) * 2.0**-24 * dot
                 sums = (32 + n / 32 + 64) * 2.0**-24
                 out = r @ vv
-                e = (HALF[self.dtype] * out.abs() * (1 + 2.0**-6) + (2 * score + 2.0**-21 + 2.0**-23 + part + 2 * sums) * mag
-                     + n * 2.0**-34 * least + 1e-300)
+                e = ((HALF[self.dtype] * out.abs() * (1 + 2.0**-6)).clamp(min=step / 2) + (2 * score + 2.0**-21 + 2.0**-23 + part + 2 * sums) * mag
+                     + n * floor * least)
                 at = slice(h * group, (h + 1) * group)
                 o[i, :, at] = (out * some[:, None]).reshape(t, group, d)
                 tol[i, :, at] = e.reshape(t, group, d)
@@ -153,8 +154,8 @@ class Case:
                 tlse[i, :, at] = (score[:, 0] + 2.0**-21 + sums + 4 * 2.0**-24 * full.abs().clamp(max=1e30)).reshape(t, group)
         return o, lse, tol, tlse
 
-    def agrees(self, got, gone=None):
-        o, lse, tol, tlse = self.exact(gone)
+    def agrees(self, got, gone=None, floor=2.0**-34):
+        o, lse, tol, tlse = self.exact(gone, floor)
         err = (got[0].double() - o).abs()
         assert bool((err <= tol).all()), f"output: {int((~(err <= tol)).sum())} of {err.numel()} beyond, worst {float((err / tol).max()):.2f}"
         empty = torch.isinf(lse)

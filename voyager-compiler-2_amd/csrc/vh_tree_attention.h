@@ -449,25 +449,23 @@ VH_DEV bool quick(const f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&v
   return far;
 }
 
-// The other form: any step, U tiles at once, with the maxima and the unit
+// The other form: any step, with the maxima and the unit
 // moved to where they belong.  seen: the keys that the rows see.  S becomes the
 // probabilities.
-template <int FMT, int U, int CT, int NT>
-VH_DEV void careful(f32x4 (&S)[U][2][NT], const f32x4 (&ks)[U][2], const f32x4 (&vs)[U][2], const float (&fac)[NT],
-                    const uint32_t (&seen)[U][NT], float (&m)[NT], float (&l)[NT], float (&top)[NT], f32x4 (&acc)[CT][NT]) {
+template <int FMT, int CT, int NT>
+VH_DEV void careful(f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&vs)[2], const float (&fac)[NT],
+                    const uint32_t (&seen)[NT], float (&m)[NT], float (&l)[NT], float (&top)[NT], f32x4 (&acc)[CT][NT]) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float v = -__builtin_inff();
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = S[u][t][nt][i] * (BYTE ? ks[u][t][i] * fac[nt] : fac[nt]);
-          S[u][t][nt][i] = seen[u][nt] >> (4 * t + i) & 1 ? x : -__builtin_inff();
-          v = fmaxf(v, S[u][t][nt][i]);
+          const float x = S[t][nt][i] * (BYTE ? ks[t][i] * fac[nt] : fac[nt]);
+          S[t][nt][i] = seen[nt] >> (4 * t + i) & 1 ? x : -__builtin_inff();
+          v = fmaxf(v, S[t][nt][i]);
         }
     const float to = fmaxf(m[nt], max_rows(v));
     const float alpha = m[nt] == -__builtin_inff() ? 0.0f : exp2_fast(m[nt] - to);
@@ -476,14 +474,12 @@ VH_DEV void careful(f32x4 (&S)[U][2][NT], const f32x4 (&ks)[U][2], const f32x4 (
     const float ref = to == -__builtin_inff() ? 0.0f : to;
     float most = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          S[u][t][nt][i] = exp2_fast(S[u][t][nt][i] - ref);
+          S[t][nt][i] = exp2_fast(S[t][nt][i] - ref);
           // a scale that is not seen may be anything
-          if (BYTE) most = fmaxf(most, seen[u][nt] >> (4 * t + i) & 1 ? S[u][t][nt][i] * vs[u][t][i] : 0.0f);
+          if (BYTE) most = fmaxf(most, seen[nt] >> (4 * t + i) & 1 ? S[t][nt][i] * vs[t][i] : 0.0f);
         }
     float down = alpha;
     if constexpr (BYTE) {
@@ -496,9 +492,10 @@ VH_DEV void careful(f32x4 (&S)[U][2][NT], const f32x4 (&ks)[U][2], const f32x4 (
   }
 }
 
-// The probabilities as the B operand of the second product (k = 4 t + i), in
-// two parts where SPLIT, times the value scales in the rows' units.
-template <int FMT, bool SPLIT, bool MASKED, int NT>
+// The probabilities as the B operand of the second product (k = 4 t + i), times
+// the value scales in the rows' units: in two 16-bit parts, as one would round
+// them by 2^-12 of float16 or 2^-9 of bfloat16, which a result in 16 bits shows.
+template <int FMT, bool MASKED, int NT>
 VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], const float (&top)[NT], const uint32_t (&seen)[NT],
                      float (&l)[NT], uint4 (&P)[NT], uint4 (&Plo)[NT]) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
@@ -522,13 +519,11 @@ VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], const float 
           }
         }
         w[2 * t + i / 2] = pack2<FMT>(p0, p1);
-        if constexpr (SPLIT) {
-          const f32x2 hi = unpack2<FMT>(w[2 * t + i / 2]);
-          u[2 * t + i / 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
-        }
+        const f32x2 hi = unpack2<FMT>(w[2 * t + i / 2]);
+        u[2 * t + i / 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
       }
     P[nt] = make_uint4(w[0], w[1], w[2], w[3]);
-    if constexpr (SPLIT) Plo[nt] = make_uint4(u[0], u[1], u[2], u[3]);
+    Plo[nt] = make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
 
@@ -624,7 +619,7 @@ constexpr int waves_of(int d, int fmt, int nt) {
 // cached ones, 8 int8 key heads of 128 and 32 query heads (353 MB): 79-84 us,
 // 4.2-4.5 TB/s, as fast as this card's memory is read by a plain sum.  One token
 // over 4096 (8.7 MB): 9.5 us, the latency of table, keys, values and joining.
-template <int D, int FMT, int NT, bool SPLIT>
+template <int D, int FMT, int NT>
 __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args a) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
   constexpr int ESZ = BYTE ? 1 : 2;
@@ -739,7 +734,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             acc[c][nt] = mfma<FMT>(A, P[nt], acc[c][nt]);
-            if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
+            acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
           }
         }
   };
@@ -756,13 +751,13 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
     do {
       const Step next = find(after());
       {
-        f32x4 S[1][2][NT], k1[1][2] = {{ks[0], ks[1]}}, v1[1][2] = {{vs[0], vs[1]}};
-        uint32_t seen[1][NT];
+        f32x4 S[2][NT];
+        uint32_t seen[NT];
         uint4 P[NT], Plo[NT];
-        products(S[0]);
-        see<NT>(a, b, ctx, key0, st.live, node, seen[0]);
-        careful<FMT>(S, k1, v1, fac, seen, m, l, top, acc);
-        operands<FMT, SPLIT, true>(S[0], vs, top, seen[0], l, P, Plo);
+        products(S);
+        see<NT>(a, b, ctx, key0, st.live, node, seen);
+        careful<FMT>(S, ks, vs, fac, seen, m, l, top, acc);
+        operands<FMT, true>(S, vs, top, seen, l, P, Plo);
         if constexpr (!BYTE) {
           uint32_t any = 0u;
 #pragma unroll
@@ -778,7 +773,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
                   vr[t][i][w][d] &= ~bits;
                 }
           if (__any(any != 0u))
-            add_nonfinite<FMT>(a, st, S[0], seen[0], acc, [&](int c, int i) { return (c / CPL) * 16 * CPL + (4 * g + i) * CPL + c % CPL; });
+            add_nonfinite<FMT>(a, st, S, seen, acc, [&](int c, int i) { return (c / CPL) * 16 * CPL + (4 * g + i) * CPL + c % CPL; });
         }
         add(P, Plo);
       }
@@ -801,7 +796,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
           load_k(st);  // once more, seldom
           break;
         }
-        operands<FMT, SPLIT, false>(p, vs, top, all, l, P, Plo);
+        operands<FMT, false>(p, vs, top, all, l, P, Plo);
         add(P, Plo);
         __builtin_amdgcn_sched_barrier(0);
         load_v(next);
@@ -880,7 +875,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 }
 
 // Many rows.  RW waves of 16 NT rows each share the keys of a step, and 4 / RW
-// groups of them take their own; a wave takes SUB tiles of 32 keys of a step.
+// groups of them take their own tile of 32 keys of it.
 //
 // A step's second product is done in the next step, so that its matrix
 // instructions run while that step's softmax does (they are issued in turn),
@@ -903,16 +898,12 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 template <int D>
 constexpr int wide_nt() { return D <= 128 ? 2 : 1; }
 
-template <int D, int FMT, int RW, bool SPLIT>
+template <int D, int FMT, int RW>
 __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
   constexpr int ESZ = BYTE ? 1 : 2;
   constexpr int NT = wide_nt<D>();
-  constexpr int KW = WAVES / RW;
-  // two where the registers hold two tiles' probabilities: a step is then
-  // longer than the latency of the next ones' keys
-  constexpr int SUB = RW == 4 && D <= 128 && !SPLIT ? 2 : 1;
-  constexpr int TILES = KW * SUB, KEYS = STEP * TILES;
+  constexpr int TILES = WAVES / RW, KEYS = STEP * TILES;
   constexpr int KS = D / 32, CT = D / 16;
   constexpr int KB = D / 8 * ESZ / 4;  // dwords of a thread's share of 32 keys: D / 8 channels of one
   constexpr int QUADS = D / 4, VP = QUADS > 32 ? QUADS / 32 : 1;  // passes of a thread over 32 keys' values
@@ -921,7 +912,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
     uint4 k[TILES][SLOTS], v[TILES][SLOTS];
     f32x4 scale[BYTE ? TILES : 1][2][8];  // of keys, of values
   };
-  static_assert(sizeof(Stage) * 2 >= (size_t)(KW - 1) * RW * CT * NT * 64 * 16, "results reuse the stages");
+  static_assert(sizeof(Stage) * 2 >= (size_t)(TILES - 1) * RW * CT * NT * 64 * 16, "results reuse the stages");
   __shared__ Stage s_stage[2];
   __shared__ float s_m[RW][16 * NT], s_l[RW][16 * NT];
 
@@ -932,7 +923,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   const int b = span.b, h = blk.h;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int rw = wave % RW, kw = KW > 1 ? wave / RW : 0;
+  const int rw = wave % RW, tile = TILES > 1 ? wave / RW : 0;
   const int row0 = blk.row0 + rw * (16 * NT);
   const int ctx = __builtin_amdgcn_readfirstlane(a.context[b]);
   const int total = visible(a, ctx, blk.row0);
@@ -1064,8 +1055,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       }
   };
 
-  uint4 P[SUB][NT], Plo[SUB][NT];  // the last step's probabilities
-  auto products = [&](const Stage& in, int tile, f32x4 (&S)[2][NT]) __attribute__((always_inline)) {
+  uint4 P[NT], Plo[NT];  // the last step's probabilities
+  auto products = [&](const Stage& in, f32x4 (&S)[2][NT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -1078,7 +1069,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       }
     }
   };
-  auto scales = [&](const Stage& in, int tile, f32x4 (&ks)[2], f32x4 (&vs)[2]) __attribute__((always_inline)) {
+  auto scales = [&](const Stage& in, f32x4 (&ks)[2], f32x4 (&vs)[2]) __attribute__((always_inline)) {
     if constexpr (BYTE) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -1089,16 +1080,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   };
   auto add = [&](const Stage& in) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < SUB; ++u)
+    for (int c = 0; c < CT; ++c) {
+      const uint4 A = in.v[tile][c * 64 + lane];
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const uint4 A = in.v[kw * SUB + u][c * 64 + lane];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[c][nt] = mfma<FMT>(A, P[u][nt], acc[c][nt]);
-          if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(A, Plo[u][nt], acc[c][nt]);
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        acc[c][nt] = mfma<FMT>(A, P[nt], acc[c][nt]);
+        acc[c][nt] = mfma<FMT>(A, Plo[nt], acc[c][nt]);
       }
+    }
   };
 
   if (begin < end) {
@@ -1143,43 +1132,31 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       if (pending) add(s_stage[half ^ 1]);
       {
         const Stage& in = s_stage[half];
-        f32x4 S[SUB][2][NT], ks[SUB][2], vs[SUB][2];
-        uint32_t seen[SUB][NT];
-        int live[SUB][2];
+        f32x4 S[2][NT], ks[2], vs[2];
+        uint32_t seen[NT];
+        Step st;
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-          const int tile = kw * SUB + u;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) live[u][t] = either(tile != 0, now.s[TILES - 1].live[t], now.s[0].live[t]);
-          products(in, tile, S[u]);
-          scales(in, tile, ks[u], vs[u]);
-          see<NT>(a, b, ctx, key0 + STEP * tile, live[u], node, seen[u]);
+        for (int t = 0; t < 2; ++t) {
+          st.row[t] = either(tile != 0, now.s[TILES - 1].row[t], now.s[0].row[t]);
+          st.live[t] = either(tile != 0, now.s[TILES - 1].live[t], now.s[0].live[t]);
         }
+        products(in, S);
+        scales(in, ks, vs);
+        see<NT>(a, b, ctx, key0 + STEP * tile, st.live, node, seen);
         careful<FMT>(S, ks, vs, fac, seen, m, l, top, acc);
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) operands<FMT, SPLIT, true>(S[u], vs[u], top, seen[u], l, P[u], Plo[u]);
+        operands<FMT, true>(S, vs, top, seen, l, P, Plo);
         if constexpr (!BYTE) {
           if (!is_plain) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-              const int tile = kw * SUB + u;
-              Step st;
-#pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                st.row[t] = either(tile != 0, now.s[TILES - 1].row[t], now.s[0].row[t]);
-                st.live[t] = live[u][t];
-              }
-              uint32_t any = 0u;
-              const uint16_t* v =
-                  (const uint16_t*)a.c.v + (either((lane & 32) != 0, st.row[1], st.row[0]) + r) * D + (lane >> 4 & 1) * (D / 2);
+            uint32_t any = 0u;
+            const uint16_t* v =
+                (const uint16_t*)a.c.v + (either((lane & 32) != 0, st.row[1], st.row[0]) + r) * D + (lane >> 4 & 1) * (D / 2);
 #pragma unroll 4
-              for (int c = 0; c < D / 2; c += 8) {
-                const uint4 x = *(const uint4*)(v + c);
-                any |= nonfinite<FMT>(x.x) | nonfinite<FMT>(x.y) | nonfinite<FMT>(x.z) | nonfinite<FMT>(x.w);
-              }
-              if (__any(any != 0u))
-                add_nonfinite<FMT>(a, st, S[u], seen[u], acc, [&](int c, int i) { return 64 * (c / 4) + 4 * (4 * g + i) + c % 4; });
+            for (int c = 0; c < D / 2; c += 8) {
+              const uint4 x = *(const uint4*)(v + c);
+              any |= nonfinite<FMT>(x.x) | nonfinite<FMT>(x.y) | nonfinite<FMT>(x.z) | nonfinite<FMT>(x.w);
             }
+            if (__any(any != 0u))
+              add_nonfinite<FMT>(a, st, S, seen, acc, [&](int c, int i) { return 64 * (c / 4) + 4 * (4 * g + i) + c % 4; });
           }
         }
       }
@@ -1192,13 +1169,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         // operands are read AHEAD of their products, and the last step's second
         // products are issued between this step's softmax, two scores at a time.
         // A step is given up as in the other kernel; a lane's sum stands for its terms.
-        constexpr int AHEAD = 4, TN = 2 * SUB;                // TN: 16-key tiles
-        constexpr int KF = KS * TN, VF = CT * SUB, HALVES = TN * NT * 2;
+        constexpr int AHEAD = 4, TN = 2;  // TN: 16-key tiles
+        constexpr int KF = KS * TN, HALVES = TN * NT * 2;
         const Stage& in = s_stage[half];
         const Stage& old = s_stage[half ^ 1];
         f32x4 S[TN][NT];
         uint32_t w[TN][NT][2], u[TN][NT][2];
-        f32x4 ks[2], vs[2], vn;  // of this 16-key tile and the next; in the unit of this tile's row
+        f32x4 ks[2], vs[2], vn;  // vn: in the unit of a row
         float sum[NT], inv[NT], high = 0.0f, operand = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -1209,24 +1186,24 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
         }
         auto key_at = [&](int n) __attribute__((always_inline)) {  // along D first: tiles' sums do not wait for each other
           const int t = n % TN, s = n / TN;
-          return in.k[kw * SUB + t / 2][(t % 2 * KS + s) * 64 + lane];
+          return in.k[tile][(t * KS + s) * 64 + lane];
         };
-        auto value_at = [&](int n) __attribute__((always_inline)) { return old.v[kw * SUB + n / CT][n % CT * 64 + lane]; };
+        auto value_at = [&](int n) __attribute__((always_inline)) { return old.v[tile][n * 64 + lane]; };
         auto scale_at = [&](int t) __attribute__((always_inline)) {
           if constexpr (BYTE) {
-            ks[t % 2] = in.scale[kw * SUB + t / 2][0][4 * (t % 2) + g];
-            vs[t % 2] = in.scale[kw * SUB + t / 2][1][4 * (t % 2) + g];
+            ks[t] = in.scale[tile][0][4 * t + g];
+            vs[t] = in.scale[tile][1][4 * t + g];
           }
         };
         auto scores2 = [&](int n) __attribute__((always_inline)) {
           const int t = n / (2 * NT), nt = n / 2 % NT, i = n % 2 * 2;
           if (BYTE && n % (2 * NT) == 0) {
-            high = fmaxf(fmaxf(high, vs[t % 2][0]), vs[t % 2][1]);
-            high = fmaxf(fmaxf(high, vs[t % 2][2]), vs[t % 2][3]);
+            high = fmaxf(fmaxf(high, vs[t][0]), vs[t][1]);
+            high = fmaxf(fmaxf(high, vs[t][2]), vs[t][3]);
             if (t + 1 < TN) scale_at(t + 1);
           }
-          if (BYTE && i == 0) vn = vs[t % 2] * inv[nt];
-          const float f0 = BYTE ? ks[t % 2][i] * fac[nt] : fac[nt], f1 = BYTE ? ks[t % 2][i + 1] * fac[nt] : fac[nt];
+          if (BYTE && i == 0) vn = vs[t] * inv[nt];
+          const float f0 = BYTE ? ks[t][i] * fac[nt] : fac[nt], f1 = BYTE ? ks[t][i + 1] * fac[nt] : fac[nt];
           float p0 = exp2_fast(fmaf(S[t][nt][i], f0, -m[nt])), p1 = exp2_fast(fmaf(S[t][nt][i + 1], f1, -m[nt]));
           sum[nt] += p0 + p1;
           if constexpr (BYTE) {
@@ -1235,13 +1212,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
             operand = fmaxf(fmaxf(operand, p0), p1);
           }
           w[t][nt][n % 2] = pack2<FMT>(p0, p1);
-          if constexpr (SPLIT) {
-            const f32x2 hi = unpack2<FMT>(w[t][nt][n % 2]);
-            u[t][nt][n % 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
-            asm volatile("" : "+v"(u[t][nt][n % 2]));
-          }
+          const f32x2 hi = unpack2<FMT>(w[t][nt][n % 2]);
+          u[t][nt][n % 2] = pack2<FMT>(p0 - hi[0], p1 - hi[1]);
           // here, between the products: the compiler would leave them for after the loop's exit
-          asm volatile("" : "+v"(w[t][nt][n % 2]), "+v"(sum[nt]));
+          asm volatile("" : "+v"(u[t][nt][n % 2]), "+v"(w[t][nt][n % 2]), "+v"(sum[nt]));
         };
         uint4 f[AHEAD];
 #pragma unroll
@@ -1256,16 +1230,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int n = 0; n < VF; ++n) {
-          const int c = n % CT;
+        for (int c = 0; c < CT; ++c) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            acc[c][nt] = mfma<FMT>(f[(KF + n) % AHEAD], P[n / CT][nt], acc[c][nt]);
-            if constexpr (SPLIT) acc[c][nt] = mfma<FMT>(f[(KF + n) % AHEAD], Plo[n / CT][nt], acc[c][nt]);
+            acc[c][nt] = mfma<FMT>(f[(KF + c) % AHEAD], P[nt], acc[c][nt]);
+            acc[c][nt] = mfma<FMT>(f[(KF + c) % AHEAD], Plo[nt], acc[c][nt]);
           }
-          if (n + AHEAD < VF) f[(KF + n) % AHEAD] = value_at(n + AHEAD);
+          if (c + AHEAD < CT) f[(KF + c) % AHEAD] = value_at(c + AHEAD);
 #pragma unroll
-          for (int x = n * HALVES / VF; x < (n + 1) * HALVES / VF; ++x) scores2(x);
+          for (int x = c * HALVES / CT; x < (c + 1) * HALVES / CT; ++x) scores2(x);
           __builtin_amdgcn_sched_barrier(0);
         }
         bool far = BYTE && operand > OPERAND_MOST;
@@ -1283,18 +1256,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           l[nt] += sum[nt];
-#pragma unroll
-          for (int v = 0; v < SUB; ++v) {
-            P[v][nt] = make_uint4(w[2 * v][nt][0], w[2 * v][nt][1], w[2 * v + 1][nt][0], w[2 * v + 1][nt][1]);
-            if constexpr (SPLIT)
-              Plo[v][nt] = make_uint4(u[2 * v][nt][0], u[2 * v][nt][1], u[2 * v + 1][nt][0], u[2 * v + 1][nt][1]);
-          }
+          P[nt] = make_uint4(w[0][nt][0], w[0][nt][1], w[1][nt][0], w[1][nt][1]);
+          Plo[nt] = make_uint4(u[0][nt][0], u[0][nt][1], u[1][nt][0], u[1][nt][1]);
         }
         advance();
       }
     } while (key0 < end);
     add(s_stage[half ^ 1]);
-    if constexpr (KW > 1) __syncthreads();  // the stages are free
+    if constexpr (TILES > 1) __syncthreads();  // the stages are free
   }
   if (find.bad && lane == 0) atomicOr(a.c.flag, VH_CACHE_ERR_PAGE);
 
@@ -1304,8 +1273,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
     L[nt] = sum_rows(l[nt]);
     M[nt] = m[nt];
   }
-  if constexpr (KW > 1) {  // the second group of keys onto the first
-    if (kw == 1 && g == 0) {
+  if constexpr (TILES > 1) {  // the second group of keys onto the first
+    if (tile == 1 && g == 0) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         s_m[rw][16 * nt + r] = M[nt];
@@ -1313,14 +1282,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       }
     }
     f32x4* s_o = (f32x4*)s_stage + rw * (CT * NT * 64);
-    if (kw == 1) {
+    if (tile == 1) {
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s_o[(c * NT + nt) * 64 + lane] = acc[c][nt] * (BYTE ? unit_of(top[nt]) : 1.0f);
     }
     __syncthreads();
-    if (kw == 1) return;
+    if (tile == 1) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float m1 = s_m[rw][16 * nt + r], to = fmaxf(M[nt], m1);
@@ -1365,21 +1334,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 template <int D>
 int launch(const Args& a, bool wide, int n, hipStream_t s);
 
-// float16 results are four times finer than float16 probabilities allow once
-// (an error of its own size would join the result's rounding), and bfloat16
-// values need bfloat16 probabilities: both take them in two parts.
 #define VH_TREE_FORMATS(KERNEL, N)                                                                    \
   switch (a.c.fmt) {                                                                                  \
-    case CACHE_E4M3:                                                                                  \
-      if (a.q_bf16) hipLaunchKernelGGL((KERNEL<D, CACHE_E4M3, N, false>), grid, block, 0, s, a);      \
-      else hipLaunchKernelGGL((KERNEL<D, CACHE_E4M3, N, true>), grid, block, 0, s, a);                \
-      break;                                                                                          \
-    case CACHE_INT8:                                                                                  \
-      if (a.q_bf16) hipLaunchKernelGGL((KERNEL<D, CACHE_INT8, N, false>), grid, block, 0, s, a);      \
-      else hipLaunchKernelGGL((KERNEL<D, CACHE_INT8, N, true>), grid, block, 0, s, a);                \
-      break;                                                                                          \
-    case CACHE_F16: hipLaunchKernelGGL((KERNEL<D, CACHE_F16, N, true>), grid, block, 0, s, a); break; \
-    default: hipLaunchKernelGGL((KERNEL<D, CACHE_BF16, N, true>), grid, block, 0, s, a); break;       \
+    case CACHE_E4M3: hipLaunchKernelGGL((KERNEL<D, CACHE_E4M3, N>), grid, block, 0, s, a); break;     \
+    case CACHE_INT8: hipLaunchKernelGGL((KERNEL<D, CACHE_INT8, N>), grid, block, 0, s, a); break;     \
+    case CACHE_F16: hipLaunchKernelGGL((KERNEL<D, CACHE_F16, N>), grid, block, 0, s, a); break;       \
+    default: hipLaunchKernelGGL((KERNEL<D, CACHE_BF16, N>), grid, block, 0, s, a); break;             \
   }
 
 template <int D>
