@@ -389,27 +389,36 @@ VH_DEV void see(const Args& a, int b, int ctx, int key0, const int (&live)[2], c
 }
 
 // A step's softmax is in two forms.  S: products of key 16 t + 4 g + i and row
-// 16 nt + r; ks, vs: the keys' scales; m, l: a row's maximum and a lane's part
-// of its sum; top: over codes, the largest probability times value scale that
+// 16 nt + r; ks, vs: the keys' scales; m, l: a row's reference (its maximum, or
+// under it) and a lane's part of its sum; top: over codes, the largest probability times value scale that
 // the row has seen.
 //
 // The operand of the second product is p * vs in the unit of its row, a power
-// of two over `top`.  Only keys that the row sees count: what another branch, a
+// of two by `top`.  Only keys that the row sees count: what another branch, a
 // node that pads or an old row behind the sequence holds does not move it.
 //
+// The sum takes a probability in float32, the operand rounds it to float16,
+// whose least is 2^-24: the largest operand is placed under 2^PLACE, so that one
+// of 2^-34 of it still counts (at 1, 32768 keys of 2^-26 beside one were in the
+// sum and not in the product, half of a result).  Over codes the unit does it;
+// float16 values have the reference of the softmax, m, that far under the maximum.
+//
 // In the quick form, for a step that every row sees, nothing moves: the
-// probabilities are taken against the maximum as it is, and the step is given
-// up (true) where an operand passes 2^13 or where a row has no maximum yet.  It
+// probabilities are taken against the reference as it is, and the step is given
+// up (true) where an operand passes 2^15 or where a row has no reference yet.  It
 // needs no maximum over lanes, and its loop holds no branch that writes the
-// accumulators (with one, the compiler keeps two copies of them).  Float16 holds
-// 2^13 as well as 1, so the maximum seldom moves.
-constexpr float OPERAND_MOST = 0x1p13f;
+// accumulators (with one, the compiler keeps two copies of them).  Five binades
+// are left for it: after the first steps the maximum seldom rises by that.
+constexpr int PLACE = 10;
+constexpr float OPERAND_MOST = 0x1p15f;
 // Bounds on a probability and on a value scale in a row's unit, so that no sum
 // and no product of the quick form passes float32.
 constexpr float QUICK_MOST = 0x1p100f;
 
-VH_DEV float unit_of(float top) {  // the power of two over `top`, 2^-126 at least
-  return __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
+VH_DEV float unit_of(float top) {  // top / 2^PLACE, up to the next power of two; 2^-126 at least
+  constexpr uint32_t LEAST = (uint32_t)PLACE << 23;
+  const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+  return __uint_as_float((e < LEAST ? LEAST : e) - LEAST + 0x00800000u);
 }
 VH_DEV float inverse_unit(float top) { return __uint_as_float(0x7f000000u - __float_as_uint(unit_of(top))); }
 
@@ -467,7 +476,7 @@ VH_DEV void careful(f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&vs)[2
           S[t][nt][i] = seen[nt] >> (4 * t + i) & 1 ? x : -__builtin_inff();
           v = fmaxf(v, S[t][nt][i]);
         }
-    const float to = fmaxf(m[nt], max_rows(v));
+    const float to = fmaxf(m[nt], max_rows(v) - (FMT == CACHE_F16 ? PLACE : 0));
     const float alpha = m[nt] == -__builtin_inff() ? 0.0f : exp2_fast(m[nt] - to);
     m[nt] = to;
     l[nt] *= alpha;
