@@ -111,6 +111,33 @@ def test_prompts_without_a_tree(fmt, b, t, heads, kv, d, context):
     c.cache.check()
 
 
+@pytest.mark.parametrize("t,heads,d", ROWS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinite_values_in_mid_sequence(dtype, t, heads, d):
+    """A 16-bit value that is infinite or NaN makes its channel so for the rows
+    that see it, and no other."""
+    c = Case(1, t, heads, 2, d, None, dtype, 16, [900], seed=t + d, spread=0.0)
+    for workgroups in (1, 4):
+        clean, lse = c.run(workgroups)
+        was = c.v.clone()
+        c.v[0, 411, 0, 3], c.v[0, 98, 0, 9], c.v[0, 700, 0, 17] = torch.inf, -torch.inf, torch.nan
+        c.v[0, 50, 0, 20], c.v[0, 51, 0, 20] = torch.inf, -torch.inf
+        c.fill()
+        o, bad = c.run(workgroups)
+        c.v = was
+        c.fill()
+        group = heads // 2
+        head = o[0, :, :group]
+        assert torch.equal(o[0, :, group:], clean[0, :, group:]) and torch.equal(bad[..., group:], lse[..., group:])
+        assert bool((head[..., 3] == torch.inf).all()) and bool((head[..., 9] == -torch.inf).all())
+        assert bool(torch.isnan(head[..., 17]).all()) and bool(torch.isnan(head[..., 20]).all())
+        rest = [i for i in range(d) if i not in (3, 9, 17, 20)]
+        ref, rlse, tol, tlse = c.exact()
+        err = (head.double() - ref[0, :, :group]).abs()[..., rest]
+        assert bool((err <= tol[0, :, :group][..., rest]).all())
+        assert bool(((bad.double() - rlse).abs() <= tlse).all())
+
+
 @pytest.mark.parametrize("fmt", ["fp8_e4m3", "int8"])
 @pytest.mark.parametrize("t,heads,d", ROWS)
 def test_a_row_without_a_scale_in_mid_sequence(fmt, t, heads, d):

@@ -217,6 +217,15 @@ VH_DEV uint32_t nonfinite(uint32_t w) {
   return ((w & e) == e ? 0xffffu : 0u) | (((w >> 16) & e) == e ? 0xffff0000u : 0u);
 }
 
+// sum, and NaN where a half of w is infinite or NaN: w times zero added.
+template <int FMT>
+VH_DEV float times_zero(uint32_t w, float sum) {
+  if constexpr (FMT == CACHE_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0u), sum, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0u), sum, false);
+}
+
 // Over the four lanes that hold a row, 16 apart, by register swaps: rows of
 // 16 lanes, then halves of the wave.
 VH_DEV float max_rows(float v) {
@@ -537,9 +546,9 @@ VH_DEV void operands(const f32x4 (&p)[2][NT], const f32x4 (&vs)[2], const float 
 }
 
 // Values of a step that are not finite, which were left out of the product
-// (they would reach rows that do not see them as 0 * inf), added to the rows
-// that do.  p: the probabilities; chan(c, i): the channel of row 4 g + i of
-// channel tile c.
+// (they would reach rows that do not see them as 0 * inf, and infinities times
+// the low part of a probability are NaN), added to the rows that see them.
+// p: the probabilities; chan(c, i): the channel of row 4 g + i of channel tile c.
 template <int FMT, int CT, int NT, typename F>
 VH_DEV void add_nonfinite(const Args& a, const Step& st, const f32x4 (&p)[2][NT], const uint32_t (&seen)[NT],
                           f32x4 (&acc)[CT][NT], F chan) {
@@ -564,6 +573,30 @@ VH_DEV void add_nonfinite(const Args& a, const Step& st, const f32x4 (&p)[2][NT]
           if (ok && nonfinite<FMT>(x) & 0xffffu) acc[c][nt][i] += w * unpack2<FMT>(x)[0];
         }
     }
+  }
+}
+
+// Whether there is a NaN among a wave's sums.
+template <int CT, int NT>
+VH_DEV bool nan_among(const f32x4 (&acc)[CT][NT]) {
+  bool nan = false;
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nan |= acc[c][nt][i] != acc[c][nt][i];
+  return nan;
+}
+
+template <int CT, int NT>
+VH_DEV void start(float (&m)[NT], float (&l)[NT], float (&top)[NT], f32x4 (&acc)[CT][NT]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = -__builtin_inff();
+    l[nt] = top[nt] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 }
 
@@ -661,13 +694,7 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 
   f32x4 acc[CT][NT];
   float m[NT], l[NT], top[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt] = -__builtin_inff();
-    l[nt] = top[nt] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  start(m, l, top, acc);
   Finder find(a, b, h, begin, end);
 
   uint4 kr[2][KQ];
@@ -801,7 +828,20 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
-        if (__any(quick<FMT>(S, k1, vs, fac, m, top, p))) {
+        bool far = quick<FMT>(S, k1, vs, fac, m, top, p);
+        if constexpr (!BYTE) {  // an infinity times the low part of a probability would be NaN
+          float odd[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int w = 0; w < VB; ++w)
+#pragma unroll
+                for (int d = 0; d < VW; ++d) odd[t] = times_zero<FMT>(vr[t][i][w][d], odd[t]);
+          far |= odd[0] != odd[0] || odd[1] != odd[1];
+        }
+        if (__any(far)) {
           load_k(st);  // once more, seldom
           break;
         }
@@ -923,6 +963,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   };
   static_assert(sizeof(Stage) * 2 >= (size_t)(TILES - 1) * RW * CT * NT * 64 * 16, "results reuse the stages");
   __shared__ Stage s_stage[2];
+  __shared__ int s_nan;
   __shared__ float s_m[RW][16 * NT], s_l[RW][16 * NT];
 
   const Block blk = block_of(a);
@@ -947,13 +988,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 
   f32x4 acc[CT][NT];
   float m[NT], l[NT], top[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt] = -__builtin_inff();
-    l[nt] = top[nt] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[c][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  start(m, l, top, acc);
   Finder find(a, b, h, begin, end);
 
   // a thread's part in the conversion
@@ -1099,14 +1134,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
     }
   };
 
-  if (begin < end) {
+  // The keys; `quickly`: with quick steps, whose products leave no value out.  An
+  // infinity among 16-bit ones may then have become NaN, and a workgroup whose
+  // sums hold one takes its keys once more without (a test of the values as they
+  // are converted would reach the other waves a step late).
+  auto pass = [&](auto quickly) __attribute__((always_inline)) {
+    constexpr bool QUICKLY = decltype(quickly)::value;
     const int whole = end < ctx ? end : ctx;
     // a step of the workgroup whose every key every row sees
     auto plain = [&](int key, const Steps& x) {
       int n = 0;
 #pragma unroll
       for (int w = 0; w < TILES; ++w) n += x.s[w].live[0] + x.s[w].live[1];
-      return key + KEYS <= whole && n == KEYS;
+      return QUICKLY && key + KEYS <= whole && n == KEYS;
     };
     // after the last step it is asked for again, and not used
     auto after = [&](int key) { return key + KEYS < end ? key + KEYS : key; };
@@ -1172,7 +1212,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       fed = false;
       pending = true;
       advance();
-      while (key0 < end && is_plain) {
+      while (QUICKLY && key0 < end && is_plain) {
         feed();
         // The quick form of the softmax, written out so that nothing waits:
         // operands are read AHEAD of their products, and the last step's second
@@ -1272,7 +1312,21 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
       }
     } while (key0 < end);
     add(s_stage[half ^ 1]);
-    if constexpr (TILES > 1) __syncthreads();  // the stages are free
+  };
+  if (begin < end) {
+    if (!BYTE && tid == 0) s_nan = 0;
+    pass(std::true_type());
+    if constexpr (!BYTE) {
+      if (nan_among(acc)) s_nan = 1;
+    }
+    if constexpr (!BYTE || TILES > 1) __syncthreads();  // the stages are free
+    if constexpr (!BYTE) {
+      if (s_nan) {
+        start(m, l, top, acc);
+        pass(std::false_type());
+        if constexpr (TILES > 1) __syncthreads();
+      }
+    }
   }
   if (find.bad && lane == 0) atomicOr(a.c.flag, VH_CACHE_ERR_PAGE);
 
