@@ -799,7 +799,8 @@ int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);
  * draft, 0) and mass = its sum (a rest of nothing is left as it was).  With no
  * draft, draft(x) counts as 1, rest(x) becomes 0 and mass loses it.  Where no
  * child is taken the last token is the first index at which the running sum
- * of rest passes r times the whole.  Sums are float64, in a fixed order.
+ * of rest passes r times the whole; where chosen children left nothing in it,
+ * the token taken out last.  Sums are float64, in a fixed order.
  * told [batch, nodes]: the tokens taken and then the last, -1 after them;
  * path [batch, nodes]: the first node and those taken, -1 after them; count
  * [batch]: how many.  A token outside the vocabulary is never taken.  work:

@@ -7,6 +7,9 @@
 // number of rejections is max(target - c * draft, 0) with c the sum of the
 // masses so far, so a row needs no buffer, only c.
 //
+// Chosen children may take everything out of a row: the last one taken out is
+// then put back, so that no token of probability 0 is told.
+//
 // The token after the kept nodes is found in two passes over one row: sums of
 // 4096 entries each, over many workgroups, then the one piece in which the
 // running sum passes r times the whole.  Sums are float64 in a fixed order:
@@ -338,6 +341,20 @@ __global__ void __launch_bounds__(PICK_THREADS) k_verify_pick(VerifyArgs a) {
   int64_t* out = a.told + b * a.nodes + row.count - 1;
   // the piece in which the running sum passes the bar, or the last with anything in it
   const int piece = pick(v > 0.0 && upto > bar, v > 0.0, s_pick);
+  if constexpr (!DRAFT) {
+    static_assert(MAX_NODES == PICK_THREADS, "a thread a node");
+    if (piece < 0 && total == 0.0) {  // the children took everything out: the last one taken out is put back
+      const int64_t x = gone[0];
+      bool out_last = x >= 0 && x < a.vocab && a.target[b * a.target_sb + row.last * a.target_sn + x] > 0.0f;
+      for (int n = row.last + 1; out_last && n < (int)threadIdx.x; ++n)  // not where an earlier sibling had
+        out_last = a.parents[b * a.nodes + n] != row.last || a.tokens[b * a.nodes + n] != x;
+      const int node = pick(false, out_last, s_pick);
+      if (node >= 0) {
+        if (threadIdx.x == node) *out = x;
+        return;
+      }
+    }
+  }
   if (piece < 0 || total != total) {  // no distribution: the end of it, or its start where it holds a NaN
     if (threadIdx.x == 0) *out = total != total ? 0 : a.vocab - 1;
     return;

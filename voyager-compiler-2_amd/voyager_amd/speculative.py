@@ -130,7 +130,8 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tens
     None: the children were chosen (a draft's best tokens), so draft(x) is 1 for
     the child's own token and rest loses it.  Where no child is taken, the last
     token is drawn from rest by ``r``: the first index at which its running sum
-    passes r times the whole.  The tokens then follow the target's distribution
+    passes r times the whole (where chosen children left nothing in it, the
+    token taken out last).  The tokens then follow the target's distribution
     for ``u [batch, nodes]`` and ``r [batch]`` uniform in [0, 1) (float32).
 
     Returns ``told [batch, nodes]`` (int64: the tokens taken, then the last; -1
