@@ -56,3 +56,17 @@ def test_many_children_that_cover_it():
     target[0, :, 999] = 0.0
     told, _, count = _run(target, [[-1] + [0] * (n - 1)], tokens, [[1 - 2.0**-24] * n], [0.9])
     assert told[0][0] == 998 and count == [1]
+
+
+@pytest.mark.parametrize("vocab", [40, 5000])
+@pytest.mark.parametrize("rejected", [0, 1, 2])
+def test_a_row_that_holds_a_nan_tells_its_start(vocab, rejected):
+    """With none, one or two sampled children rejected before."""
+    g = torch.Generator().manual_seed(vocab)
+    draft = torch.randn(1, 3, vocab, generator=g).softmax(-1)
+    target = torch.randn(1, 3, vocab, generator=g).softmax(-1)
+    target[0, 0, 7], target[0, 0, 8] = 0.0, 0.0
+    target[0, 0, vocab - 5] = float("nan")
+    parents = [[-1] + [0] * rejected + [-1] * (2 - rejected)]
+    told, path, count = _run(target, parents, torch.tensor([[0, 7, 8]]), [[0.5] * 3], [0.4], draft)
+    assert told == [[0, -1, -1]] and path == [[0, -1, -1]] and count == [1]

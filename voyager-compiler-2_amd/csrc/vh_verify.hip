@@ -97,6 +97,13 @@ VH_DEV void tell_none(const VerifyArgs& a, int64_t b, int count, int threads) {
   if (threadIdx.x == 0) a.count[b] = count;
 }
 
+// What rejections leave of a probability: max(p - c q, 0), and NaN where that is
+// one, so that a row which holds a NaN has no sum, with a rejection or without.
+VH_DEV double left_of(double p, double c, double q) {
+  const double x = p - c * q;
+  return x <= 0.0 ? 0.0 : x;
+}
+
 // The sum over the workgroup in a fixed order; every thread gets it.
 template <int N>
 VH_DEV double block_sum(double v, double* s_part) {
@@ -131,14 +138,14 @@ __global__ void __launch_bounds__(WALK_THREADS) k_verify_walk(VerifyArgs a) {
       const double more = c + mass;
       double v = 0.0;
 #pragma unroll 8
-      for (int64_t x = threadIdx.x; x < a.vocab; x += WALK_THREADS) v += fmax((double)p[x] - more * (double)q[x], 0.0);
+      for (int64_t x = threadIdx.x; x < a.vocab; x += WALK_THREADS) v += left_of(p[x], more, q[x]);
       const double left = block_sum<WALK_THREADS>(v, s_part);
       if (left > 0.0) {
         c = more;
         mass = left;
       }
     }
-    const double q = s.q[n], rest = fmax((double)s.p[n] - c * q, 0.0);
+    const double q = s.q[n], rest = left_of(s.p[n], c, q);
     if ((double)s.u[n] * mass * q < rest) {
       if (threadIdx.x == 0) tell(a, b, s, count, n);
       ++count;
@@ -216,7 +223,7 @@ struct Rest {
     if constexpr (DRAFT) {
       const float y0 = q[first + at];
       const double y = i < n ? y0 : 0.0f;
-      return double2{c > 0.0 ? fmax(x - c * y, 0.0) : x, c_before > 0.0 ? fmax(x - c_before * y, 0.0) : x};
+      return double2{c > 0.0 ? left_of(x, c, y) : x, c_before > 0.0 ? left_of(x, c_before, y) : x};
     } else {
       return double2{gone[i >> 5] >> (i & 31) & 1 ? 0.0 : x, 0.0};
     }
