@@ -90,7 +90,6 @@ class Rotary:
         self.dim, self.rotary_dim, self.interleaved = dim, rotary_dim, bool(interleaved)
         f, self.factor = frequencies(rotary_dim, theta, scaling)
         self.turns = (f / (2 * math.pi)).to(device)  # per position: the kernel drops whole turns in float64
-        self._rest = _ROPE_REST.pack(dim, rotary_dim, 1 if interleaved else 0, self.factor, self.turns.data_ptr())
         self._checked = None
 
     def __call__(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor):
@@ -150,8 +149,10 @@ class Rotary:
         ps = positions.stride()
         # one position a token for all sequences: no step from one to the next
         step = ps[0] if len(ps) == 2 and positions.shape[0] > 1 else 0
+        # the frequencies' address as it is at the call: a copy of the embedding has its own
         d = ROPE.pack(*qd[:5], *kd[:5], positions.data_ptr(), step, ps[-1], batch, tokens, qd[5], kd[5], dtype_code(x.dtype),
-                      64 if positions.dtype is torch.int64 else 32, 1 if inverse else 0) + self._rest
+                      64 if positions.dtype is torch.int64 else 32, 1 if inverse else 0) + _ROPE_REST.pack(
+                          self.dim, self.rotary_dim, 1 if self.interleaved else 0, self.factor, self.turns.data_ptr())
         st = load().vh_rope(d, stream_on(x.device))
         if st:
             check(st, "vh_rope")
