@@ -10,6 +10,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libvoyager_hip.so")
@@ -267,6 +268,13 @@ def stream_on(device: torch.device) -> int:
         raise ValueError(f"Expected a cuda device, but got: {device}")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raise where a tensor carries a forward-mode tangent, which a kernel
+    would drop."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: no forward-mode derivative")
 
 
 def ptr(t: Optional[torch.Tensor]):

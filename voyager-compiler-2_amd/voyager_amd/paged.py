@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, load, ptr, stream_on
+from ._lib import check, dtype_code, load, no_tangents, ptr, stream_on
 
 FORMATS = {"fp8_e4m3": _lib.CACHE_E4M3, "int8": _lib.CACHE_INT8}
 MAX_DIM = 512
@@ -107,6 +107,7 @@ class PagedCache:
         n = self._slots(slots)
         if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             raise RuntimeError("PagedCache.write: the cache passes no gradient; write under torch.no_grad()")
+        no_tangents("PagedCache.write", k, v)
         shape = (n, self.kv_heads, self.dim)
         for name, t in (("k", k), ("v", v)):
             if t.shape != shape or t.dtype is not self.dtype or t.device != self.device:

@@ -15,7 +15,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import check, dtype_code, load, stream_on
+from ._lib import check, dtype_code, load, no_tangents, stream_on
 
 MAX_DIM = 512
 #: ``vh_rope_desc``: up to ``inverse``, which a call gives, and the rest, which the embedding does
@@ -97,12 +97,13 @@ class Rotary:
         dim]`` (either may be None) turned by ``positions [batch, tokens]`` or
         ``[tokens]`` (int32 or int64), contiguous, of the inputs' dtype
         (bfloat16, float16 or float32).  Views with dense channels are read in
-        place.  Differentiable in q and k, any number of times."""
+        place.  Differentiable in q and k, any number of times, in reverse mode."""
         given = (None if q is None else (q.shape, q.dtype, q.device), None if k is None else (k.shape, k.dtype, k.device),
                  positions.shape, positions.dtype, positions.device)
         if given != self._checked:  # a step's sizes are mostly those of the step before
             self._check(q, k, positions)
             self._checked = given
+        no_tangents("Rotary", q, k)
         if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
             return _Turn.apply(q, k, positions, self, False)
         return self._turn(q, k, positions, False)

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import check, load, stream_on
+from ._lib import check, load, no_tangents, stream_on
 from .paged import CacheFlag, PagedCache, _int32, _rows
 
 MAX_NODES = _lib.TREE_MAX_NODES
@@ -79,6 +79,7 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, cont
                          f"(got {q.dtype} {list(q.shape)} on {q.device})")
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("tree_attention: passes no gradient; call it under torch.no_grad()")
+    no_tangents("tree_attention", q)
     b, t, heads, dim = q.shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"tree_attention: {heads} query heads over {cache.kv_heads} of the cache")
