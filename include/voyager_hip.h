@@ -772,7 +772,8 @@ int vh_tree_masks(const int32_t* parents, int64_t batch, int32_t nodes, uint64_t
  * aligned device memory of vh_tree_attention_workspace_bytes(desc) bytes
  * (which goes by the sizes alone).
  * The keys of all sequences are shared out, by their number as the device reads
- * it, to about `workgroups` workgroups (0: the library chooses). */
+ * it, to about `workgroups` workgroups (0: the library chooses); what all
+ * tables have room for must stay under 2^39 positions. */
 typedef struct vh_tree_desc {
   vh_cache cache;
   const void* q;

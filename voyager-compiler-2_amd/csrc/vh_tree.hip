@@ -222,6 +222,8 @@ int desc_check(const vh_tree_desc* d, const char* what) {
   VH_REQUIRE((int64_t)d->nodes * (d->heads / c.kv_heads) < (1 << 24), "%s: too many rows", what);
   VH_REQUIRE((int64_t)d->table_pages * c.page < (1ll << 31) - 4096, "%s: too many pages", what);
   VH_REQUIRE((int64_t)d->batch * c.kv_heads < (1 << 20), "%s: too many sequences", what);
+  VH_REQUIRE(d->batch * (((int64_t)d->table_pages * c.page + tree::PIECE - 1) / tree::PIECE) < (1ll << 32),
+             "%s: too many keys", what);
   VH_REQUIRE(!d->masks || d->nodes <= MAX_NODES, "%s: at most %d nodes", what, MAX_NODES);
   VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
   VH_REQUIRE(d->workgroups >= 0 && d->workgroups <= (1 << 20), "%s: bad number of workgroups", what);

@@ -94,6 +94,7 @@ VH_DEV int visible(const Args& a, int ctx, int row0) {
 // of 256, two tokens: 44 us at one piece a split, 32 at three).  Every lane of a
 // wave calls these together; a lane holds a sequence.
 constexpr int PIECE = 128, CHUNK = 4;
+constexpr uint32_t CHUNK_MOST = 0x7fffffffu / PIECE;  // more pieces than a sequence has; its keys are an int
 VH_DEV uint32_t pieces(const Args& a, int b) {
   const int ctx = b < a.batch ? a.context[b] : -1;
   return fits(a, ctx) && b < a.batch ? ((uint32_t)ctx + a.nodes + PIECE - 1) / PIECE : 0u;
@@ -110,8 +111,8 @@ VH_DEV uint32_t chunk_of(const Args& a) {
   }
   all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
   if (all == 0u) return 1u;
-  const uint32_t least = (all + a.share - 1) / a.share;
-  return least >= CHUNK ? least : max(least, min((uint32_t)CHUNK, (all + a.fill - 1) / a.fill));
+  const uint32_t least = all / a.share + (all % a.share ? 1u : 0u);
+  return least >= CHUNK ? min(least, CHUNK_MOST) : max(least, min((uint32_t)CHUNK, (all + a.fill - 1) / a.fill));
 }
 VH_DEV uint32_t splits_of(uint32_t piece, uint32_t chunk) { return piece <= chunk ? 1u : (piece + chunk - 1) / chunk; }
 
