@@ -263,11 +263,15 @@ def stream_of(t: torch.Tensor) -> int:
 def stream_on(device: torch.device) -> int:
     """The current HIP stream of ``device``, as a raw handle
     (``torch.cuda.current_stream`` without the stream object it builds,
-    which costs 2 us of every launch)."""
+    which costs 2 us of every launch).  A kernel runs on the current device,
+    whatever its stream's: another one's tensors are refused."""
     if device.type != "cuda":
         raise ValueError(f"Expected a cuda device, but got: {device}")
-    index = device.index
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+    current = torch._C._cuda_getDevice()
+    if device.index is not None and device.index != current:
+        raise RuntimeError(f"voyager_amd: tensors on {device} while the current device is cuda:{current}; "
+                           f"call under torch.cuda.device({device.index})")
+    return torch._C._cuda_getCurrentRawStream(current)
 
 
 def no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
