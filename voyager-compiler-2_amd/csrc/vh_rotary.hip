@@ -8,8 +8,10 @@
 //
 // The angle is formed in float64 as turns (position times turns per position,
 // then the fraction): at position 1e6 a float32 product is off by 0.06 turns,
-// the float64 one by less than 1e-9.  Sine and cosine are taken in float32 of
-// the fraction, once per token and pair, and shared by all heads through LDS.
+// the float64 one by less than 1e-9.  Sine and cosine are taken of the fraction,
+// once per token and pair, and shared by all heads through LDS: for 16-bit
+// values in float32 (off by less than 2^-22, where a result rounds by 2^-12 or
+// more), for float32 ones in float64, rounded once with the factor.
 //
 // Bound by memory: 4 bytes moved per bfloat16 value, 3 operations.  32 + 8
 // heads of 128 in bfloat16: 8192 tokens (168 MB read and written) 29-33 us,
@@ -89,9 +91,15 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a) {
     const int64_t at = b * a.pos_sb + n * a.pos_st;
     const int64_t p = a.pos64 ? ((const int64_t*)a.pos)[at] : (int64_t)((const int32_t*)a.pos)[at];
     const double turn = (double)p * a.turns[j];
-    float s, c;
-    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-    s_cs[t * half + j] = make_float2(c * a.factor, s * a.factor * a.sign);
+    if constexpr (sizeof(T) == 4) {
+      double s, c;
+      sincospi(2.0 * (turn - rint(turn)), &s, &c);
+      s_cs[t * half + j] = make_float2((float)(c * a.factor), (float)(s * a.factor * a.sign));
+    } else {
+      float s, c;
+      sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+      s_cs[t * half + j] = make_float2(c * a.factor, s * a.factor * a.sign);
+    }
   }
   __syncthreads();
   const int heads = a.nq + a.nk;
