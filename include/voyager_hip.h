@@ -791,8 +791,9 @@ int vh_tree_attention(const vh_tree_desc* desc, void* work, int64_t work_bytes, 
 int64_t vh_tree_attention_workspace_bytes(const vh_tree_desc* desc);
 
 /* The choice among drafted tokens.  target [batch, nodes, vocab] float32: the
- * target's probabilities after each node; draft: those of the draft model, or
- * NULL where each node's children were chosen, not sampled; tokens [batch,
+ * target's probabilities after each node; draft: those of the draft model, from
+ * which a node's children were sampled with replacement, or NULL where they were
+ * chosen, not sampled; tokens [batch,
  * nodes]: each node's token (the first's is not read); u [batch, nodes], r
  * [batch]: numbers in [0, 1).  From the first node on, a node's children are
  * tried in order: with rest = the target's row and mass = 1, child n of token

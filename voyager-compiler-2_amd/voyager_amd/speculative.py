@@ -127,7 +127,9 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, tree: Tree, u: torch.Tens
     token x is taken if ``u[n] * mass * draft(x) < rest(x)``, where rest begins
     as the target's row and mass as 1; if not, ``rest = max(rest - mass *
     draft, 0)`` and mass is its sum.  ``draft [batch, nodes, vocab]``: the draft
-    model's probabilities after each node, from which its children were sampled;
+    model's probabilities after each node, from which its children were sampled,
+    each on its own (with replacement: a token may come twice, and the rule
+    counts on it);
     None: the children were chosen (a draft's best tokens), so draft(x) is 1 for
     the child's own token and rest loses it.  Where no child is taken, the last
     token is drawn from rest by ``r``: the first index at which its running sum
