@@ -89,3 +89,22 @@ def test_values_over_many_binades(fmt, t, heads, d, rising):
     c.fill()
     for workgroups in (0, 1):
         c.agrees(c.run(workgroups=workgroups), floor=2.0**-34)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("t,heads,d", SINKS)
+@pytest.mark.parametrize("size", [2.0**126, 2.0**-80])
+def test_values_near_the_ends_of_their_type(fmt, t, heads, d, size):
+    """Values between 1 and 2 times ``size`` under scores that grow along the
+    keys: sums of exponentials times such values are not finite, results are."""
+    c = Case(2, t, heads, 1, d, fmt, torch.bfloat16, 64, [1500, 70], seed=t, spread=0.0, parents=None)
+    g = torch.Generator().manual_seed(t)
+    at = torch.arange(c.k.shape[1])[:, None, None]
+    base = torch.randn(d, generator=g)
+    base *= d ** 0.5 / base.norm()
+    c.q = (base + 0.1 * torch.randn(c.q.shape, generator=g)).bfloat16().cuda()
+    c.k = (base * at * 0.004 / d ** 0.5 + 0.3 * torch.randn(c.k.shape, generator=g)).bfloat16().cuda()
+    c.v = ((1 + 0.9 * torch.rand(c.v.shape, generator=g)) * size).bfloat16().cuda()
+    c.fill()
+    for workgroups in (0, 1, 8):
+        c.agrees(c.run(workgroups), floor=2.0**-34)

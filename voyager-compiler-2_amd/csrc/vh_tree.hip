@@ -90,6 +90,9 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
   const int splits = (int)sp.n;
   const int64_t step = (int64_t)a.c.kv_heads * a.rows, at = ((int64_t)sp.before * a.c.kv_heads + h) * a.rows + row;
   if (!in) return;
+  // splits' sums are under 1 and their results no larger than the largest value:
+  // so is what is joined, with the reference this far over the largest one
+  const float room = splits > 1 ? (float)(32 - __clz(splits - 1)) : 0.0f;
   float M = -__builtin_inff(), L = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   // four splits at a time, so that their reads overlap
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
         x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
     }
-    const float to = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M);
+    const float to = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)) + room, M);
     const float keep = M == -__builtin_inff() ? 1.0f : tree::exp2_fast(M - to);
     M = to;
     L *= keep;

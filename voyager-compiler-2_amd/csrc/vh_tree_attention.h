@@ -412,15 +412,22 @@ VH_DEV void see(const Args& a, int b, int ctx, int key0, const int (&live)[2], c
 // of 2^-34 of it still counts (at 1, 32768 keys of 2^-26 beside one were in the
 // sum and not in the product, half of a result).  Over codes the unit does it;
 // float16 values have the reference of the softmax, m, that far under the maximum.
+// bfloat16 has the range of float32 and needs no place: there the maximum is put
+// at 2^-20, so that sums of probabilities times values near the type's largest
+// stay finite, as their result is.
 //
 // In the quick form, for a step that every row sees, nothing moves: the
 // probabilities are taken against the reference as it is, and the step is given
-// up (true) where an operand passes 2^15 or where a row has no reference yet.  It
-// needs no maximum over lanes, and its loop holds no branch that writes the
-// accumulators (with one, the compiler keeps two copies of them).  Five binades
-// are left for it: after the first steps the maximum seldom rises by that.
+// up (true) where an operand passes 2^5 times its place or where a row has no
+// reference yet.  It needs no maximum over lanes, and its loop holds no branch
+// that writes the accumulators (with one, the compiler keeps two copies of them).
+// After the first steps the maximum seldom rises by five binades.
 constexpr int PLACE = 10;
-constexpr float OPERAND_MOST = 0x1p15f;
+template <int FMT>
+constexpr float operand_most() { return FMT == CACHE_BF16 ? 0x1p-15f : 0x1p15f; }
+// What lies between a row's maximum and its reference, in binades.
+template <int FMT>
+constexpr float reference_under() { return FMT == CACHE_F16 ? 10.0f : FMT == CACHE_BF16 ? -20.0f : 0.0f; }
 // Bounds on a probability and on a value scale in a row's unit, so that no sum
 // and no product of the quick form passes float32.
 constexpr float QUICK_MOST = 0x1p100f;
@@ -430,6 +437,16 @@ VH_DEV float unit_of(float top) {  // top / 2^PLACE, up to the next power of two
   const uint32_t e = __float_as_uint(top) & 0x7f800000u;
   return __uint_as_float((e < LEAST ? LEAST : e) - LEAST + 0x00800000u);
 }
+// A row's sum brought to [1/2, 1) by a power of two, which the reference takes
+// and by which the accumulators are to be multiplied: they then are no larger
+// than the largest value.
+VH_DEV float bring(float& L, float& M) {
+  const int e = __builtin_amdgcn_frexp_expf(L);
+  L = __builtin_amdgcn_ldexpf(L, -e);
+  M += (float)e;
+  return __builtin_amdgcn_ldexpf(1.0f, -e);
+}
+
 VH_DEV float inverse_unit(float top) { return __uint_as_float(0x7f000000u - __float_as_uint(unit_of(top))); }
 
 template <int FMT, int NT>
@@ -462,8 +479,8 @@ VH_DEV bool quick(const f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&v
       }
     }
     far |= m[nt] == -__builtin_inff();
-    if constexpr (BYTE) far |= operand > OPERAND_MOST || most > QUICK_MOST || high * inv > QUICK_MOST;
-    else far |= most > OPERAND_MOST;
+    if constexpr (BYTE) far |= operand > operand_most<FMT>() || most > QUICK_MOST || high * inv > QUICK_MOST;
+    else far |= most > operand_most<FMT>();
   }
   return far;
 }
@@ -486,7 +503,7 @@ VH_DEV void careful(f32x4 (&S)[2][NT], const f32x4 (&ks)[2], const f32x4 (&vs)[2
           S[t][nt][i] = seen[nt] >> (4 * t + i) & 1 ? x : -__builtin_inff();
           v = fmaxf(v, S[t][nt][i]);
         }
-    const float to = fmaxf(m[nt], max_rows(v) - (FMT == CACHE_F16 ? PLACE : 0));
+    const float to = fmaxf(m[nt], max_rows(v) - reference_under<FMT>());
     const float alpha = m[nt] == -__builtin_inff() ? 0.0f : exp2_fast(m[nt] - to);
     m[nt] = to;
     l[nt] *= alpha;
@@ -879,7 +896,8 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
       const float mw = s_m[w][16 * nt + r];
       L[nt] += s_l[w][16 * nt + r] * (mw == -__builtin_inff() ? 1.0f : exp2_fast(mw - M[nt]));
     }
-    const float f = (m[nt] == -__builtin_inff() ? 1.0f : exp2_fast(m[nt] - M[nt])) * (BYTE ? unit_of(top[nt]) : 1.0f);
+    float f = (m[nt] == -__builtin_inff() ? 1.0f : exp2_fast(m[nt] - M[nt])) * (BYTE ? unit_of(top[nt]) : 1.0f);
+    f *= bring(L[nt], M[nt]);
     const bool none = pads(a, b, node[nt]);
     if (none) {
       M[nt] = -__builtin_inff();
@@ -1291,10 +1309,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
           for (int x = c * HALVES / CT; x < (c + 1) * HALVES / CT; ++x) scores2(x);
           __builtin_amdgcn_sched_barrier(0);
         }
-        bool far = BYTE && operand > OPERAND_MOST;
+        bool far = BYTE && operand > operand_most<FMT>();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          far |= sum[nt] > (BYTE ? QUICK_MOST : OPERAND_MOST) || m[nt] == -__builtin_inff();
+          far |= sum[nt] > (BYTE ? QUICK_MOST : operand_most<FMT>()) || m[nt] == -__builtin_inff();
           if constexpr (BYTE) far |= high * inv[nt] > QUICK_MOST;
         }
         pending = false;
@@ -1331,11 +1349,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
   }
   if (find.bad && lane == 0) atomicOr(a.c.flag, VH_CACHE_ERR_PAGE);
 
-  float M[NT], L[NT];
+  float M[NT], L[NT], unit[NT];  // unit: of the accumulators
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     L[nt] = sum_rows(l[nt]);
     M[nt] = m[nt];
+    unit[nt] = bring(L[nt], M[nt]) * (BYTE ? unit_of(top[nt]) : 1.0f);
   }
   if constexpr (TILES > 1) {  // the second group of keys onto the first
     if (tile == 1 && g == 0) {
@@ -1350,26 +1369,26 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s_o[(c * NT + nt) * 64 + lane] = acc[c][nt] * (BYTE ? unit_of(top[nt]) : 1.0f);
+        for (int nt = 0; nt < NT; ++nt) s_o[(c * NT + nt) * 64 + lane] = acc[c][nt] * unit[nt];
     }
     __syncthreads();
     if (tile == 1) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float m1 = s_m[rw][16 * nt + r], to = fmaxf(M[nt], m1);
+      const float m1 = s_m[rw][16 * nt + r], to = fmaxf(M[nt], m1) + 1.0f;  // room for two
       const float f0 = M[nt] == -__builtin_inff() ? 1.0f : exp2_fast(M[nt] - to);
       const float f1 = m1 == -__builtin_inff() ? 1.0f : exp2_fast(m1 - to);
       M[nt] = to;
       L[nt] = L[nt] * f0 + s_l[rw][16 * nt + r] * f1;
-      const float f = f0 * (BYTE ? unit_of(top[nt]) : 1.0f);
+      const float f = f0 * unit[nt];
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[c][nt] = acc[c][nt] * f + s_o[(c * NT + nt) * 64 + lane] * f1;
     }
-  } else if constexpr (BYTE) {
+  } else {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) acc[c][nt] *= unit_of(top[nt]);
+      for (int c = 0; c < CT; ++c) acc[c][nt] *= unit[nt];
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
