@@ -23,7 +23,7 @@
 // products of S are exact.  bfloat16 queries over codes are scaled by a power
 // of two per row into float16; what falls under its least value is under 2^-38
 // of the row's largest channel.  A key's scale multiplies its score, a value's
-// scale its probability.
+// scale its probability, which goes into the second product in two 16-bit parts.
 //
 // Two kernels.  k_tree is for few rows (a token or two of a grouped head),
 // where the cache's bytes bound it: each wave takes its own keys straight from
@@ -91,7 +91,8 @@ VH_DEV int visible(const Args& a, int ctx, int row0) {
 // with which all pieces make no more than `share` splits and a rest a sequence,
 // and four where that still makes `fill`, so that a wave has steps to ask ahead
 // in and a split's results are few beside its keys (8 sequences of 8192, heads
-// of 256, two tokens: 44 us at one piece a split, 32 at three).  Every lane of a
+// of 256, two tokens: 42 us at one piece a split, 37 at three; one token over
+// 4096 each: 28 and 22).  Every lane of a
 // wave calls these together; a lane holds a sequence.
 constexpr int PIECE = 128, CHUNK = 4;
 constexpr uint32_t CHUNK_MOST = 0x7fffffffu / PIECE;  // more pieces than a sequence has; its keys are an int
@@ -594,16 +595,21 @@ VH_DEV void add_nonfinite(const Args& a, const Step& st, const f32x4 (&p)[2][NT]
   }
 }
 
-// Whether there is a NaN among a wave's sums.
+// Whether a NaN is among the results of a wave's rows whose scores are numbers:
+// then it comes from the values.
 template <int CT, int NT>
-VH_DEV bool nan_among(const f32x4 (&acc)[CT][NT]) {
+VH_DEV bool nan_among(const f32x4 (&acc)[CT][NT], const float (&l)[NT]) {
   bool nan = false;
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
+  for (int nt = 0; nt < NT; ++nt) {
+    const float sum = sum_rows(l[nt]);
+    bool mine = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) nan |= acc[c][nt][i] != acc[c][nt][i];
+      for (int i = 0; i < 4; ++i) mine |= acc[c][nt][i] != acc[c][nt][i];
+    nan |= mine && sum == sum;
+  }
   return nan;
 }
 
@@ -676,9 +682,10 @@ constexpr int waves_of(int d, int fmt, int nt) {
 // once, at the end.
 //
 // Bound by the cache's bytes: 32 tokens, one a sequence, over 2048 to 8192
-// cached ones, 8 int8 key heads of 128 and 32 query heads (353 MB): 79-84 us,
-// 4.2-4.5 TB/s, as fast as this card's memory is read by a plain sum.  One token
-// over 4096 (8.7 MB): 9.5 us, the latency of table, keys, values and joining.
+// cached ones, 8 int8 key heads of 128 and 32 query heads (353 MB): 76-82 us,
+// 4.3-4.6 TB/s, as fast as this card's memory is read by a plain sum.  In
+// bfloat16, all of 8192 (1.07 GB): 201 us with the joining, 5.3 TB/s.  One token
+// over 4096 (8.7 MB): 8.8 us, the latency of table, keys, values and joining.
 template <int D, int FMT, int NT>
 __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args a) {
   constexpr bool BYTE = FMT == CACHE_E4M3 || FMT == CACHE_INT8;
@@ -957,12 +964,12 @@ __global__ void __launch_bounds__(WAVES * 64, waves_of(D, FMT, NT)) k_tree(Args 
 // writes half an operand of each).
 //
 // 8 trees of 64 nodes over 1024 to 4096 cached tokens, 8 E4M3 key heads of 128
-// and 32 query heads (56 MB, 24 GFLOP): 50-65 us, 0.36-0.47 PFLOP/s.  The vector
-// instructions and LDS bound it (softmax, conversion and operand reads: each
-// half of all cycles, the matrix instructions a third; 0.77 PFLOP/s from one
-// length to the next), with about 18 us before the first product and after the
-// last.  2 of 13 nodes over 8192 to 32768 in float16
-// (218 MB): 46 us, 4.7 TB/s.
+// and 32 query heads (56 MB, 24 GFLOP): 75 us, 0.31 PFLOP/s (65 with
+// probabilities in one part, two tiles a step).  No unit is full: a third of the
+// CUs' cycles go to the start, the end and splits of different lengths, and of
+// the rest the vector instructions take a half, the matrix instructions three
+// tenths and LDS a fifth, with two waves a SIMD to fill each other's waits.  2 of
+// 13 nodes over 8192 to 32768 in float16 (218 MB): 49 us, 4.5 TB/s.
 template <int D>
 constexpr int wide_nt() { return D <= 128 ? 2 : 1; }
 
@@ -1336,7 +1343,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_tree_wide(Args a) {
     if (!BYTE && tid == 0) s_nan = 0;
     pass(std::true_type());
     if constexpr (!BYTE) {
-      if (nan_among(acc)) s_nan = 1;
+      if (nan_among(acc, l)) s_nan = 1;
     }
     if constexpr (!BYTE || TILES > 1) __syncthreads();  // the stages are free
     if constexpr (!BYTE) {
