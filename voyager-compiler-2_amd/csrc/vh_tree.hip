@@ -151,10 +151,10 @@ __global__ void __launch_bounds__(256) k_tree_merge(Args a) {
 
 // Many splits a sequence and few rows: a workgroup a row, whose groups share the
 // splits.  Else as many rows as fit one: rows alone fill the card then.  (us of
-// attention and joining, by the first and the second: 32 rows of 32 splits 10.6
-// and 14.2, 512 of 64 22.8 and 25.9, 832 of 32 65.6 and 67.0; 4096 of 8 42.8 and
-// 36.6, 16384 of 4 or 5 96.4 and 72.7.)  Joining these 16384 rows reads 42 MB in
-// 10.2 us, the most of it from the last cache.
+// attention and joining, by the first and the second: 32 rows of 32 splits 10.5
+// and 14.2, 512 of 64 24.1 and 27.0, 832 of 32 69 and 68; 4096 of 8 46.8 and
+// 39.3, 16384 of 4 or 5 110 and 86.)  Joining these 16384 rows reads 42 MB in
+// 10.4 us, the most of it from the last cache.
 template <int D>
 void merge(const Args& a, hipStream_t s) {
   constexpr int ALL = 1024 / D;  // groups of lanes in a workgroup
@@ -173,9 +173,9 @@ struct Plan {
 // The shape of the launch.  Up to 32 rows of a key head (16 of heads of 256)
 // a wave holds them all and takes its own keys; more share converted keys.  (us
 // by the first and the second, 4 sequences of 8192 over 8 key heads of 128,
-// E4M3: 8 rows 22.9 and 32.5, 32 rows 29.5 and 34.7, 48 rows 43.4 and 35.8; 4
-// heads of 256: 16 rows 24.1 and 32.0, 32 rows 30.8 and 33.1, but with 16
-// sequences 91 and 72, and of 16-bit keys 168 and 113.)
+// E4M3: 8 rows 22.4 and 34.6, 32 rows 30.6 and 36.4, 40 rows 43.7 and 36.8; 4
+// heads of 256: 16 rows 24.3 and 32.8, 32 rows 31.5 and 35.3, but with 16
+// sequences 92 and 83, and of 16-bit keys 165 and 114.)
 Plan plan_of(const vh_tree_desc* d) {
   Plan p;
   const int64_t rows = (int64_t)d->nodes * (d->heads / d->cache.kv_heads);
@@ -194,8 +194,8 @@ Plan plan_of(const vh_tree_desc* d) {
   const int64_t blocks = (int64_t)d->cache.kv_heads * p.row_blocks;
   // Two workgroups a CU hold their registers where rows are many, and each more
   // share costs its rows' partial results twice; single tokens' keys fill the
-  // card best at six, whose results are few.  (8 trees of 64 over 4096: 80 us at
-  // 1024, 67 at 512, 84 at 256; 32 tokens over 8192: 88 us at 512, 84 at 1536.)
+  // card best at six, whose results are few.  (8 trees of 64 over 4096: 103 us at
+  // 1024, 90 at 512, 101 at 256; 32 tokens over 2048 to 8192: 94 us at 512, 89 at 1536.)
   const int64_t slots = d->workgroups > 0 ? d->workgroups : p.wide ? 512 : 1536;
   int64_t share = slots / blocks;
   if (share < 1) share = 1;

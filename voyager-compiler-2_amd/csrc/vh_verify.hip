@@ -20,7 +20,11 @@
 // draft's probabilities may have to be summed during the walk).  32 trees of 31
 // chosen tokens, 128,000 entries a row (16.4 MB): 9.3 us for the walk with the
 // sums and 6.4 for the pick; five sampled tokens, 32,000 entries: 2.4 for the
-// walk, 3.8 for the sums, 6.4 for the pick.
+// walk, 3.8 for the sums, 6.4 for the pick.  Sampled siblings cost more: each that
+// is tried after a rejection has its row summed first, by the one workgroup of its
+// sequence: about 24 us a sum at 128,000 entries (1 MB), 5 at 32,000.  Trees of
+// three sampled children a node, 128,000 entries: one sequence 13 us where no
+// second sibling is tried and 61 with two sums, 32 sequences 59 as drawn.
 #include <hip/hip_runtime.h>
 
 #include "vh_device.h"
