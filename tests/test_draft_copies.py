@@ -42,3 +42,14 @@ def test_frequencies_put_elsewhere_are_followed(monkeypatch):
     r.turns = r.turns.clone()
     r(torch.zeros(1, 2, 3, 8), None, torch.arange(2))
     assert struct.unpack_from("@Q", seen[0], len(seen[0]) - 8)[0] == r.turns.data_ptr()
+
+
+def test_frequencies_on_another_device_are_refused(monkeypatch):
+    monkeypatch.setattr(rotary, "load", lambda: type("Entry", (), {"vh_rope": staticmethod(lambda d, s: 0)}))
+    monkeypatch.setattr(rotary, "stream_on", lambda device: 0)
+    r = rotary.Rotary(8, device="cpu")
+    args = torch.zeros(1, 2, 3, 8), None, torch.arange(2)
+    r(*args)
+    r.turns = r.turns.to("meta")
+    with pytest.raises(ValueError, match="frequencies on meta"):
+        r(*args)

@@ -99,7 +99,7 @@ class Rotary:
         (bfloat16, float16 or float32).  Views with dense channels are read in
         place.  Differentiable in q and k, any number of times, in reverse mode."""
         given = (None if q is None else (q.shape, q.dtype, q.device), None if k is None else (k.shape, k.dtype, k.device),
-                 positions.shape, positions.dtype, positions.device)
+                 positions.shape, positions.dtype, positions.device, self.turns.device)
         if given != self._checked:  # a step's sizes are mostly those of the step before
             self._check(q, k, positions)
             self._checked = given
