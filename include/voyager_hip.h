@@ -822,6 +822,35 @@ typedef struct vh_verify_desc {
 int vh_verify(const vh_verify_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
 int64_t vh_verify_workspace_bytes(int64_t batch, int64_t vocab);
 
+/* ------------------------------------------------ a pass over packed sequences
+ * Operators of a prompt's first pass, of the scoring of given text and of the
+ * step that trains on it, beside the reference's own (it has none of them). */
+
+/* Norms of queries and keys a head and their rotary positions in one pass:
+ * y = turn(w * x * r), r = (mean of a head's x^2 + eps)^-1/2, `rope` as vh_rope
+ * has it (`inverse` is not read), q_weight and k_weight [dim] of weight_dtype
+ * (float32 or the values'), eps positive.  Squares are summed in float32.
+ * The backward pass reads the inputs from rope.q and rope.k, the results'
+ * gradients from gq and gk (channels dense, strides in elements), writes the
+ * inputs' gradients to rope.q_out and rope.k_out (NULL: not wanted) and the
+ * weights' to gq_weight and gk_weight (NULL: not wanted), summed in a fixed
+ * order.  work: vh_norm_rope_workspace_bytes(desc) bytes, 16-byte aligned, not
+ * read where no weights' gradient is wanted. */
+typedef struct vh_norm_rope_desc {
+  vh_rope_desc rope;
+  const void *q_weight, *k_weight;
+  const void* gq;
+  int64_t gq_sb, gq_st, gq_sh;
+  const void* gk;
+  int64_t gk_sb, gk_st, gk_sh;
+  void *gq_weight, *gk_weight;
+  int32_t weight_dtype;
+  float eps;
+} vh_norm_rope_desc;
+int vh_norm_rope(const vh_norm_rope_desc* desc, vh_stream_t stream);
+int vh_norm_rope_backward(const vh_norm_rope_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
+int64_t vh_norm_rope_workspace_bytes(const vh_norm_rope_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif
