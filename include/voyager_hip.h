@@ -851,6 +851,36 @@ int vh_norm_rope(const vh_norm_rope_desc* desc, vh_stream_t stream);
 int vh_norm_rope_backward(const vh_norm_rope_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
 int64_t vh_norm_rope_workspace_bytes(const vh_norm_rope_desc* desc);
 
+/* Log probabilities of given tokens.  logits [rows, vocab] (bfloat16, float16
+ * or float32, entries dense, row stride in elements); tokens [rows]: a negative
+ * one pads (its results are 0, its alternatives -1, its gradient 0), one past
+ * the vocabulary has the log probability NaN, in its gradient as well.
+ * logprob, entropy [rows] float32, natural logarithms; top_logprob, top_token
+ * [rows, top]: the largest entries in order, of equal ones the first, a NaN
+ * before all others.  Entries of -inf have probability 0; a row of nothing else, or with
+ * +inf or NaN, has no probabilities: NaN.  stats [rows, 2] float32 (8-byte
+ * aligned) is for the backward pass, which reads logits, tokens, entropy,
+ * stats and top_token again and writes grad [rows, vocab], contiguous, for the
+ * gradients g_logprob, g_entropy [rows], g_top [rows, top] (NULL: none).
+ * work: vh_score_workspace_bytes(desc) bytes, 16-byte aligned. */
+#define VH_SCORE_MAX_TOP 64
+#define VH_SCORE_MAX_VOCAB 1048576
+typedef struct vh_score_desc {
+  const void* logits;
+  int64_t logits_st;
+  const int64_t* tokens;
+  int64_t rows, vocab;
+  float *logprob, *entropy, *stats;
+  float* top_logprob;
+  int64_t* top_token;
+  const float *g_logprob, *g_entropy, *g_top;
+  void* grad;
+  int32_t dtype, top;
+} vh_score_desc;
+int vh_score(const vh_score_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
+int vh_score_backward(const vh_score_desc* desc, vh_stream_t stream);
+int64_t vh_score_workspace_bytes(const vh_score_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,3 +65,59 @@ def within(got, ref, tol, what=""):
     err = (got.detach().double().cpu() - ref.cpu()).abs()
     ok = (err <= tol.cpu()) | (torch.isnan(ref.cpu()) & torch.isnan(err))
     assert bool(ok.all()), f"{what}: {int((~ok).sum())} of {ok.numel()} beyond, worst {float((err / tol.cpu()).max()):.3g}"
+
+
+# ----------------------------------------------------------------- scores
+def scores(logits, tokens, top, g=None, h=None, t=None):
+    """``(logprob, entropy, top_logprob, top_token, grad)`` of rows, from the definition."""
+    x = logits.double()
+    rows, vocab = x.shape
+    z = torch.log_softmax(x, -1)
+    p = torch.exp(z)
+    pz = torch.where(p == 0, 0.0, p * z)
+    entropy = -pz.sum(-1)
+    pad, past = tokens < 0, tokens >= vocab
+    logprob = torch.where(past, math.nan, z.gather(1, tokens.clamp(0, vocab - 1)[:, None])[:, 0])
+    # NaN above all, as a sort has it; of equal values the first
+    best = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top]
+    top_logprob = z.gather(1, best)
+    grad = None
+    if g is not None:
+        g, h, t = g.double(), h.double(), t.double()
+        at = torch.zeros_like(x).scatter_add_(1, tokens.clamp(0, vocab - 1)[:, None], g[:, None])
+        if top:
+            at = at.scatter_add_(1, best, t)
+        flat = torch.where(p == 0, 0.0, p * (z + entropy[:, None]))
+        grad = at - p * (g + t.sum(-1))[:, None] - h[:, None] * flat
+        grad = torch.where(past[:, None], math.nan, grad)
+        grad[pad] = 0
+    for y in (logprob, entropy, top_logprob):
+        y[pad] = 0
+    best[pad] = -1
+    return logprob, entropy, top_logprob, best, grad
+
+
+def score_tolerances(logits, ref, g=None, h=None, t=None):
+    """Of the results of :func:`scores`.  A power's exponent (x - m) log2(e) is
+    two roundings of its size, 2^-23 |d| relative in the power, where powers count
+    (|d| below 2^4 and a little), and the constant's 2^-25; the power
+    2^-22; sums of at most 64 terms a thread, 64 threads, 8 waves and 64 pieces
+    joined: under 150 roundings.  A logarithm: 2^-22 of its size."""
+    x = logits.double()
+    top = x.masked_fill(~torch.isfinite(x), -1e4).amax(-1)
+    rel = (32 + 4 + 150) * U
+    far = (x.masked_fill(~torch.isfinite(x), 0) - top[:, None]).abs()
+    entropy = ref[1]
+    lse = torch.logsumexp(x - top[:, None], -1).nan_to_num(0)
+    # log of the sum, and the token's own exponent
+    t_log = lambda size: rel + 2.0**-22 * (size.abs() + lse.abs() + 1)
+    tol = [t_log(ref[0].nan_to_num(0, neginf=0)), 2 * rel * (1 + entropy.nan_to_num(0)) + 2.0**-21 * (lse.abs() + 1)]
+    tol.append(rel + 2.0**-22 * (ref[2].nan_to_num(0, neginf=0).abs() + lse.abs()[:, None] + 1))
+    if g is not None:
+        p = torch.softmax(x, -1).nan_to_num(0)
+        size = p * ((g.double().abs() + t.double().abs().sum(-1))[:, None] * (rel + U * (far + 70))
+                    + h.double().abs()[:, None] * (2 * rel + 2.0**-21) * (far + entropy.nan_to_num(0)[:, None] + 1 + far * far * U))
+        given = sum(y.double().abs() for y in (g, h)).amax() + t.double().abs().sum(-1).amax()
+        tol.append(HALF[logits.dtype] * ref[4].nan_to_num(0).abs() + size * 1.01 + 70 * U * ref[4].nan_to_num(0).abs()
+                   + least(logits.dtype) + 1e-37 * given)
+    return tol

@@ -10,7 +10,7 @@ import re
 import pytest
 import torch
 
-from voyager_amd import _lib, rotary
+from voyager_amd import _lib, rotary, score
 
 P = 1 << 20
 
@@ -36,6 +36,7 @@ def test_descriptors_are_as_long_as_the_header_says():
     rope = rotary.ROPE.size + rotary._ROPE_REST.size
     assert _size("vh_rope_desc") == rope
     assert _size("vh_norm_rope_desc") == rope + rotary.NORM.size
+    assert _size("vh_score_desc") == score.SCORE.size
 
 
 # ------------------------------------------------------- norms and positions
@@ -117,3 +118,72 @@ def test_norm_refuses_tangents():
     with fwAD.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             r.normed(x, None, torch.arange(3), fwAD.make_dual(w, w), None)
+
+
+# ----------------------------------------------------------------- scores
+def _score(entry="vh_score", work=P, work_bytes=1 << 40, **kw):
+    a = dict(logits=P, logits_st=1000, tokens=P, rows=2, vocab=1000, logprob=P, entropy=P, stats=P, top_logprob=P, top_token=P,
+             g_logprob=P, g_entropy=0, g_top=0, grad=P, dtype=_lib.VH_F32, top=3)
+    a.update(kw)
+    d, lib = score.SCORE.pack(*a.values()), _lib.load()
+    if entry == "vh_score":
+        return lib.vh_score(d, work, work_bytes, None)
+    return lib.vh_score_backward(d, None) if entry == "vh_score_backward" else lib.vh_score_workspace_bytes(d)
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=_lib.VH_U8), dict(dtype=7), dict(rows=-1), dict(rows=1 << 24), dict(vocab=0),
+                                dict(vocab=-5), dict(vocab=(1 << 20) + 1), dict(top=-1), dict(top=65), dict(vocab=2)])
+def test_score_entries_refuse(kw):
+    assert _score(**kw) == 1 and _lib.load().vh_last_error().startswith(b"vh_score:")
+    assert _score("vh_score_backward", **kw) == 1 and _lib.load().vh_last_error().startswith(b"vh_score_backward:")
+    assert _score("vh_score_workspace_bytes", **kw) == -1
+
+
+def test_score_entries_need_their_tensors():
+    for kw in (dict(logits=0), dict(tokens=0), dict(logprob=0), dict(entropy=0), dict(stats=0), dict(top_logprob=0),
+               dict(top_token=0), dict(vocab=100000, work=None), dict(vocab=100000, work=P + 4), dict(vocab=100000, work_bytes=8)):
+        assert _score(**kw) == 1
+    for kw in (dict(logits=0), dict(tokens=0), dict(entropy=0), dict(stats=0), dict(grad=0), dict(g_top=P, top_token=0)):
+        assert _score("vh_score_backward", **kw) == 1
+
+
+def test_score_workspace_and_nothing():
+    need = lambda **kw: _score("vh_score_workspace_bytes", **kw)
+    assert need(rows=0) == 0 and need() == 0  # a row of 1000 is one piece
+    assert 0 < need(vocab=100000) < need(vocab=100000, top=64)
+    # where rows fill the card, pieces are as long as a workgroup holds
+    assert need(rows=4096, vocab=32768, dtype=_lib.VH_BF16) == 0
+    assert need(rows=4096, vocab=32769, dtype=_lib.VH_BF16) == 4096 * 2 * (3 * 8 + 12)
+    assert _score(rows=0, work=None, work_bytes=0) == 0 and _score("vh_score_backward", rows=0) == 0
+
+
+def test_score_arguments_refused():
+    x, t = torch.zeros(2, 3, 100), torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="tokens"):
+        score.token_scores(x, t[0])
+    with pytest.raises(ValueError, match="int64"):
+        score.token_scores(x, t.int())
+    with pytest.raises(TypeError, match="float16 or float32"):
+        score.token_scores(x.double(), t)
+    with pytest.raises(ValueError, match="vocabulary"):
+        score.token_scores(x[..., :0], t)
+    with pytest.raises(ValueError, match="vocabulary"):
+        score.token_scores(torch.zeros(1).expand((1 << 20) + 1), torch.tensor(0))
+    for top in (-1, 65, 101):
+        with pytest.raises(ValueError, match="alternatives"):
+            score.token_scores(x, t, top=top)
+    with pytest.raises(ValueError, match="alternatives"):
+        score.token_scores(x[..., :4], t, top=5)
+    with pytest.raises(ValueError, match="logits"):
+        score.token_scores(torch.tensor(1.0), t)
+    with pytest.raises(ValueError, match="cuda"):  # no CPU form
+        score.token_scores(x, t)
+
+
+def test_score_refuses_tangents():
+    import torch.autograd.forward_ad as fwAD
+
+    x = torch.zeros(2, 8)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            score.token_scores(fwAD.make_dual(x, x), torch.zeros(2, dtype=torch.int64))

@@ -205,10 +205,14 @@ _SIGNATURES = {
     "vh_tree_attention_workspace_bytes": ([_P], _I64),
     "vh_verify": ([_P, _P, _I64, _P], _I32),
     "vh_verify_workspace_bytes": ([_I64, _I64], _I64),
-    # a pass over packed sequences: descriptors' bytes as well (rotary.NORM after vh_rope_desc's)
+    # a pass over packed sequences: descriptors' bytes as well (rotary.NORM after vh_rope_desc's,
+    # score.SCORE)
     "vh_norm_rope": ([_P, _P], _I32),
     "vh_norm_rope_backward": ([_P, _P, _I64, _P], _I32),
     "vh_norm_rope_workspace_bytes": ([_P], _I64),
+    "vh_score": ([_P, _P, _I64, _P], _I32),
+    "vh_score_backward": ([_P, _P], _I32),
+    "vh_score_workspace_bytes": ([_P], _I64),
 }
 
 DECODE_ERR_FP16_RANGE = 1
