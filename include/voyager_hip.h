@@ -881,6 +881,49 @@ int vh_score(const vh_score_desc* desc, void* work, int64_t work_bytes, vh_strea
 int vh_score_backward(const vh_score_desc* desc, vh_stream_t stream);
 int64_t vh_score_workspace_bytes(const vh_score_desc* desc);
 
+/* The plan of a packed batch: sequence s is the rows offsets[s] ... offsets[s +
+ * 1] - 1 of `tokens` (offsets [sequences + 1] begin at 0 and do not fall; rows
+ * behind the last pad).  plan: vh_packing_ints(tokens) int32 of device memory.
+ * Offsets are read on the device: where they are not as they should be, all
+ * rows pad and VH_PACKING_ERR_OFFSETS is set in `flag`. */
+#define VH_PROMPT_BLOCK 128
+#define VH_PROMPT_MAX_TOKENS 16777216
+#define VH_PACKING_ERR_OFFSETS 1
+int64_t vh_packing_ints(int64_t tokens);
+int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_t* plan, int32_t* flag, vh_stream_t stream);
+
+/* Causal attention of a packed batch with grouped heads: q [tokens, heads,
+ * dim], k and v [tokens, kv_heads, dim] (bfloat16 or float16; channels dense,
+ * strides in elements; rows 16-byte aligned), heads a multiple of kv_heads,
+ * dim 64, 128 or 256.  Row i of a sequence sees the sequence's rows up to
+ * itself.  o: contiguous; lse [tokens, heads] float32, the logarithm of the sum
+ * of exponentials; rows that pad give 0 and -inf.  o_low (NULL: not wanted):
+ * what the rounding of o left out, in bfloat16, laid out as o.
+ * The backward pass reads q, k, v, o, o_low, lse and the result's gradient go
+ * (strides as above) and writes gq, gk, gv, contiguous, in a fixed order of sums.  work:
+ * vh_prompt_attention_workspace_bytes(desc) bytes, 16-byte aligned. */
+typedef struct vh_prompt_desc {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const int32_t* plan;
+  void* o;
+  void* o_low;
+  float* lse;
+  const void* go;
+  int64_t go_st, go_sh;
+  void *gq, *gk, *gv;
+  int64_t tokens;
+  float scale; /* of the scores, positive */
+  int32_t dtype, heads, kv_heads, dim;
+} vh_prompt_desc;
+int vh_prompt_attention(const vh_prompt_desc* desc, vh_stream_t stream);
+int vh_prompt_attention_backward(const vh_prompt_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
+int64_t vh_prompt_attention_workspace_bytes(const vh_prompt_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif

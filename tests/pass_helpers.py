@@ -121,3 +121,67 @@ def score_tolerances(logits, ref, g=None, h=None, t=None):
         tol.append(HALF[logits.dtype] * ref[4].nan_to_num(0).abs() + size * 1.01 + 70 * U * ref[4].nan_to_num(0).abs()
                    + least(logits.dtype) + 1e-37 * given)
     return tol
+
+
+# ------------------------------------------------------------- attention
+def packed_attention(q, k, v, offsets, scale, go=None):
+    """Causal attention of packed sequences and its gradients for ``go``, one
+    sequence and head at a time, with what their errors may be.
+
+    With dot the largest scale * sum |q| |k| that a row sees, w = its weights:
+
+    * scores: d products summed in float32 and six more roundings; the
+      exponential within 2^-22; sums of n terms: (n + 64) 2^-24;
+    * a weight is rounded once to the values' type for the second product, and
+      goes down to 2^-36 of the largest of its row in float16;
+    * gradients of weights: dP and D are d products each, D of a result that
+      is known to 2^-17 of itself and otherwise as exactly as the output, and they are
+      rounded once, going down to 2^-36 of the largest of their row (key) in float16;
+    * half a step of each result, which has a least size.
+    """
+    n, heads, d = q.shape
+    kv, group = k.shape[1], heads // k.shape[1]
+    f64 = dict(dtype=torch.float64, device=q.device)
+    o, lse = torch.zeros(n, heads, d, **f64), torch.full((n, heads), -math.inf, **f64)
+    to, tlse = torch.zeros_like(o), torch.zeros_like(lse)
+    gq, tq = torch.zeros_like(o), torch.zeros_like(o)
+    gk, gv, tk, tv = (torch.zeros(n, kv, d, **f64) for _ in range(4))
+    half, small = HALF[q.dtype], least(q.dtype)
+    f16 = 2.0**-36 if q.dtype == torch.float16 else 0.0
+    for a, b in zip(offsets, offsets[1:]):
+        m = b - a
+        if m <= 0:
+            continue
+        hidden = torch.ones(m, m, dtype=torch.bool, device=q.device).triu(1)
+        for h in range(heads):
+            g = h // group
+            qq, kk, vv = q[a:b, h].double(), k[a:b, g].double(), v[a:b, g].double()
+            s = (qq @ kk.t() * scale).masked_fill(hidden, -math.inf)
+            p, full = torch.softmax(s, -1), torch.logsumexp(s, -1)
+            dot = (qq.abs() @ kk.abs().t() * scale).masked_fill(hidden, 0).amax(-1, keepdim=True)
+            score = (d + 6) * U * dot + 2.0**-21
+            sums = (m + 64) * U
+            x = p @ vv
+            mag = p @ vv.abs()
+            raw = (half + 2 * score + 2 * sums) * mag + m * f16 * vv.abs().amax()
+            o[a:b, h], to[a:b, h] = x, half * x.abs() * 1.01 + raw + small
+            lse[a:b, h], tlse[a:b, h] = full, score[:, 0] + sums + 2.0**-21 * full.abs()
+            if go is None:
+                continue
+            gg = go[a:b, h].double()
+            rel = score + tlse[a:b, h][:, None]  # of a weight
+            dp, big = gg @ vv.t(), gg.abs() @ vv.abs().t()
+            dd = (gg * x).sum(-1, keepdim=True)
+            td = (gg.abs() * (raw + 2.0**-16 * x.abs())).sum(-1, keepdim=True) + d * U * (gg.abs() * x.abs()).sum(-1, keepdim=True)
+            ds = p * (dp - dd)
+            tds = (p * (rel * (dp - dd).abs() + d * U * big + td)).masked_fill(hidden, 0)
+            row = (half + sums) * ds.abs() + tds
+            gq[a:b, h] = ds @ kk * scale
+            tq[a:b, h] = (row + f16 * ds.abs().amax(-1, keepdim=True).expand(m, m).masked_fill(hidden, 0)) @ kk.abs() * scale
+            gk[a:b, g] += ds.t() @ qq * scale
+            tk[a:b, g] += (row + f16 * ds.abs().amax(0, keepdim=True).expand(m, m).masked_fill(hidden, 0)).t() @ qq.abs() * scale
+            gv[a:b, g] += p.t() @ gg
+            tv[a:b, g] += (p * (half + rel + sums) + f16).masked_fill(hidden, 0).t() @ gg.abs()
+    for t, ref in ((tq, gq), (tk, gk), (tv, gv)):
+        t += half * ref.abs() * 1.01 + heads * U * ref.abs() + small
+    return (o, lse, gq, gk, gv), (to, tlse, tq, tk, tv)

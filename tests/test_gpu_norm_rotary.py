@@ -128,6 +128,14 @@ def test_one_tensor_and_partial_gradients():
     assert torch.equal(torch.autograd.grad((a, b), (qw, kw), (c.gq, c.gk))[1], whole[3])
 
 
+def test_no_second_gradient():
+    c = Case(1, 2, 2, 1, 64)
+    leaves = c.leaves()
+    q, qw, k, kw = leaves
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(c.run(q, k, qw=qw, kw=kw), leaves, (c.gq, c.gk), create_graph=True)
+
+
 def test_gradients_against_differences():
     c = Case(1, 2, 2, 1, 8, rotary_dim=4, dtype=torch.float32)
     leaves = c.leaves()

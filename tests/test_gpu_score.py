@@ -150,6 +150,12 @@ def test_some_gradients_only():
         within(dx, ref[4], score_tolerances(x.detach(), ref, *given)[3], f"gradient of output {which}")
 
 
+def test_no_second_gradient():
+    x = _logits(3, 100, torch.float32).requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(score.token_scores(x, _tokens(3, 100)).logprob.sum(), x, create_graph=True)
+
+
 def test_the_token_among_the_alternatives():
     """The same entry twice: both gradients are added."""
     x = _logits(4, 900, torch.float32)

@@ -10,7 +10,7 @@ import re
 import pytest
 import torch
 
-from voyager_amd import _lib, rotary, score
+from voyager_amd import _lib, prompt, rotary, score
 
 P = 1 << 20
 
@@ -37,6 +37,7 @@ def test_descriptors_are_as_long_as_the_header_says():
     assert _size("vh_rope_desc") == rope
     assert _size("vh_norm_rope_desc") == rope + rotary.NORM.size
     assert _size("vh_score_desc") == score.SCORE.size
+    assert _size("vh_prompt_desc") == prompt.PROMPT.size
 
 
 # ------------------------------------------------------- norms and positions
@@ -187,3 +188,100 @@ def test_score_refuses_tangents():
     with fwAD.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             score.token_scores(fwAD.make_dual(x, x), torch.zeros(2, dtype=torch.int64))
+
+
+# ------------------------------------------------------------- attention
+def _prompt(entry="vh_prompt_attention", work=P, work_bytes=1 << 50, **kw):
+    a = dict(q=P, q_st=256, q_sh=64, k=P, k_st=128, k_sh=64, v=P, v_st=128, v_sh=64, plan=P, o=P, o_low=P, lse=P, go=P,
+             go_st=256, go_sh=64, gq=P, gk=P, gv=P, tokens=100, scale=0.125, dtype=_lib.VH_BF16, heads=4, kv_heads=2, dim=64)
+    a.update(kw)
+    d, lib = prompt.PROMPT.pack(*a.values()), _lib.load()
+    if entry == "vh_prompt_attention":
+        return lib.vh_prompt_attention(d, None)
+    if entry == "vh_prompt_attention_backward":
+        return lib.vh_prompt_attention_backward(d, work, work_bytes, None)
+    return lib.vh_prompt_attention_workspace_bytes(d)
+
+
+BACK = "vh_prompt_attention_backward"
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=_lib.VH_F32), dict(dim=96), dict(dim=0), dict(tokens=-1), dict(tokens=1 << 24), dict(heads=3), dict(heads=0),
+    dict(kv_heads=0), dict(heads=-4), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
+    dict(q_st=1 << 23), dict(k_st=1 << 23), dict(v_st=1 << 40), dict(go_st=1 << 23),
+    dict(tokens=(1 << 24) - 1, heads=1 << 20, kv_heads=1 << 20)])
+def test_prompt_entries_refuse(kw):
+    assert _prompt(**kw) == 1 and _lib.load().vh_last_error().startswith(b"vh_prompt_attention:")
+    assert _prompt(BACK, **kw) == 1 and _lib.load().vh_last_error().startswith(b"vh_prompt_attention_backward:")
+    assert _prompt("bytes", **kw) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(q=0), dict(k=0), dict(v=0), dict(plan=0), dict(o=0), dict(lse=0), dict(q=P + 8), dict(k=P + 2),
+                                dict(v=P + 4), dict(o=P + 8), dict(q_st=260), dict(k_sh=4), dict(v_st=-8)])
+def test_prompt_entries_need_aligned_tensors(kw):
+    assert _prompt(**kw) == 1 and _prompt(BACK, **kw) == 1
+
+
+@pytest.mark.parametrize("kw", [dict(go=0), dict(o_low=0), dict(gq=0), dict(gk=0), dict(gv=0), dict(go=P + 8), dict(go_sh=2),
+                                dict(gk=P + 8), dict(work=None), dict(work=P + 8), dict(work_bytes=16)])
+def test_prompt_backward_needs_its_tensors(kw):
+    assert _prompt(BACK, **kw) == 1
+
+
+def test_prompt_workspace_and_nothing():
+    need = lambda **kw: _prompt("bytes", **kw)
+    assert need(tokens=0) == 0 and 0 < need() < need(tokens=5000) < need(tokens=5000, heads=8)
+    assert need(tokens=1 << 20, heads=8, kv_heads=8) == (1 << 20) * 8 * 8  # more blocks than are cut
+    assert _prompt(tokens=0, q=0) == 0 and _prompt(BACK, tokens=0, q=0, work=None, work_bytes=0) == 0
+
+
+def test_packing_entry_refuses():
+    lib = _lib.load()
+    assert lib.vh_packing_ints(0) == 0 and lib.vh_packing_ints(129) == 2 * (129 + 2)
+    assert lib.vh_packing_ints(-1) == -1 and lib.vh_packing_ints(1 << 24) == -1
+    for args in ((None, 1, 10, P, P), (P, 1, 10, None, P), (P, 1, 10, P, None), (P, -1, 10, P, P), (P, 1, -1, P, P),
+                 (P, 1, 1 << 24, P, P)):
+        assert lib.vh_packing(*args, None) == 1
+
+
+def test_packing_refuses():
+    for bad in (torch.zeros(2, dtype=torch.int32), torch.zeros(2), torch.zeros(2, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="offsets"):
+            prompt.Packing(bad, 4)  # the first: not on the GPU
+
+
+def test_prompt_arguments_refused():
+    class Plan:  # a packing that was made on a GPU
+        tokens, device = 6, torch.device("cpu")
+
+    q, k = torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16)
+    run = prompt.prompt_attention
+    for bad in (q[:5], q[None], q.float(), q[..., :32], torch.zeros(6, 4, 96, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="q must be"):
+            run(bad, k, k, Plan)
+    for bad in (k[:5], k.half(), k[0], torch.zeros(6, 2, 128, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="k must be"):
+            run(q, bad, k, Plan)
+    for bad in (k[:, :1], k.half()):
+        with pytest.raises(ValueError, match="v must be"):
+            run(q, k, bad, Plan)
+    for heads, kv in ((3, 2), (0, 2), (4, 0)):
+        with pytest.raises(ValueError, match="query heads"):
+            run(torch.zeros(6, heads, 64, dtype=torch.bfloat16), *(torch.zeros(6, kv, 64, dtype=torch.bfloat16),) * 2, Plan)
+    with pytest.raises(ValueError, match="cuda"):  # no CPU form
+        run(q, k, k, type("Other", (), dict(tokens=6, device=torch.device("cpu"), plan=torch.zeros(1))))
+    with pytest.raises(ValueError, match="its packing on"):
+        run(q, k, k, type("Other", (), dict(tokens=6, device=torch.device("cuda", 0))))
+
+
+def test_prompt_refuses_tangents():
+    import torch.autograd.forward_ad as fwAD
+
+    class Plan:
+        tokens, device = 6, torch.device("cpu")
+
+    k = torch.zeros(6, 2, 64, dtype=torch.bfloat16)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            prompt.prompt_attention(fwAD.make_dual(k, k), k, k, Plan)

@@ -1,0 +1,185 @@
+// The forward pass of packed causal attention: vh_prompt.h says how.
+#pragma once
+
+#include "vh_prompt.h"
+
+namespace prompt {
+
+constexpr int KEYS = 64;  // of a tile
+constexpr int SUB = 32;   // that a wave takes at a time
+
+// A weight's exponent is its score less a reference that lies under the row's
+// largest score by at most `SLACK`, so that sums are rarely scaled, and moved
+// by `LIFT`: float16 weights then reach down to 2^-35 of the largest, and
+// bfloat16 ones, whose range is float32's, stay so small that neither their sum
+// nor a product with the largest values overflows over 2^24 keys.
+template <bool BF>
+struct Range {
+  static constexpr float SLACK = BF ? 8.0f : 4.0f, LIFT = BF ? -32.0f : 11.0f;
+};
+
+// Adds to 32 channels of a wave's rows what infinite and NaN values of 16 keys
+// give: weights of the keys that hold one in a channel, by products with ones.
+template <bool BF>
+VH_DEV void add_nonfinite(uint4 v, uint4 weights, f32x16& acc) {
+  constexpr uint32_t ONE = BF ? 0x3f80u : 0x3c00u, INFINITE = BF ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int kind = 0; kind < 3; ++kind) {
+    const auto ones = [&](uint32_t w) {
+      uint32_t out = 0u;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t x = (w >> (16 * half)) & 0xffffu;
+        const bool is = kind == 0 ? x == INFINITE : kind == 1 ? x == (INFINITE | 0x8000u) : (x & 0x7fffu) > INFINITE;
+        out |= (is ? ONE : 0u) << (16 * half);
+      }
+      return out;
+    };
+    f32x16 some = {};
+    some = mfma<BF>(make_uint4(ones(v.x), ones(v.y), ones(v.z), ones(v.w)), weights, some);
+    const float what = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] += some[r] > 0.0f ? what : 0.0f;
+  }
+}
+
+template <int D, bool BF, bool CAREFUL>
+struct Forward {
+  f32x16 acc[D / 32];
+  float ref, sum;  // a row's reference, and the half of its sum that is this lane's
+
+  // SUB keys from key0 on, row `at` of the tile.  masked: some are not seen by some rows.
+  __device__ __forceinline__ void step(const uint4 (&q)[D / 16], const char* k, const char* v, int at, int key0, int row, int first, bool masked, float scale) {
+    const int half = (threadIdx.x & 63) >> 5;
+    f32x16 s[SUB / 32];
+#pragma unroll
+    for (int t = 0; t < SUB / 32; ++t) {
+      s[t] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s[t] = mfma<BF>(rows_operand<D>(k, at + 32 * t, i), q[i], s[t]);
+    }
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < SUB / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key0 + 32 * t + result_row(r) + 4 * half;
+          s[t][r] = key >= first && key <= row ? s[t][r] : -__builtin_inff();
+        }
+    }
+    float most = s[0][0];
+#pragma unroll
+    for (int t = 0; t < SUB / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[t][r]);
+    most = max_halves(most) * scale;
+    const bool over = most > ref + Range<BF>::SLACK;
+    if (__any(over)) {
+      const float to = over ? most : ref, by = ref == -__builtin_inff() ? 1.0f : exp2_fast(ref - to);
+      ref = to;
+      sum *= by;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) acc[c] *= by;
+    }
+    const float less = (ref == -__builtin_inff() ? 0.0f : ref) - Range<BF>::LIFT;
+    uint4 p[SUB / 16];
+#pragma unroll
+    for (int t = 0; t < SUB / 32; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], scale, -less));
+        sum += s[t][r];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p[2 * t + i] = make_uint4(pack2<BF>(s[t][8 * i], s[t][8 * i + 1]), pack2<BF>(s[t][8 * i + 2], s[t][8 * i + 3]),
+                                  pack2<BF>(s[t][8 * i + 4], s[t][8 * i + 5]), pack2<BF>(s[t][8 * i + 6], s[t][8 * i + 7]));
+    }
+#pragma unroll
+    for (int i = 0; i < SUB / 16; ++i)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint4 x = turned_operand<D>(v, at + 16 * i, c);
+        if constexpr (CAREFUL) {
+          // what all rows see is as it is
+          acc[c] = mfma<BF>(masked ? finite_part<BF>(x) : x, p[i], acc[c]);
+          if (masked) add_nonfinite<BF>(x, p[i], acc[c]);
+        } else {
+          acc[c] = mfma<BF>(x, p[i], acc[c]);
+        }
+      }
+  }
+};
+
+// A workgroup's rows of one head.  True where a row may have got an infinity
+// or NaN that it does not see.
+template <int D, bool BF, bool CAREFUL>
+VH_DEV bool prompt_block(const Args& a, char* tiles) {
+  constexpr int BYTES = KEYS * D * 2;  // of a tile: two of keys, two of values
+  const int rank = blockIdx.x / a.heads, spread = blockIdx.x - rank * a.heads;
+  // heads of a group lie `kv_heads` workgroups apart: on one die where those are a multiple of 8
+  const int kv = spread % a.kv_heads, head = kv * a.group + spread / a.kv_heads;
+  const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave0 = row0 + 32 * wave, row = wave0 + (lane & 31);
+  const bool in = row < a.tokens;
+  const int first = in ? a.first[row] : row + 1;
+  const int wave_first = __builtin_amdgcn_readlane(first, 0), wave_last_first = __builtin_amdgcn_readlane(first, 31);
+  const int begin = a.first[row0], end = min(row0 + BLOCK, a.tokens);
+  uint4 q[D / 16];
+  load_columns<D>(a.q, head, wave0, a.tokens, q);
+  Loader<D, KEYS> kl, vl;
+  kl.init(a.k, kv);
+  vl.init(a.v, kv);
+  const float scale = a.scale * LOG2E;
+  Forward<D, BF, CAREFUL> f;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) f.acc[c] = f32x16{};
+  f.ref = -__builtin_inff();
+  f.sum = 0.0f;
+  if (begin < end) {
+    kl.load(tiles, begin, a.tokens);
+    vl.load(tiles + 2 * BYTES, begin, a.tokens);
+  }
+  int at = 0;
+  for (int key0 = begin; key0 < end; key0 += KEYS, at ^= 1) {
+    arrived();
+    if (key0 + KEYS < end) {
+      kl.load(tiles + (at ^ 1) * BYTES, key0 + KEYS, a.tokens);
+      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + KEYS, a.tokens);
+    }
+    const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
+#pragma unroll
+    for (int sub = 0; sub < KEYS; sub += SUB) {
+      const int key = key0 + sub;
+      if (key >= wave0 + 32 || key + SUB <= wave_first) continue;
+      f.step(q, k, v, sub, key, row, first, key + SUB > wave0 + 1 || key < wave_last_first, scale);
+    }
+  }
+  f.sum = sum_halves(f.sum);
+  const float by = f.sum == 0.0f ? 0.0f : 1.0f / f.sum;
+  store_columns<D, D, BF>(a.o, a.o_low, a.heads, head, row, in, 0, f.acc, by);
+  if (in && lane < 32)
+    a.lse[(int64_t)row * a.heads + head] = f.sum == 0.0f ? -__builtin_inff() : (f.ref - Range<BF>::LIFT + log2f(f.sum)) * LN2;
+  // a row whose sum is not finite sees something that is not
+  return !CAREFUL && in && f.sum < __builtin_inff() && any_nonfinite(f.acc);
+}
+
+// A masked key's weight is 0, but 0 times an infinity or NaN is not: a block
+// into whose rows such a value may have come is done once more, with these
+// values apart.
+template <int D, bool BF>
+__global__ void __launch_bounds__(THREADS, waves_of(D)) k_prompt(Args a) {
+  __shared__ __attribute__((aligned(16))) char s_tiles[4 * KEYS * D * 2];
+  const bool apart = prompt_block<D, BF, false>(a, s_tiles);
+  if (__syncthreads_or(apart)) prompt_block<D, BF, true>(a, s_tiles);
+}
+
+template <int D>
+int forward(const Args& a, bool bf16, hipStream_t s) {
+  const dim3 grid((unsigned)((a.tokens + BLOCK - 1) / BLOCK * a.heads));
+  if (bf16) hipLaunchKernelGGL((k_prompt<D, true>), grid, dim3(THREADS), 0, s, a);
+  else hipLaunchKernelGGL((k_prompt<D, false>), grid, dim3(THREADS), 0, s, a);
+  return vh::check_launch("vh_prompt_attention");
+}
+
+}  // namespace prompt

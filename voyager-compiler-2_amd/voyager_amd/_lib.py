@@ -206,10 +206,15 @@ _SIGNATURES = {
     "vh_verify": ([_P, _P, _I64, _P], _I32),
     "vh_verify_workspace_bytes": ([_I64, _I64], _I64),
     # a pass over packed sequences: descriptors' bytes as well (rotary.NORM after vh_rope_desc's,
-    # score.SCORE)
+    # prompt.PROMPT, score.SCORE)
     "vh_norm_rope": ([_P, _P], _I32),
     "vh_norm_rope_backward": ([_P, _P, _I64, _P], _I32),
     "vh_norm_rope_workspace_bytes": ([_P], _I64),
+    "vh_packing_ints": ([_I64], _I64),
+    "vh_packing": ([_P, _I64, _I64, _P, _P, _P], _I32),
+    "vh_prompt_attention": ([_P, _P], _I32),
+    "vh_prompt_attention_backward": ([_P, _P, _I64, _P], _I32),
+    "vh_prompt_attention_workspace_bytes": ([_P], _I64),
     "vh_score": ([_P, _P, _I64, _P], _I32),
     "vh_score_backward": ([_P, _P], _I32),
     "vh_score_workspace_bytes": ([_P], _I64),
@@ -287,6 +292,13 @@ def no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
     would drop."""
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{what}: no forward-mode derivative")
+
+
+def once(what: str) -> None:
+    """In a backward pass without a gradient of its own: raise where its graph
+    is wanted (``create_graph``), from which it would be missing."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: differentiable once; its gradient has no graph")
 
 
 def ptr(t: Optional[torch.Tensor]):

@@ -15,9 +15,8 @@ import struct
 from typing import Dict, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, dtype_code, load, no_tangents, ptr, stream_on
+from ._lib import check, dtype_code, load, no_tangents, once, ptr, stream_on
 
 MAX_DIM = 512
 #: ``vh_rope_desc``: up to ``inverse``, which a call gives, and the rest, which the embedding does
@@ -307,8 +306,8 @@ class _NormTurn(torch.autograd.Function):
         return rotary._norm_turn(q, k, q_weight, k_weight, positions, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
+        once("Rotary.normed")
         if gq is None and gk is None:
             return (None,) * 7
         q, k, q_weight, k_weight, positions = ctx.saved_tensors

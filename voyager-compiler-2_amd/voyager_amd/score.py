@@ -12,9 +12,8 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, dtype_code, load, no_tangents, ptr, stream_on
+from ._lib import check, dtype_code, load, no_tangents, once, ptr, stream_on
 
 MAX_TOP = 64
 MAX_VOCAB = 1 << 20
@@ -108,8 +107,8 @@ class _Scores(torch.autograd.Function):
         return logprob, entropy, best, index
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logprob, g_entropy, g_best=None, _=None):
+        once("token_scores")
         if g_logprob is None and g_entropy is None and g_best is None:
             return None, None, None
         x, tokens, entropy, stats, index = ctx.saved_tensors
