@@ -133,7 +133,8 @@ def packed_attention(q, k, v, offsets, scale, go=None):
     * scores: d products summed in float32 and six more roundings; the
       exponential within 2^-22; sums of n terms: (n + 64) 2^-24;
     * a weight is rounded once to the values' type for the second product, and
-      goes down to 2^-36 of the largest of its row in float16;
+      goes down to 2^-36 of the largest of its row in float16; weights p (1 + e)
+      over their own sum give sum p e (v - o) more: |e| times both magnitudes;
     * gradients of weights: dP and D are d products each, D of a result that
       is known to 2^-17 of itself and otherwise as exactly as the output, and they are
       rounded once, going down to 2^-36 of the largest of their row (key) in float16;
@@ -163,7 +164,7 @@ def packed_attention(q, k, v, offsets, scale, go=None):
             sums = (m + 64) * U
             x = p @ vv
             mag = p @ vv.abs()
-            raw = (half + 2 * score + 2 * sums) * mag + m * f16 * vv.abs().amax()
+            raw = (half + 2 * score + 2 * sums) * (mag + x.abs()) + m * f16 * vv.abs().amax()
             o[a:b, h], to[a:b, h] = x, half * x.abs() * 1.01 + raw + small
             lse[a:b, h], tlse[a:b, h] = full, score[:, 0] + sums + 2.0**-21 * full.abs()
             if go is None:

@@ -87,6 +87,12 @@ VH_DEV f32x2 unpack2(uint32_t w) {
   if constexpr (BF) return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
   else return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
 }
+// sum and both halves of w.
+template <bool BF>
+VH_DEV float add_pairs(uint32_t w, float sum) {
+  if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
+}
 template <bool BF>
 VH_DEV f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
   if constexpr (BF)

@@ -46,7 +46,8 @@ VH_DEV void add_nonfinite(uint4 v, uint4 weights, f32x16& acc) {
 template <int D, bool BF, bool CAREFUL>
 struct Forward {
   f32x16 acc[D / 32];
-  float ref, sum;  // a row's reference, and the half of its sum that is this lane's
+  // a row's reference, and of its sum, and of its sum of rounded weights, the half that is this lane's
+  float ref, sum, rounded;
 
   // SUB keys from key0 on, row `at` of the tile.  masked: some are not seen by some rows.
   __device__ __forceinline__ void step(const uint4 (&q)[D / 16], const char* k, const char* v, int at, int key0, int row, int first, bool masked, float scale) {
@@ -78,6 +79,7 @@ struct Forward {
       const float to = over ? most : ref, by = ref == -__builtin_inff() ? 1.0f : exp2_fast(ref - to);
       ref = to;
       sum *= by;
+      rounded *= by;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) acc[c] *= by;
     }
@@ -95,6 +97,8 @@ struct Forward {
         p[2 * t + i] = make_uint4(pack2<BF>(s[t][8 * i], s[t][8 * i + 1]), pack2<BF>(s[t][8 * i + 2], s[t][8 * i + 3]),
                                   pack2<BF>(s[t][8 * i + 4], s[t][8 * i + 5]), pack2<BF>(s[t][8 * i + 6], s[t][8 * i + 7]));
     }
+#pragma unroll
+    for (int i = 0; i < SUB / 16; ++i) rounded = add_pairs<BF>(p[i].x, add_pairs<BF>(p[i].y, add_pairs<BF>(p[i].z, add_pairs<BF>(p[i].w, rounded))));
 #pragma unroll
     for (int i = 0; i < SUB / 16; ++i)
 #pragma unroll
@@ -135,7 +139,7 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) f.acc[c] = f32x16{};
   f.ref = -__builtin_inff();
-  f.sum = 0.0f;
+  f.sum = f.rounded = 0.0f;
   if (begin < end) {
     kl.load(tiles, begin, a.tokens);
     vl.load(tiles + 2 * BYTES, begin, a.tokens);
@@ -156,7 +160,10 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
     }
   }
   f.sum = sum_halves(f.sum);
-  const float by = f.sum == 0.0f ? 0.0f : 1.0f / f.sum;
+  f.rounded = sum_halves(f.rounded);
+  // Divided by the sum of the rounded weights, a row whose weight is one key's has
+  // none of its rounding, in its result as in the gradients' D.
+  const float by = f.rounded == 0.0f ? 0.0f : 1.0f / f.rounded;
   store_columns<D, D, BF>(a.o, a.o_low, a.heads, head, row, in, 0, f.acc, by);
   if (in && lane < 32)
     a.lse[(int64_t)row * a.heads + head] = f.sum == 0.0f ? -__builtin_inff() : (f.ref - Range<BF>::LIFT + log2f(f.sum)) * LN2;
