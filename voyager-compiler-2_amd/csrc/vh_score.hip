@@ -175,9 +175,9 @@ VH_DEV int count_all(int n, int* s_n) {
   return n;
 }
 
-// NV vectors of 16 bytes a thread.
-template <typename T, int NV>
-__global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
+// NV vectors of 16 bytes a thread.  TOP: with alternatives.
+template <typename T, int NV, bool TOP>
+__global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
   constexpr int VEC = 16 / sizeof(T);
   __shared__ float s_f[3][WAVES];
   __shared__ uint32_t s_bound[WAVES];
@@ -200,17 +200,22 @@ __global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
   if (end >= VEC) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = load16<T>(x, first + i * THREADS * VEC, end);
+    const int whole = (end - begin) / (THREADS * VEC);  // rounds of vectors that lie in the row
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = shift16<T>(v[i], first + i * THREADS * VEC, end);
+    for (int i = 0; i < NV; ++i)
+      if (i >= whole) v[i] = shift16<T>(v[i], first + i * THREADS * VEC, end);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = load_short<T>(x, i == 0 && threadIdx.x == 0 ? end : 0);
   }
-  float m = -INF;
+  float m = -INF, most[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    most[i] = entry<T>(v[i], 0);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) m = maximum(m, entry<T>(v[i], j));
+    for (int j = 1; j < VEC; ++j) most[i] = maximum(most[i], entry<T>(v[i], j));
+    m = maximum(m, most[i]);
+  }
   const float lane_most = m;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) m = maximum(m, __shfl_xor(m, d));
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
     s_f[1][wave] = l;
     s_f[2][wave] = e;
   }
-  if (a.top > 0) {
+  if constexpr (TOP) {
     // The top-th largest of the lanes' maxima of a wave: as many of its entries reach that.
     const uint32_t mine = rank_of(lane_most);
     uint32_t bound = 0u;
@@ -266,13 +271,14 @@ __global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
       s_stats = write_row(a, row, token, token < a.vocab ? (float)x[token] : 0.0f, m, l, e);
     }
   }
-  if (a.top == 0) return;
+  if constexpr (!TOP) return;
   // every entry's rank and index, once more
-  const auto each = [&](auto f) {
+  const auto each = [&](float least, auto f) {  // of vectors that reach `least`, or hold a NaN
     int from = first;
     asm volatile("" : "+v"(from));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (most[i] < least) continue;
       const uint4 w = convert_again(v[i]);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
   // Entries that reach the bound; where ties make them too many, the bound is
   // made the top-th largest value itself, and of those at it the first are taken.
   for (int again = 0; again < 2; ++again) {
-    each([&](uint32_t r, uint32_t at) {
+    each(value_of(bound), [&](uint32_t r, uint32_t at) {
       if (r > bound || (r == bound && at <= upto)) {
         const uint32_t n = atomicAdd(&s_count, 1u);  // in any order: they are ranked below
         if (n < CANDIDATES) s_key[n] = key_of(r, at);
@@ -301,17 +307,17 @@ __global__ void __launch_bounds__(THREADS, 4) k_score(Args a) {
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t t = bound | 1u << bit;
       int n = 0;
-      each([&](uint32_t r, uint32_t) { n += r >= t; });
+      each(-INF, [&](uint32_t r, uint32_t) { n += r >= t; });
       if (count_all(n, s_n) >= a.top) bound = t;
     }
     int above = 0;
-    each([&](uint32_t r, uint32_t) { above += r > bound; });
+    each(-INF, [&](uint32_t r, uint32_t) { above += r > bound; });
     const int need = a.top - count_all(above, s_n);
     upto = 0u;  // the largest index that fewer than `need` ties come before
     for (int bit = 30; bit >= 0; --bit) {
       const uint32_t t = upto | 1u << bit;
       int n = 0;
-      each([&](uint32_t r, uint32_t at) { n += r == bound && at < t; });
+      each(-INF, [&](uint32_t r, uint32_t at) { n += r == bound && at < t; });
       if (count_all(n, s_n) < need) upto = t;
     }
     upto = min(upto, (uint32_t)end - 1u);
@@ -513,13 +519,18 @@ Args args_of(const vh_score_desc* d) {
   return a;
 }
 
+template <typename T, int NV>
+void launch_of(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.rows * a.pieces));
+  if (a.top > 0) hipLaunchKernelGGL((k_score<T, NV, true>), grid, dim3(THREADS), 0, s, a);
+  else hipLaunchKernelGGL((k_score<T, NV, false>), grid, dim3(THREADS), 0, s, a);
+}
 template <typename T>
 void launch(const Args& a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * a.pieces));
-  if (p.nv == 1) hipLaunchKernelGGL((k_score<T, 1>), grid, dim3(THREADS), 0, s, a);
-  else if (p.nv == 2) hipLaunchKernelGGL((k_score<T, 2>), grid, dim3(THREADS), 0, s, a);
-  else if (p.nv == 4) hipLaunchKernelGGL((k_score<T, 4>), grid, dim3(THREADS), 0, s, a);
-  else hipLaunchKernelGGL((k_score<T, 8>), grid, dim3(THREADS), 0, s, a);
+  if (p.nv == 1) launch_of<T, 1>(a, s);
+  else if (p.nv == 2) launch_of<T, 2>(a, s);
+  else if (p.nv == 4) launch_of<T, 4>(a, s);
+  else launch_of<T, 8>(a, s);
   if (a.pieces > 1) hipLaunchKernelGGL((k_score_join<T>), dim3((unsigned)a.rows), dim3(JOIN_THREADS), 0, s, a);
 }
 
