@@ -96,7 +96,7 @@ int check(const vh_prompt_desc* d, const char* what) {
   VH_REQUIRE(d->dim == 64 || d->dim == 128 || d->dim == 256, "%s: heads of 64, 128 or 256 (got %d)", what, d->dim);
   VH_REQUIRE(d->tokens >= 0 && d->tokens < VH_PROMPT_MAX_TOKENS, "%s: at most %d tokens", what, VH_PROMPT_MAX_TOKENS - 1);
   VH_REQUIRE(d->kv_heads > 0 && d->heads > 0 && d->heads % d->kv_heads == 0, "%s: query heads must be a multiple of the keys'", what);
-  VH_REQUIRE((blocks_of(d->tokens) + 1) * d->heads < (1ll << 31) && d->tokens * d->heads * (d->dim / 8) < (1ll << 39),
+  VH_REQUIRE((blocks_of(d->tokens) + 1) * d->heads < (1ll << 30),
              "%s: too many heads", what);
   VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
   VH_REQUIRE(d->q_st < MOST_STRIDE && d->k_st < MOST_STRIDE && d->v_st < MOST_STRIDE && d->go_st < MOST_STRIDE,

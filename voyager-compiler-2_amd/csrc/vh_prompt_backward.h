@@ -1,7 +1,7 @@
 // The backward pass of packed causal attention: vh_prompt.h says how.
 //
-// Three kernels: D_i of every row; a pass over blocks of rows for dq, and one
-// over blocks of keys for dk and dv.  Scores and dP are formed in both: five
+// A pass over blocks of rows, which finds D_i and gives dq, and one over blocks
+// of keys for dk and dv.  Scores and dP are formed in both: five
 // products become seven, but every sum has one owner and one order, and
 // nothing is added up in memory.
 #pragma once
@@ -38,9 +38,10 @@ VH_DEV int sum_before(int x, int* s_sum, int& all) {  // over the workgroup's th
   }
   return before + upto - x;
 }
-VH_DEV void prompt_items(const Args& a, int group, int groups) {
-  __shared__ int s_tiles[MOST_CUT], s_sum[WAVES];
-  __shared__ uint16_t s_pieces[MOST_CUT];
+constexpr int ITEM_BYTES = MOST_CUT * 6 + 16;  // of LDS
+VH_DEV void prompt_items(const Args& a, int group, int groups, char* lds) {
+  int *s_sum = (int*)lds, *s_tiles = s_sum + WAVES;
+  uint16_t* s_pieces = (uint16_t*)(s_tiles + MOST_CUT);
   const int blocks = (a.tokens + BLOCK - 1) / BLOCK;
   int sum = 0, all;
   for (int b = threadIdx.x; b < blocks; b += THREADS) {
@@ -84,39 +85,6 @@ VH_DEV void prompt_items(const Args& a, int group, int groups) {
     for (int i = all + threadIdx.x; i < a.item_count; i += THREADS) a.items[i] = make_int4(-1, 0, 0, -1);
 }
 
-// D_i = do_i . o_i, beside lse_i log2(e), which is inf where a row sees
-// nothing, so that its weights are 0.  D / 8 lanes a row and head.
-template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS) k_prompt_rows(Args a, int item_groups) {
-  constexpr int LANES = D / 8;
-  if ((int)blockIdx.x < item_groups) {
-    prompt_items(a, blockIdx.x, item_groups);
-    return;
-  }
-  const int64_t id = ((int64_t)(blockIdx.x - item_groups) * THREADS + threadIdx.x) / LANES;
-  const int64_t all = (int64_t)a.tokens * a.heads;
-  const int64_t at = id < all ? id : all - 1;
-  const int row = (int)(at / a.heads), head = (int)(at - (int64_t)row * a.heads), c = threadIdx.x % LANES * 8;
-  const uint4 x = *(const uint4*)((const uint16_t*)a.o + at * D + c), z = *(const uint4*)((const uint16_t*)a.o_low + at * D + c);
-  const uint4 y = *(const uint4*)((const uint16_t*)a.go.p + row * a.go.st + head * a.go.sh + c);
-  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2 u = unpack2<BF>(xs[i]), v = unpack2<BF>(ys[i]), w = unpack2<true>(zs[i]);
-    sum = __builtin_fmaf(u[0] + w[0], v[0], sum);
-    sum = __builtin_fmaf(u[1] + w[1], v[1], sum);
-  }
-#pragma unroll
-  for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d);
-  if (c == 0 && id < all) {
-    const float lse = a.lse[at];
-    float* to = a.rows + (int64_t)head * 2 * a.tokens + row;
-    to[0] = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
-    to[a.tokens] = sum;
-  }
-}
-
 // Sixteen weights, or their gradients, rounded: the operand of two products.
 template <bool BF>
 VH_DEV void pack16(const f32x16& s, uint4 (&p)[2]) {
@@ -157,9 +125,9 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
 constexpr int DQ_KEYS = 64;  // of a tile; a wave takes 32 at a time
 
 template <int D, bool BF, bool CAREFUL>
-VH_DEV bool prompt_dq_block(const Args& a, char* tiles) {
+VH_DEV bool prompt_dq_block(const Args& a, int id, char* tiles) {
   constexpr int BYTES = DQ_KEYS * D * 2;
-  const int rank = blockIdx.x / a.heads, spread = blockIdx.x - rank * a.heads;
+  const int rank = id / a.heads, spread = id - rank * a.heads;
   const int kv = spread % a.kv_heads, head = kv * a.group + spread / a.kv_heads;
   const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wave0 = row0 + 32 * wave, row = wave0 + (lane & 31), half = lane >> 5;
@@ -167,11 +135,37 @@ VH_DEV bool prompt_dq_block(const Args& a, char* tiles) {
   const int first = in ? a.first[row] : row + 1;
   const int wave_first = __builtin_amdgcn_readlane(first, 0), wave_last_first = __builtin_amdgcn_readlane(first, 31);
   const int begin = a.first[row0], end = min(row0 + BLOCK, a.tokens);
-  const float* rows = a.rows + (int64_t)head * 2 * a.tokens + min(row, a.tokens - 1);
-  const float lse = rows[0], dot = rows[a.tokens];
   uint4 q[D / 16], go[D / 16];
   load_columns<D>(a.q, head, wave0, a.tokens, q);
   load_columns<D>(a.go, head, wave0, a.tokens, go);
+  // D, and lse log2(e), which is inf where a row sees nothing, so that its weights are 0: for the keys' pass as well
+  const float natural = in ? a.lse[(int64_t)row * a.heads + head] : -__builtin_inff();
+  const float lse = natural == -__builtin_inff() ? __builtin_inff() : natural * LOG2E;
+  float dot = 0.0f;
+  {
+    uint4 o[D / 16];
+    const Tensor out{a.o, (int64_t)a.heads * D, D}, low{a.o_low, (int64_t)a.heads * D, D};
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      load_columns<D>(part == 0 ? out : low, head, wave0, a.tokens, o);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const uint32_t xs[4] = {o[s].x, o[s].y, o[s].z, o[s].w}, ys[4] = {go[s].x, go[s].y, go[s].z, go[s].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 u = part == 0 ? unpack2<BF>(xs[i]) : unpack2<true>(xs[i]), v = unpack2<BF>(ys[i]);
+          dot = __builtin_fmaf(u[0], v[0], dot);
+          dot = __builtin_fmaf(u[1], v[1], dot);
+        }
+      }
+    }
+    dot = sum_halves(dot);
+  }
+  if (in) {
+    float* to = a.rows + (int64_t)head * 2 * a.tokens + row;
+    if (half == 0) to[0] = lse;
+    else to[a.tokens] = dot;
+  }
   Loader<D, DQ_KEYS> kl, vl;
   kl.init(a.k, kv);
   vl.init(a.v, kv);
@@ -232,10 +226,16 @@ VH_DEV bool prompt_dq_block(const Args& a, char* tiles) {
 }
 
 template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dq(Args a) {
+__global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dq(Args a, int item_groups) {
   __shared__ __attribute__((aligned(16))) char s_tiles[4 * DQ_KEYS * D * 2];
-  const bool apart = prompt_dq_block<D, BF, false>(a, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, true>(a, s_tiles);
+  static_assert(sizeof(s_tiles) >= ITEM_BYTES, "the items' lists");
+  const int id = (int)blockIdx.x - item_groups;
+  if (id < 0) {
+    prompt_items(a, blockIdx.x, item_groups, s_tiles);
+    return;
+  }
+  const bool apart = prompt_dq_block<D, BF, false>(a, id, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, true>(a, id, s_tiles);
 }
 
 // ------------------------------------------------------------- dk and dv
@@ -426,10 +426,8 @@ template <int D, bool BF>
 void backward_of(Args a, const int32_t* q_order, const int32_t* k_order, hipStream_t s) {
   constexpr int C = key_channels_of(D);
   const unsigned blocks = (unsigned)((a.tokens + BLOCK - 1) / BLOCK), groups = a.items ? (blocks + 63) / 64 : 0;
-  const int64_t threads = (int64_t)a.tokens * a.heads * (D / 8);
-  hipLaunchKernelGGL((k_prompt_rows<D, BF>), dim3((unsigned)((threads + THREADS - 1) / THREADS) + groups), dim3(THREADS), 0, s, a, (int)groups);
   a.order = q_order;
-  hipLaunchKernelGGL((k_prompt_dq<D, BF>), dim3(blocks * a.heads), dim3(THREADS), 0, s, a);
+  hipLaunchKernelGGL((k_prompt_dq<D, BF>), dim3(blocks * a.heads + groups), dim3(THREADS), 0, s, a, (int)groups);
   a.order = k_order;
   hipLaunchKernelGGL((k_prompt_dk<D, C, BF>), dim3((a.items ? a.item_count : blocks) * a.kv_heads * (D / C)), dim3(THREADS), 0, s, a);
   if (a.items) hipLaunchKernelGGL((k_prompt_join<D, BF>), dim3(blocks * a.kv_heads, 2 * BLOCK * D / 4 / THREADS), dim3(THREADS), 0, s, a);
