@@ -6,7 +6,10 @@
 namespace prompt {
 
 constexpr int KEYS = 64;  // of a tile
-constexpr int SUB = 32;   // that a wave takes at a time
+// Keys that a wave takes at a time: 64 where the registers hold their scores
+// beside four waves of a SIMD, or fewer waves share one (a prompt of 4096, 32 + 8
+// heads of 128: 173 us by 32, 165 by 64; 64 prompts, 16 heads of 64: 21 and 23).
+constexpr int sub_of(int d) { return d == 64 ? 32 : 64; }
 
 // A weight's exponent is its score less a reference that lies under the row's
 // largest score by at most `SLACK`, so that sums are rarely scaled, and moved
@@ -45,6 +48,7 @@ VH_DEV void add_nonfinite(uint4 v, uint4 weights, f32x16& acc) {
 
 template <int D, bool BF, bool CAREFUL>
 struct Forward {
+  static constexpr int SUB = sub_of(D);
   f32x16 acc[D / 32];
   // a row's reference, and of its sum, and of its sum of rounded weights, the half that is this lane's
   float ref, sum, rounded;
@@ -85,13 +89,16 @@ struct Forward {
     }
     const float less = (ref == -__builtin_inff() ? 0.0f : ref) - Range<BF>::LIFT;
     uint4 p[SUB / 16];
+    float part[SUB / 32][4];
 #pragma unroll
     for (int t = 0; t < SUB / 32; ++t) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], scale, -less));
-        sum += s[t][r];
+        if (r < 4) part[t][r] = s[t][r];
+        else part[t][r & 3] += s[t][r];  // four sums, so that one addition does not wait for the one before
       }
+      sum += (part[t][0] + part[t][1]) + (part[t][2] + part[t][3]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         p[2 * t + i] = make_uint4(pack2<BF>(s[t][8 * i], s[t][8 * i + 1]), pack2<BF>(s[t][8 * i + 2], s[t][8 * i + 3]),
@@ -153,7 +160,8 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
     }
     const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
 #pragma unroll
-    for (int sub = 0; sub < KEYS; sub += SUB) {
+    for (int sub = 0; sub < KEYS; sub += sub_of(D)) {
+      constexpr int SUB = sub_of(D);
       const int key = key0 + sub;
       if (key >= wave0 + 32 || key + SUB <= wave_first) continue;
       f.step(q, k, v, sub, key, row, first, key + SUB > wave0 + 1 || key < wave_last_first, scale);
