@@ -896,9 +896,10 @@ int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_
  * dim], k and v [tokens, kv_heads, dim] (bfloat16 or float16; channels dense,
  * strides in elements; rows 16-byte aligned), heads a multiple of kv_heads,
  * dim 64, 128 or 256.  Row i of a sequence sees the sequence's rows up to
- * itself.  o: contiguous; lse [tokens, heads] float32, the logarithm of the sum
- * of exponentials; rows that pad give 0 and -inf.  o_low (NULL: not wanted):
- * what the rounding of o left out, in bfloat16, laid out as o.
+ * itself.  sequences: of the plan, by whose number the launch is shaped.  o:
+ * contiguous; lse [tokens, heads] float32, the logarithm of the sum of
+ * exponentials; rows that pad give 0 and -inf.  o_low (NULL: not wanted): what
+ * the rounding of o left out, in bfloat16, laid out as o.
  * The backward pass reads q, k, v, o, o_low, lse and the result's gradient go
  * (strides as above) and writes gq, gk, gv, contiguous, in a fixed order of sums.  work:
  * vh_prompt_attention_workspace_bytes(desc) bytes, 16-byte aligned. */
@@ -918,7 +919,7 @@ typedef struct vh_prompt_desc {
   void *gq, *gk, *gv;
   int64_t tokens;
   float scale; /* of the scores, positive */
-  int32_t dtype, heads, kv_heads, dim;
+  int32_t dtype, heads, kv_heads, dim, sequences;
 } vh_prompt_desc;
 int vh_prompt_attention(const vh_prompt_desc* desc, vh_stream_t stream);
 int vh_prompt_attention_backward(const vh_prompt_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);

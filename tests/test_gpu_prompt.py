@@ -124,15 +124,16 @@ def test_a_gradient_of_one_value_for_all():
 
 @pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 128), (BF16, 64), (F16, 256)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_what_is_not_seen_has_no_part(dtype, d, bad):
+@pytest.mark.parametrize("lengths", [(70, 41, 90), (600, 41, 900)])  # the second: by two halves of a workgroup
+def test_what_is_not_seen_has_no_part(dtype, d, bad, lengths):
     """Infinities and NaN in a sequence's last row, in the rows that pad and
     in q, k, v and the result's gradient there: earlier rows and other sequences are as
     they were, bit for bit, and so are the keys that these rows do not see."""
-    c = Case([70, 41, 90], 4, 2, d, dtype, 20)
+    c = Case(lengths, 4, 2, d, dtype, 20)
     want = c.check()
-    n = c.offsets[-1]
+    n, third = c.offsets[-1], c.offsets[2]
     for what in ("q", "k", "v", "go"):
-        for rows in ([110], [200], list(range(n, n + 20)), [30, 150]):
+        for rows in ([third - 1], [n - 1], list(range(n, n + 20)), [30, third + 39]):
             t = {x: getattr(c, x).clone() for x in ("q", "k", "v", "go")}
             for r in rows:
                 t[what][r, 1, 5] = bad
@@ -162,23 +163,25 @@ def test_what_is_not_seen_has_no_part(dtype, d, bad):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("d", [64, 128, 256])
-def test_an_infinite_value_gives_its_channel_an_infinity(dtype, d):
-    c = Case([150], 2, 1, d, dtype)
+@pytest.mark.parametrize("pad", [0, 600])  # rows enough for two halves of a workgroup
+def test_an_infinite_value_gives_its_channel_an_infinity(dtype, d, pad):
+    c = Case([150], 2, 1, d, dtype, pad)
     clean = c.run()[0]
     v = c.v.clone()
     v[100, 0, 7], v[140, 0, 9] = math.inf, -math.inf
     o = c.run(v=v)[0]
-    assert bool((o[100:, :, 7] == math.inf).all()) and bool((o[140:, :, 9] == -math.inf).all())
-    o[100:, :, 7], o[140:, :, 9] = clean[100:, :, 7], clean[140:, :, 9]
+    assert bool((o[100:150, :, 7] == math.inf).all()) and bool((o[140:150, :, 9] == -math.inf).all())
+    o[100:150, :, 7], o[140:150, :, 9] = clean[100:150, :, 7], clean[140:150, :, 9]
     assert torch.equal(o, clean)
     v[120, 0, 7] = -math.inf
     o = c.run(v=v)[0]
-    assert bool((o[100:120, :, 7] == math.inf).all()) and bool(torch.isnan(o[120:, :, 7]).all())
+    assert bool((o[100:120, :, 7] == math.inf).all()) and bool(torch.isnan(o[120:150, :, 7]).all())
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_the_largest_values_give_finite_results(dtype):
-    c = Case([300, 40], 2, 1, 128, dtype)
+@pytest.mark.parametrize("lengths", [(300, 40), (1000, 40)])
+def test_the_largest_values_give_finite_results(dtype, lengths):
+    c = Case(lengths, 2, 1, 128, dtype)
     most = torch.finfo(dtype).max
     c.v = torch.where(c.v > 0, most, -most).to(dtype)
     c.check(which=slice(0, 2))
@@ -187,11 +190,12 @@ def test_the_largest_values_give_finite_results(dtype):
     assert bool((o == most).all())
 
 
+@pytest.mark.parametrize("length", [500, 1100])  # the second: by two halves of a workgroup
 @pytest.mark.parametrize("size", [2.0**-14, 2.0**10])
-def test_small_and_large_gradients_in_float16(size):
+def test_small_and_large_gradients_in_float16(size, length):
     """Gradients of weights that float16 could not hold as they come: under its
     least value, or, where values are large as well, over its largest."""
-    c = Case([500, 30], 2, 1, 64, F16)
+    c = Case([length, 30], 2, 1, 64, F16)
     c.go = (c.go * 0 + 1) * torch.randn(c.go.shape, generator=torch.Generator().manual_seed(1)).cuda() * size
     c.go = c.go.to(F16)
     if size > 1:

@@ -193,7 +193,7 @@ def test_score_refuses_tangents():
 # ------------------------------------------------------------- attention
 def _prompt(entry="vh_prompt_attention", work=P, work_bytes=1 << 50, **kw):
     a = dict(q=P, q_st=256, q_sh=64, k=P, k_st=128, k_sh=64, v=P, v_st=128, v_sh=64, plan=P, o=P, o_low=P, lse=P, go=P,
-             go_st=256, go_sh=64, gq=P, gk=P, gv=P, tokens=100, scale=0.125, dtype=_lib.VH_BF16, heads=4, kv_heads=2, dim=64)
+             go_st=256, go_sh=64, gq=P, gk=P, gv=P, tokens=100, scale=0.125, dtype=_lib.VH_BF16, heads=4, kv_heads=2, dim=64, sequences=1)
     a.update(kw)
     d, lib = prompt.PROMPT.pack(*a.values()), _lib.load()
     if entry == "vh_prompt_attention":
@@ -208,7 +208,7 @@ BACK = "vh_prompt_attention_backward"
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=_lib.VH_F32), dict(dim=96), dict(dim=0), dict(tokens=-1), dict(tokens=1 << 24), dict(heads=3), dict(heads=0),
-    dict(kv_heads=0), dict(heads=-4), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
+    dict(kv_heads=0), dict(heads=-4), dict(sequences=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
     dict(q_st=1 << 23), dict(k_st=1 << 23), dict(v_st=1 << 40), dict(go_st=1 << 23),
     dict(tokens=(1 << 24) - 1, heads=1 << 20, kv_heads=1 << 20)])
 def test_prompt_entries_refuse(kw):
@@ -253,7 +253,7 @@ def test_packing_refuses():
 
 def test_prompt_arguments_refused():
     class Plan:  # a packing that was made on a GPU
-        tokens, device = 6, torch.device("cpu")
+        tokens, sequences, device = 6, 1, torch.device("cpu")
 
     q, k = torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16)
     run = prompt.prompt_attention
@@ -270,7 +270,7 @@ def test_prompt_arguments_refused():
         with pytest.raises(ValueError, match="query heads"):
             run(torch.zeros(6, heads, 64, dtype=torch.bfloat16), *(torch.zeros(6, kv, 64, dtype=torch.bfloat16),) * 2, Plan)
     with pytest.raises(ValueError, match="cuda"):  # no CPU form
-        run(q, k, k, type("Other", (), dict(tokens=6, device=torch.device("cpu"), plan=torch.zeros(1))))
+        run(q, k, k, type("Other", (), dict(tokens=6, sequences=1, device=torch.device("cpu"), plan=torch.zeros(1))))
     with pytest.raises(ValueError, match="its packing on"):
         run(q, k, k, type("Other", (), dict(tokens=6, device=torch.device("cuda", 0))))
 
@@ -279,7 +279,7 @@ def test_prompt_refuses_tangents():
     import torch.autograd.forward_ad as fwAD
 
     class Plan:
-        tokens, device = 6, torch.device("cpu")
+        tokens, sequences, device = 6, 1, torch.device("cpu")
 
     k = torch.zeros(6, 2, 64, dtype=torch.bfloat16)
     with fwAD.dual_level():

@@ -45,7 +45,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int THREADS = 256, WAVES = 4;
+constexpr int THREADS = 256, WAVES = 4;  // that share a tile
 constexpr int BLOCK = VH_PROMPT_BLOCK;  // rows of a workgroup, 32 a wave
 // Waves of a SIMD that the registers are held to, forward and back.
 constexpr int waves_of(int d) { return d == 64 ? 4 : d == 128 ? 2 : 1; }
@@ -72,8 +72,21 @@ struct Args {
   float* part;        // [slots, kv_heads, dk and dv, 128 keys, dim]
   int item_count, share;
   float scale;
-  int tokens, heads, kv_heads, group;
+  int tokens, sequences, heads, kv_heads, group;
 };
+
+// Where blocks are few for the card, or one is long beside them, two halves of
+// a workgroup take a block's tiles in turn, and join through LDS: the longest
+// block takes half the time.
+template <int D, int HALVES>
+struct Halves {
+  static constexpr int WIDTH = HALVES * THREADS;
+  __device__ __forceinline__ static int half() { return HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / THREADS); }
+};
+// One register of every lane of a wave, beside those of its other registers.
+VH_DEV float* lane_slot(char* lds, int n) {
+  return (float*)lds + (threadIdx.x % THREADS / 64 * n) * 64 + (threadIdx.x & 63);
+}
 
 // The element type's conversions and products.
 template <bool BF>
@@ -164,7 +177,8 @@ VH_DEV uint4 turned_operand(const char* tile, int row0, int c) {
 
 // Loads ROWS rows of a tensor's head from row0 on into a tile, straight to
 // LDS; rows past `rows` are zero.  Every thread of the workgroup calls it, and
-// waits (`arrived`) before it reads.  The load is written out, as the compiler
+// waits (`arrived`) before it reads (of a workgroup of two halves, every thread
+// of a half).  The load is written out, as the compiler
 // would wait for it before any read of LDS; it has no register for a result.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 VH_DEV i32x4 buffer_of(const char* p, int bytes) {
@@ -195,19 +209,22 @@ struct Loader {
   int offset[TURNS];                                          // of a thread's pieces, in bytes
   const char* base;
   int64_t step;  // bytes of a row
+  uint32_t wave_at;  // of a wave's pieces in a tile, in bytes
   __device__ __forceinline__ void init(const Tensor& t, int head) {
+    const int thread = threadIdx.x % THREADS;
+    wave_at = (uint32_t)__builtin_amdgcn_readfirstlane(thread / 64 * 1024);
     base = (const char*)t.p + head * t.sh * 2;
     step = t.st * 2;
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-      const int row = i * APART + threadIdx.x / Tile<D>::PIECES;
-      offset[i] = row * (int)step + (((threadIdx.x % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 16);
+      const int row = i * APART + thread / Tile<D>::PIECES;
+      offset[i] = row * (int)step + (((thread % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 16);
     }
   }
   __device__ __forceinline__ void load(const char* tile, int row0, int rows) const {
     const int n = rows - row0 < ROWS ? rows - row0 : ROWS;  // that there are
     const i32x4 r = buffer_of(base + row0 * step, n > 0 ? (int)((n - 1) * step) + D * 2 : 0);
-    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_address(tile) + (threadIdx.x >> 6) * 1024));
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(tile)) + wave_at;
     int apart = (int)step * (APART * TURNS);
     asm volatile("" : "+s"(apart));  // sums are formed here, not kept
 #pragma unroll
@@ -278,6 +295,16 @@ VH_DEV uint32_t bad_rows(const char* tile, int row0) {
   }
   const uint64_t all = __ballot(bad != 0u);
   return (uint32_t)all | (uint32_t)(all >> 32);
+}
+
+// Whether two halves of a workgroup share a block: where one wave of workgroups
+// holds all blocks, so that the longest is the pass, and sequences are long.
+// (us by one and by two, 16 + 4 heads: a prompt of 6000, heads of 64, 150 and 111,
+// of 3000, heads of 128, 85 and 64; four of 775 44 and 36; 16 of 250 22 and 27.
+// 32 + 8 heads of 128, 4096: 164 and 176.)
+inline bool in_halves(const Args& a, int waves) {
+  const int64_t blocks = (a.tokens + BLOCK - 1) / BLOCK;
+  return blocks * a.heads <= 256 * waves && a.tokens >= 512ll * a.sequences;
 }
 
 template <int D>

@@ -98,6 +98,7 @@ int check(const vh_prompt_desc* d, const char* what) {
   VH_REQUIRE(d->kv_heads > 0 && d->heads > 0 && d->heads % d->kv_heads == 0, "%s: query heads must be a multiple of the keys'", what);
   VH_REQUIRE((blocks_of(d->tokens) + 1) * d->heads < (1ll << 30),
              "%s: too many heads", what);
+  VH_REQUIRE(d->sequences >= 0, "%s: negative size", what);
   VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
   VH_REQUIRE(d->q_st < MOST_STRIDE && d->k_st < MOST_STRIDE && d->v_st < MOST_STRIDE && d->go_st < MOST_STRIDE,
              "%s: tokens lie too far apart", what);
@@ -129,6 +130,7 @@ Args args_of(const vh_prompt_desc* d) {
   a.lse = d->lse;
   a.scale = d->scale;
   a.tokens = (int)d->tokens;
+  a.sequences = d->sequences;
   a.heads = d->heads;
   a.kv_heads = d->kv_heads;
   a.group = d->heads / d->kv_heads;

@@ -18,7 +18,7 @@ constexpr int LEAST = 2 * BLOCK / DK_ROWS;       // tiles of an item at least, b
 // to be done in one go, or what a block has left.  The largest come first, of
 // equal ones the first: an item's place is the number of those before it.
 // `groups` workgroups share the blocks.
-VH_DEV int sum_before(int x, int* s_sum, int& all) {  // over the workgroup's threads
+VH_DEV int sum_before(int x, int* s_sum, int& all) {  // over the first THREADS
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int upto = x;
 #pragma unroll
@@ -27,7 +27,7 @@ VH_DEV int sum_before(int x, int* s_sum, int& all) {  // over the workgroup's th
     upto += lane >= d ? y : 0;
   }
   __syncthreads();
-  if (lane == 63) s_sum[wave] = upto;
+  if (lane == 63 && wave < WAVES) s_sum[wave] = upto;
   __syncthreads();
   int before = 0;
   all = 0;
@@ -40,21 +40,22 @@ VH_DEV int sum_before(int x, int* s_sum, int& all) {  // over the workgroup's th
 }
 constexpr int ITEM_BYTES = MOST_CUT * 6 + 16;  // of LDS
 VH_DEV void prompt_items(const Args& a, int group, int groups, char* lds) {
+  const int thread = threadIdx.x < THREADS ? threadIdx.x : MOST_CUT;  // a second half has no block
   int *s_sum = (int*)lds, *s_tiles = s_sum + WAVES;
   uint16_t* s_pieces = (uint16_t*)(s_tiles + MOST_CUT);
   const int blocks = (a.tokens + BLOCK - 1) / BLOCK;
   int sum = 0, all;
-  for (int b = threadIdx.x; b < blocks; b += THREADS) {
+  for (int b = thread; b < blocks; b += THREADS) {
     const int key0 = b * BLOCK;
     s_tiles[b] = (max(a.past[min(key0 + BLOCK, a.tokens) - 1] - key0, 0) + DK_ROWS - 1) / DK_ROWS;
     sum += s_tiles[b];
   }
   sum_before(sum, s_sum, all);
   const int size = max((all + a.share - 1) / a.share, LEAST);
-  for (int b = threadIdx.x; b < blocks; b += THREADS) s_pieces[b] = (uint16_t)max((s_tiles[b] + size - 1) / size, 1);
+  for (int b = thread; b < blocks; b += THREADS) s_pieces[b] = (uint16_t)max((s_tiles[b] + size - 1) / size, 1);
   __syncthreads();
   // a thread has consecutive blocks: the slots before them
-  const int each = (blocks + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * each, blocks), b1 = min(b0 + each, blocks);
+  const int each = (blocks + THREADS - 1) / THREADS, b0 = min(thread * each, blocks), b1 = min(b0 + each, blocks);
   int items = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
     items += s_pieces[b];
@@ -82,7 +83,7 @@ VH_DEV void prompt_items(const Args& a, int group, int groups, char* lds) {
     }
   }
   if (group == 0)
-    for (int i = all + threadIdx.x; i < a.item_count; i += THREADS) a.items[i] = make_int4(-1, 0, 0, -1);
+    for (int i = all + (int)threadIdx.x; i < a.item_count; i += blockDim.x) a.items[i] = make_int4(-1, 0, 0, -1);
 }
 
 // Sixteen weights, or their gradients, rounded: the operand of two products.
@@ -124,12 +125,14 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
 // ------------------------------------------------------------------ dq
 constexpr int DQ_KEYS = 64;  // of a tile; a wave takes 32 at a time
 
-template <int D, bool BF, bool CAREFUL>
-VH_DEV bool prompt_dq_block(const Args& a, int id, char* tiles) {
+template <int D, bool BF, int HALVES, bool CAREFUL>
+VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   constexpr int BYTES = DQ_KEYS * D * 2;
+  const int turn = Halves<D, HALVES>::half();
+  char* tiles = lds + turn * 4 * BYTES;
   const int rank = id / a.heads, spread = id - rank * a.heads;
   const int kv = spread % a.kv_heads, head = kv * a.group + spread / a.kv_heads;
-  const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x % THREADS / 64), lane = threadIdx.x & 63;
   const int wave0 = row0 + 32 * wave, row = wave0 + (lane & 31), half = lane >> 5;
   const bool in = row < a.tokens;
   const int first = in ? a.first[row] : row + 1;
@@ -161,7 +164,7 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* tiles) {
     }
     dot = sum_halves(dot);
   }
-  if (in) {
+  if (in && turn == 0) {
     float* to = a.rows + (int64_t)head * 2 * a.tokens + row;
     if (half == 0) to[0] = lse;
     else to[a.tokens] = dot;
@@ -174,17 +177,19 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* tiles) {
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) acc[c] = f32x16{};
   float up = Lift<BF>::FIRST;
-  if (begin < end) {
-    kl.load(tiles, begin, a.tokens);
-    vl.load(tiles + 2 * BYTES, begin, a.tokens);
+  const int first_key = begin + turn * DQ_KEYS;
+  if (first_key < end) {
+    kl.load(tiles, first_key, a.tokens);
+    vl.load(tiles + 2 * BYTES, first_key, a.tokens);
   }
   int at = 0;
-  for (int key0 = begin; key0 < end; key0 += DQ_KEYS, at ^= 1) {
+  for (int key0 = first_key; key0 - turn * DQ_KEYS < end; key0 += HALVES * DQ_KEYS, at ^= 1) {
     arrived();
-    if (key0 + DQ_KEYS < end) {
-      kl.load(tiles + (at ^ 1) * BYTES, key0 + DQ_KEYS, a.tokens);
-      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + DQ_KEYS, a.tokens);
+    if (key0 + HALVES * DQ_KEYS < end) {
+      kl.load(tiles + (at ^ 1) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
+      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
     }
+    if (HALVES > 1 && key0 >= end) continue;
     const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
 #pragma unroll
     for (int sub = 0; sub < DQ_KEYS; sub += 32) {
@@ -221,21 +226,41 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* tiles) {
         }
     }
   }
+  if constexpr (HALVES > 1) {
+    constexpr int N = D / 2 + 1;
+    __syncthreads();
+    float* to = lane_slot(lds, N);
+    if (turn > 0) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(16 * c + r) * 64] = acc[c][r];
+      to[(N - 1) * 64] = up;
+    }
+    __syncthreads();
+    if (turn > 0) return false;
+    const float mine = 1.0f / up, by = 1.0f / to[(N - 1) * 64];
+    up = 1.0f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[c][r] = acc[c][r] * mine + to[(16 * c + r) * 64] * by;
+  }
   store_columns<D, D, BF>(a.gq, nullptr, a.heads, head, row, in, 0, acc, a.scale / up);
   return !CAREFUL && in && any_nonfinite(acc);
 }
 
-template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dq(Args a, int item_groups) {
-  __shared__ __attribute__((aligned(16))) char s_tiles[4 * DQ_KEYS * D * 2];
+template <int D, bool BF, int HALVES>
+__global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq(Args a, int item_groups) {
+  __shared__ __attribute__((aligned(16))) char s_tiles[HALVES * 4 * DQ_KEYS * D * 2];
   static_assert(sizeof(s_tiles) >= ITEM_BYTES, "the items' lists");
   const int id = (int)blockIdx.x - item_groups;
   if (id < 0) {
     prompt_items(a, blockIdx.x, item_groups, s_tiles);
     return;
   }
-  const bool apart = prompt_dq_block<D, BF, false>(a, id, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, true>(a, id, s_tiles);
+  const bool apart = prompt_dq_block<D, BF, HALVES, false>(a, id, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, HALVES, true>(a, id, s_tiles);
 }
 
 // ------------------------------------------------------------- dk and dv
@@ -427,7 +452,13 @@ void backward_of(Args a, const int32_t* q_order, const int32_t* k_order, hipStre
   constexpr int C = key_channels_of(D);
   const unsigned blocks = (unsigned)((a.tokens + BLOCK - 1) / BLOCK), groups = a.items ? (blocks + 63) / 64 : 0;
   a.order = q_order;
-  hipLaunchKernelGGL((k_prompt_dq<D, BF>), dim3(blocks * a.heads + groups), dim3(THREADS), 0, s, a, (int)groups);
+  const dim3 grid(blocks * a.heads + groups);
+  bool halves = false;
+  if constexpr (D <= 128) {
+    halves = in_halves(a, back_waves_of(D));
+    if (halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 2>), grid, dim3(2 * THREADS), 0, s, a, (int)groups);
+  }
+  if (!halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 1>), grid, dim3(THREADS), 0, s, a, (int)groups);
   a.order = k_order;
   hipLaunchKernelGGL((k_prompt_dk<D, C, BF>), dim3((a.items ? a.item_count : blocks) * a.kv_heads * (D / C)), dim3(THREADS), 0, s, a);
   if (a.items) hipLaunchKernelGGL((k_prompt_join<D, BF>), dim3(blocks * a.kv_heads, 2 * BLOCK * D / 4 / THREADS), dim3(THREADS), 0, s, a);

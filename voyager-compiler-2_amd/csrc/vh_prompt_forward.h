@@ -124,13 +124,15 @@ struct Forward {
 
 // A workgroup's rows of one head.  True where a row may have got an infinity
 // or NaN that it does not see.
-template <int D, bool BF, bool CAREFUL>
-VH_DEV bool prompt_block(const Args& a, char* tiles) {
+template <int D, bool BF, int HALVES, bool CAREFUL>
+VH_DEV bool prompt_block(const Args& a, char* lds) {
   constexpr int BYTES = KEYS * D * 2;  // of a tile: two of keys, two of values
+  const int turn = Halves<D, HALVES>::half();
+  char* tiles = lds + turn * 4 * BYTES;
   const int rank = blockIdx.x / a.heads, spread = blockIdx.x - rank * a.heads;
   // heads of a group lie `kv_heads` workgroups apart: on one die where those are a multiple of 8
   const int kv = spread % a.kv_heads, head = kv * a.group + spread / a.kv_heads;
-  const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row0 = a.order[rank] * BLOCK, wave = __builtin_amdgcn_readfirstlane(threadIdx.x % THREADS / 64), lane = threadIdx.x & 63;
   const int wave0 = row0 + 32 * wave, row = wave0 + (lane & 31);
   const bool in = row < a.tokens;
   const int first = in ? a.first[row] : row + 1;
@@ -147,17 +149,19 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
   for (int c = 0; c < D / 32; ++c) f.acc[c] = f32x16{};
   f.ref = -__builtin_inff();
   f.sum = f.rounded = 0.0f;
-  if (begin < end) {
-    kl.load(tiles, begin, a.tokens);
-    vl.load(tiles + 2 * BYTES, begin, a.tokens);
+  const int first_key = begin + turn * KEYS;
+  if (first_key < end) {
+    kl.load(tiles, first_key, a.tokens);
+    vl.load(tiles + 2 * BYTES, first_key, a.tokens);
   }
   int at = 0;
-  for (int key0 = begin; key0 < end; key0 += KEYS, at ^= 1) {
+  for (int key0 = first_key; key0 - turn * KEYS < end; key0 += HALVES * KEYS, at ^= 1) {
     arrived();
-    if (key0 + KEYS < end) {
-      kl.load(tiles + (at ^ 1) * BYTES, key0 + KEYS, a.tokens);
-      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + KEYS, a.tokens);
+    if (key0 + HALVES * KEYS < end) {
+      kl.load(tiles + (at ^ 1) * BYTES, key0 + HALVES * KEYS, a.tokens);
+      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + HALVES * KEYS, a.tokens);
     }
+    if (HALVES > 1 && key0 >= end) continue;
     const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
 #pragma unroll
     for (int sub = 0; sub < KEYS; sub += sub_of(D)) {
@@ -166,6 +170,32 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
       if (key >= wave0 + 32 || key + SUB <= wave_first) continue;
       f.step(q, k, v, sub, key, row, first, key + SUB > wave0 + 1 || key < wave_last_first, scale);
     }
+  }
+  if constexpr (HALVES > 1) {
+    constexpr int N = D / 2 + 3;
+    __syncthreads();
+    float* to = lane_slot(lds, N);
+    if (turn > 0) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(16 * c + r) * 64] = f.acc[c][r];
+      to[(N - 3) * 64] = f.ref;
+      to[(N - 2) * 64] = f.sum;
+      to[(N - 1) * 64] = f.rounded;
+    }
+    __syncthreads();
+    if (turn > 0) return false;
+    const float other = to[(N - 3) * 64], most = fmaxf(f.ref, other);
+    const float mine = f.ref == -__builtin_inff() ? 1.0f : exp2_fast(f.ref - most);  // of nothing: 0 times 1
+    const float by = other == -__builtin_inff() ? 1.0f : exp2_fast(other - most);
+    f.ref = most;
+    f.sum = f.sum * mine + to[(N - 2) * 64] * by;
+    f.rounded = f.rounded * mine + to[(N - 1) * 64] * by;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) f.acc[c][r] = f.acc[c][r] * mine + to[(16 * c + r) * 64] * by;
   }
   f.sum = sum_halves(f.sum);
   f.rounded = sum_halves(f.rounded);
@@ -182,18 +212,29 @@ VH_DEV bool prompt_block(const Args& a, char* tiles) {
 // A masked key's weight is 0, but 0 times an infinity or NaN is not: a block
 // into whose rows such a value may have come is done once more, with these
 // values apart.
+template <int D, bool BF, int HALVES>
+__global__ void __launch_bounds__(HALVES* THREADS, waves_of(D)) k_prompt(Args a) {
+  __shared__ __attribute__((aligned(16))) char s_tiles[HALVES * 4 * KEYS * D * 2];
+  const bool apart = prompt_block<D, BF, HALVES, false>(a, s_tiles);
+  if (__syncthreads_or(apart)) prompt_block<D, BF, HALVES, true>(a, s_tiles);
+}
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS, waves_of(D)) k_prompt(Args a) {
-  __shared__ __attribute__((aligned(16))) char s_tiles[4 * KEYS * D * 2];
-  const bool apart = prompt_block<D, BF, false>(a, s_tiles);
-  if (__syncthreads_or(apart)) prompt_block<D, BF, true>(a, s_tiles);
+void forward_of(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.tokens + BLOCK - 1) / BLOCK * a.heads));
+  if constexpr (D <= 128) {
+    if (in_halves(a, waves_of(D))) {
+      hipLaunchKernelGGL((k_prompt<D, BF, 2>), grid, dim3(2 * THREADS), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((k_prompt<D, BF, 1>), grid, dim3(THREADS), 0, s, a);
 }
 
 template <int D>
 int forward(const Args& a, bool bf16, hipStream_t s) {
-  const dim3 grid((unsigned)((a.tokens + BLOCK - 1) / BLOCK * a.heads));
-  if (bf16) hipLaunchKernelGGL((k_prompt<D, true>), grid, dim3(THREADS), 0, s, a);
-  else hipLaunchKernelGGL((k_prompt<D, false>), grid, dim3(THREADS), 0, s, a);
+  if (bf16) forward_of<D, true>(a, s);
+  else forward_of<D, false>(a, s);
   return vh::check_launch("vh_prompt_attention");
 }
 

@@ -19,7 +19,7 @@ MAX_TOKENS = (1 << 24) - 1
 DIMS = (64, 128, 256)
 PACKING_ERR_OFFSETS = 1
 #: ``vh_prompt_desc``
-PROMPT = struct.Struct("@QqqQqqQqqQQQQQqqQQQqfiiii4x")
+PROMPT = struct.Struct("@QqqQqqQqqQQQQQqqQQQqfiiiii")
 
 
 class Packing:
@@ -99,7 +99,7 @@ def _desc(q, k, v, packing, o, low, lse, scale, go=None, grads=(0, 0, 0)):
     return PROMPT.pack(q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
                        packing.plan.data_ptr(), o.data_ptr(), ptr(low) or 0, lse.data_ptr(), ptr(go) or 0,
                        *(go.stride()[:2] if go is not None else (0, 0)), *grads, packing.tokens, scale, dtype_code(q.dtype),
-                       q.shape[1], k.shape[1], q.shape[2])
+                       q.shape[1], k.shape[1], q.shape[2], packing.sequences)
 
 
 def _forward(q, k, v, packing, scale, train=False):
