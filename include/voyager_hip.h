@@ -859,7 +859,7 @@ int64_t vh_norm_rope_workspace_bytes(const vh_norm_rope_desc* desc);
  * [rows, top]: the largest entries in order, of equal ones the first, a NaN
  * before all others.  Entries of -inf have probability 0; a row of nothing else, or with
  * +inf or NaN, has no probabilities: NaN.  stats [rows, 2] float32 (8-byte
- * aligned) is for the backward pass, which reads logits, tokens, entropy,
+ * aligned; NULL: not wanted) is for the backward pass, which reads logits, tokens, entropy,
  * stats and top_token again and writes grad [rows, vocab], contiguous, for the
  * gradients g_logprob, g_entropy [rows], g_top [rows, top] (NULL: none).
  * work: vh_score_workspace_bytes(desc) bytes, 16-byte aligned. */

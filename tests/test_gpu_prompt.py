@@ -102,7 +102,8 @@ def test_views(d):
         x = torch.empty(n, t.shape[1], d + 3, dtype=BF16, device="cuda")[..., 1:d + 1]
         odd.append(x.copy_(t))
     turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (c.q, c.k, c.v)]
-    for q, k, v in (parts, heads_first, odd, turned):
+    off = [torch.cat((t.flatten()[:3], t.flatten()))[3:].view(t.shape) for t in (c.q, c.k, c.v)]  # dense, but off 16 bytes
+    for q, k, v in (parts, heads_first, odd, turned, off):
         assert all(torch.equal(a, b) for a, b in zip(c.run(q, k, v), want))
     for go in (torch.cat((c.go, c.go), 1)[:, :4], c.go.transpose(0, 1).contiguous().transpose(0, 1),
                c.go.transpose(1, 2).contiguous().transpose(1, 2)):

@@ -141,7 +141,7 @@ def test_score_entries_refuse(kw):
 
 
 def test_score_entries_need_their_tensors():
-    for kw in (dict(logits=0), dict(tokens=0), dict(logprob=0), dict(entropy=0), dict(stats=0), dict(top_logprob=0),
+    for kw in (dict(logits=0), dict(tokens=0), dict(logprob=0), dict(entropy=0), dict(top_logprob=0),
                dict(top_token=0), dict(vocab=100000, work=None), dict(vocab=100000, work=P + 4), dict(vocab=100000, work_bytes=8)):
         assert _score(**kw) == 1
     for kw in (dict(logits=0), dict(tokens=0), dict(entropy=0), dict(stats=0), dict(grad=0), dict(g_top=P, top_token=0)):
@@ -253,7 +253,7 @@ def test_packing_refuses():
 
 def test_prompt_arguments_refused():
     class Plan:  # a packing that was made on a GPU
-        tokens, sequences, device = 6, 1, torch.device("cpu")
+        tokens, sequences, device, _checked = 6, 1, torch.device("cpu"), None
 
     q, k = torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16)
     run = prompt.prompt_attention
@@ -270,16 +270,16 @@ def test_prompt_arguments_refused():
         with pytest.raises(ValueError, match="query heads"):
             run(torch.zeros(6, heads, 64, dtype=torch.bfloat16), *(torch.zeros(6, kv, 64, dtype=torch.bfloat16),) * 2, Plan)
     with pytest.raises(ValueError, match="cuda"):  # no CPU form
-        run(q, k, k, type("Other", (), dict(tokens=6, sequences=1, device=torch.device("cpu"), plan=torch.zeros(1))))
+        run(q, k, k, type("Other", (), dict(tokens=6, sequences=1, _checked=None, device=torch.device("cpu"), plan=torch.zeros(1))))
     with pytest.raises(ValueError, match="its packing on"):
-        run(q, k, k, type("Other", (), dict(tokens=6, device=torch.device("cuda", 0))))
+        run(q, k, k, type("Other", (), dict(tokens=6, _checked=None, device=torch.device("cuda", 0))))
 
 
 def test_prompt_refuses_tangents():
     import torch.autograd.forward_ad as fwAD
 
     class Plan:
-        tokens, sequences, device = 6, 1, torch.device("cpu")
+        tokens, sequences, device, _checked = 6, 1, torch.device("cpu"), None
 
     k = torch.zeros(6, 2, 64, dtype=torch.bfloat16)
     with fwAD.dual_level():

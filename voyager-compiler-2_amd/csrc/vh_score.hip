@@ -129,7 +129,7 @@ VH_DEV float2 write_row(const Args& a, int64_t row, int64_t token, float x, floa
   const float2 s = good ? make_float2(m, log2l * LN2) : make_float2(nan, nan);
   a.logprob[row] = token < a.vocab ? x - s.x - s.y : nan;
   a.entropy[row] = good ? fmaxf((log2l - e / l) * LN2, 0.0f) : nan;
-  a.stats[row] = s;
+  if (a.stats) a.stats[row] = s;
   return s;
 }
 VH_DEV void write_top(const Args& a, int64_t row, float2 s, int at, okey key) {
@@ -140,7 +140,7 @@ template <int N>
 VH_DEV void write_padding(const Args& a, int64_t row) {
   if (threadIdx.x == 0) {
     a.logprob[row] = a.entropy[row] = 0.0f;
-    a.stats[row] = make_float2(0.0f, 0.0f);
+    if (a.stats) a.stats[row] = make_float2(0.0f, 0.0f);
   }
   for (int i = threadIdx.x; i < a.top; i += N) {
     a.top_logprob[row * a.top + i] = 0.0f;
@@ -345,6 +345,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_score_join(Args a) {
   const int64_t token = a.tokens[row];
   if (token < 0) return;
   const okey* lists = a.part_top + row * a.pieces * a.top;
+  const int listed = a.pieces * a.top;
+  const okey early = (int)threadIdx.x < listed ? lists[threadIdx.x] : 0ull;  // on its way while the rest is found
   if (threadIdx.x < 64) {
     const int p = threadIdx.x;
     const float* part = a.part + (row * a.pieces + (p < a.pieces ? p : 0)) * 3;
@@ -375,8 +377,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_score_join(Args a) {
   if (a.top == 0) return;
   __syncthreads();
   const okey bound = s_bound;
-  for (int i = threadIdx.x; i < a.pieces * a.top; i += JOIN_THREADS) {
-    const okey key = lists[i];
+  for (int i = threadIdx.x; i < listed; i += JOIN_THREADS) {
+    const okey key = i < JOIN_THREADS ? early : lists[i];
     if (key >= bound) s_key[atomicAdd(&s_count, 1u)] = key;
   }
   __syncthreads();
@@ -544,7 +546,7 @@ extern "C" int64_t vh_score_workspace_bytes(const vh_score_desc* d) {
 extern "C" int vh_score(const vh_score_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
   if (int e = check(d, "vh_score")) return e;
   if (d->rows == 0) return VH_OK;
-  VH_REQUIRE(d->logits && d->tokens && d->logprob && d->entropy && d->stats && (d->top == 0 || (d->top_logprob && d->top_token)),
+  VH_REQUIRE(d->logits && d->tokens && d->logprob && d->entropy && (d->top == 0 || (d->top_logprob && d->top_token)),
              "vh_score: null argument");
   const Plan p = plan_of(d);
   const int64_t need = part_bytes(d, p);

@@ -37,6 +37,7 @@ class Packing:
         if not 0 <= tokens <= MAX_TOKENS:
             raise ValueError(f"Packing: at most {MAX_TOKENS} tokens (got {tokens})")
         self.tokens, self.sequences, self.device = tokens, offsets.shape[0] - 1, offsets.device
+        self._checked = None
         lib = load()
         self.flag = torch.zeros(1, dtype=torch.int32, device=offsets.device)
         #: each row's first key, the row after the last that sees it as a key, and the blocks in order
@@ -67,6 +68,20 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     float32; weights, and in the backward pass their gradients, are rounded to
     the values' type for the matrix instructions.  Differentiable once in q, k
     and v; sums are in a fixed order."""
+    given = (q.shape, q.dtype, q.device, k.shape, k.dtype, k.device, v.shape, v.dtype, v.device)
+    if given != packing._checked:  # a layer's sizes are mostly those of the layer before
+        _check(q, k, v, packing)
+        packing._checked = given
+    no_tangents("prompt_attention", q, k, v)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _Attention.apply(q, k, v, packing, scale)
+    else:
+        o, lse = _forward(q, k, v, packing, scale)[:2]
+    return (o, lse) if return_lse else o
+
+
+def _check(q, k, v, packing) -> None:
     t = packing.tokens
     if q.dim() != 3 or q.shape[0] != t or q.shape[2] not in DIMS or q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"prompt_attention: q must be bfloat16 or float16 [{t}, heads, 64, 128 or 256] (got {q.dtype} "
@@ -80,19 +95,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
             raise ValueError(f"prompt_attention: {name} is on {x.device}, its packing on {packing.device}")
     if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"prompt_attention: {q.shape[1]} query heads over {k.shape[1]}")
-    no_tangents("prompt_attention", q, k, v)
-    scale = q.shape[2] ** -0.5 if scale is None else scale
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _Attention.apply(q, k, v, packing, scale)
-    else:
-        o, lse = _forward(q, k, v, packing, scale)[:2]
-    return (o, lse) if return_lse else o
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with dense channels and its rows aligned to 16 bytes."""
     st, sh, sc = t.stride()
-    return t if sc == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0 and st < 1 << 23 else t.contiguous()
+    if sc == 1 and not (st | sh) & 7 and not t.data_ptr() & 15 and st < 1 << 23:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _desc(q, k, v, packing, o, low, lse, scale, go=None, grads=(0, 0, 0)):

@@ -19,6 +19,7 @@ MAX_TOP = 64
 MAX_VOCAB = 1 << 20
 #: ``vh_score_desc``
 SCORE = struct.Struct("@QqQqqQQQQQQQQQii")
+_work = {}  # bytes of workspace, by a call's sizes
 
 
 class Scores(NamedTuple):
@@ -61,7 +62,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Sc
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _Scores.apply(x, t, top)
     else:
-        out = _scores(x, t, top)[:4 if top else 2]
+        out = _scores(x, t, top, False)[:4 if top else 2]
     shape = tokens.shape
     if len(shape) != 1:
         out = [y.view(shape + y.shape[1:]) for y in out]
@@ -72,18 +73,26 @@ def _rows(x):
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
-def _scores(x, tokens, top):
+def _scores(x, tokens, top, train):
     x, tokens = _rows(x), tokens.contiguous()
     rows, vocab = x.shape
     dev = x.device
     f = dict(dtype=torch.float32, device=dev)
-    logprob, entropy, stats = torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, 2, **f)
+    logprob, entropy = torch.empty(rows, **f), torch.empty(rows, **f)
+    stats = torch.empty(rows, 2, **f) if train else None
     best = torch.empty(rows, top, **f) if top else None
     index = torch.empty(rows, top, dtype=torch.int64, device=dev) if top else None
     d = SCORE.pack(x.data_ptr(), x.stride(0), tokens.data_ptr(), rows, vocab, logprob.data_ptr(), entropy.data_ptr(),
-                   stats.data_ptr(), ptr(best) or 0, ptr(index) or 0, 0, 0, 0, 0, dtype_code(x.dtype), top)
+                   ptr(stats) or 0, ptr(best) or 0, ptr(index) or 0, 0, 0, 0, 0, dtype_code(x.dtype), top)
     lib = load()
-    need = lib.vh_score_workspace_bytes(d)
+    sizes = (rows, vocab, x.dtype, top)
+    need = _work.get(sizes)
+    if need is None:
+        need = lib.vh_score_workspace_bytes(d)
+        if need >= 0:  # or the call says what is wrong
+            if len(_work) >= 4096:
+                _work.clear()
+            _work[sizes] = need
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     st = lib.vh_score(d, ptr(work), max(need, 0), stream_on(dev))
     if st:
@@ -97,7 +106,7 @@ class _Scores(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, tokens, top):
-        logprob, entropy, best, index, stats = _scores(x, tokens, top)
+        logprob, entropy, best, index, stats = _scores(x, tokens, top, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, tokens, entropy, stats, index)
         ctx.top = top
