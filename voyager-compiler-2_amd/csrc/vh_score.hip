@@ -148,6 +148,27 @@ VH_DEV void write_padding(const Args& a, int64_t row) {
   }
 }
 
+// The m-th largest of a wave's ranks, found bit by bit.
+VH_DEV uint32_t largest(uint32_t mine, int m) {
+  uint32_t bound = 0u;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = bound | 1u << bit;
+    if (__popcll(__ballot(mine >= t)) >= m) bound = t;
+  }
+  return bound;
+}
+
+// Of G groups, each with at least t entries that reach a bound of its own,
+// the m-th largest bound is reached by m t entries: by `top`, with these.
+struct Share {
+  int t, m;
+};
+VH_DEV Share share_of(int top, int groups) {
+  const int t = (top + groups - 1) / groups;
+  return Share{t, (top + t - 1) / t};
+}
+
 // The `top` largest of n keys, in order, with 0 for those that are not there.
 template <int N>
 VH_DEV void rank_keys(const okey* keys, int n, int top, okey* best) {
@@ -244,14 +265,8 @@ __global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
     s_f[2][wave] = e;
   }
   if constexpr (TOP) {
-    // The top-th largest of the lanes' maxima of a wave: as many of its entries reach that.
-    const uint32_t mine = rank_of(lane_most);
-    uint32_t bound = 0u;
-#pragma unroll
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = bound | 1u << bit;
-      if (__popcll(__ballot(mine >= t)) >= a.top) bound = t;
-    }
+    // the t-th largest of the lanes' maxima of a wave: as many of its entries reach that
+    const uint32_t bound = largest(rank_of(lane_most), share_of(a.top, WAVES).t);
     if (lane == 0) s_bound[wave] = bound;
   }
   __syncthreads();
@@ -286,9 +301,14 @@ __global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
       }
     }
   };
-  uint32_t bound = 0u;
+  uint32_t bound = 0u;  // the m-th largest of the waves'
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) bound = umax32(bound, s_bound[w]);
+  for (int w = 0; w < WAVES; ++w) {
+    int reach = 0;
+#pragma unroll
+    for (int u = 0; u < WAVES; ++u) reach += s_bound[u] >= s_bound[w];
+    if (reach >= share_of(a.top, WAVES).m) bound = umax32(bound, s_bound[w]);
+  }
   // The last index of entries at the bound that count: what stands in for entries
   // past the end is -inf, as low as an entry can be, and so at the bound at most.
   uint32_t upto = (uint32_t)end - 1u;
@@ -359,15 +379,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_score_join(Args a) {
     const float by = in ? exponent(mine, to) : 0.0f, f = in ? exp2_fast(by) : 0.0f;
     const float l = wave_sum(in ? part[1] * f : 0.0f);
     const float e = wave_sum(in ? __builtin_fmaf(part[1], by, part[2]) * f : 0.0f);
-    // every list's last key has `top` keys that reach it
-    if (a.top > 0) {
-      okey least = p < a.pieces ? lists[(int64_t)p * a.top + a.top - 1] : 0ull;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const okey other = __shfl_xor(least, d);
-        least = other > least ? other : least;
-      }
-      if (p == 0) s_bound = least > 1ull ? least : 1ull;
+    if (a.top > 0) {  // lists are in order: t keys of one reach its t-th
+      const Share by = share_of(a.top, a.pieces);
+      const uint32_t reach = largest(p < a.pieces ? (uint32_t)(lists[p * a.top + by.t - 1] >> 32) : 0u, by.m);
+      if (p == 0) s_bound = reach > 0u ? (okey)reach << 32 : 1ull;
     }
     if (p == 0) {
       s_stats = write_row(a, row, token, x, to, l, e);
