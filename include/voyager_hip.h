@@ -887,6 +887,7 @@ int64_t vh_score_workspace_bytes(const vh_score_desc* desc);
  * Offsets are read on the device: where they are not as they should be, all
  * rows pad and VH_PACKING_ERR_OFFSETS is set in `flag`. */
 #define VH_PROMPT_BLOCK 128
+#define VH_PROMPT_SHORT 512
 #define VH_PROMPT_MAX_TOKENS 16777216
 #define VH_PACKING_ERR_OFFSETS 1
 int64_t vh_packing_ints(int64_t tokens);
@@ -899,7 +900,8 @@ int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_
  * itself.  sequences: of the plan, by whose number the launch is shaped.  o:
  * contiguous; lse [tokens, heads] float32, the logarithm of the sum of
  * exponentials; rows that pad give 0 and -inf.  o_low (NULL: not wanted): what
- * the rounding of o left out, in bfloat16, laid out as o.
+ * the rounding of o left out, in bfloat16, laid out as o; the backward pass
+ * reads it unless there are fewer than VH_PROMPT_SHORT tokens a sequence.
  * The backward pass reads q, k, v, o, o_low, lse and the result's gradient go
  * (strides as above) and writes gq, gk, gv, contiguous, in a fixed order of sums.  work:
  * vh_prompt_attention_workspace_bytes(desc) bytes, 16-byte aligned. */

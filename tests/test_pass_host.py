@@ -38,6 +38,10 @@ def test_descriptors_are_as_long_as_the_header_says():
     assert _size("vh_norm_rope_desc") == rope + rotary.NORM.size
     assert _size("vh_score_desc") == score.SCORE.size
     assert _size("vh_prompt_desc") == prompt.PROMPT.size
+    text = open(os.path.join(os.path.dirname(__file__), "..", "include", "voyager_hip.h")).read()
+    for name, value in (("VH_PROMPT_SHORT", prompt.SHORT), ("VH_PROMPT_MAX_TOKENS", prompt.MAX_TOKENS + 1),
+                        ("VH_SCORE_MAX_TOP", score.MAX_TOP), ("VH_SCORE_MAX_VOCAB", score.MAX_VOCAB)):
+        assert int(re.search(rf"#define {name} (\d+)", text).group(1)) == value
 
 
 # ------------------------------------------------------- norms and positions
@@ -223,7 +227,7 @@ def test_prompt_entries_need_aligned_tensors(kw):
     assert _prompt(**kw) == 1 and _prompt(BACK, **kw) == 1
 
 
-@pytest.mark.parametrize("kw", [dict(go=0), dict(o_low=0), dict(gq=0), dict(gk=0), dict(gv=0), dict(go=P + 8), dict(go_sh=2),
+@pytest.mark.parametrize("kw", [dict(go=0), dict(o_low=0, tokens=512), dict(gq=0), dict(gk=0), dict(gv=0), dict(go=P + 8), dict(go_sh=2),
                                 dict(gk=P + 8), dict(work=None), dict(work=P + 8), dict(work_bytes=16)])
 def test_prompt_backward_needs_its_tensors(kw):
     assert _prompt(BACK, **kw) == 1

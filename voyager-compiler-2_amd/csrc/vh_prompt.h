@@ -297,14 +297,15 @@ VH_DEV uint32_t bad_rows(const char* tile, int row0) {
   return (uint32_t)all | (uint32_t)(all >> 32);
 }
 
-// Whether two halves of a workgroup share a block: where one wave of workgroups
+// Whether two halves of a workgroup share a block, which `short_sequences`, by their mean, never do: where one wave of workgroups
 // holds all blocks, so that the longest is the pass, and sequences are long.
 // (us by one and by two, 16 + 4 heads: a prompt of 6000, heads of 64, 150 and 111,
 // of 3000, heads of 128, 85 and 64; four of 775 44 and 36; 16 of 250 22 and 27.
 // 32 + 8 heads of 128, 4096: 164 and 176.)
+VH_DEV __host__ bool short_sequences(const Args& a) { return a.tokens < (int64_t)VH_PROMPT_SHORT * a.sequences; }
 inline bool in_halves(const Args& a, int waves) {
   const int64_t blocks = (a.tokens + BLOCK - 1) / BLOCK;
-  return blocks * a.heads <= 256 * waves && a.tokens >= 512ll * a.sequences;
+  return blocks * a.heads <= 256 * waves && !short_sequences(a);
 }
 
 template <int D>

@@ -144,8 +144,40 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   // D, and lse log2(e), which is inf where a row sees nothing, so that its weights are 0: for the keys' pass as well
   const float natural = in ? a.lse[(int64_t)row * a.heads + head] : -__builtin_inff();
   const float lse = natural == -__builtin_inff() ? __builtin_inff() : natural * LOG2E;
+  Loader<D, DQ_KEYS> kl, vl;
+  kl.init(a.k, kv);
+  vl.init(a.v, kv);
+  const float scale = a.scale * LOG2E;
   float dot = 0.0f;
-  {
+  if (HALVES == 1 && short_sequences(a)) {
+    // A short row's result has weights in it that are rounded and few, and of
+    // that D is more wrong than a weight's own rounding makes its gradient: D as
+    // sum P dP instead, by the keys once more.
+    for (int key0 = begin; key0 < end; key0 += DQ_KEYS) {
+      if (key0 > begin) __syncthreads();
+      kl.load(tiles, key0, a.tokens);
+      vl.load(tiles + 2 * BYTES, key0, a.tokens);
+      arrived();
+#pragma unroll
+      for (int sub = 0; sub < DQ_KEYS; sub += 32) {
+        const int key = key0 + sub;
+        if (key >= wave0 + 32 || key + 32 <= wave_first) continue;
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(tiles, sub, i), q[i], s);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dp = mfma<BF>(rows_operand<D>(tiles + 2 * BYTES, sub, i), go[i], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = key + result_row(r) + 4 * half;
+          const float x = exp2_fast(__builtin_fmaf(s[r], scale, -lse)) * dp[r];
+          dot += j >= first && j <= row ? x : 0.0f;
+        }
+      }
+    }
+    dot = sum_halves(dot);
+    __syncthreads();  // the tiles are loaded over next
+  } else {
     uint4 o[D / 16];
     const Tensor out{a.o, (int64_t)a.heads * D, D}, low{a.o_low, (int64_t)a.heads * D, D};
 #pragma unroll
@@ -169,10 +201,6 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
     if (half == 0) to[0] = lse;
     else to[a.tokens] = dot;
   }
-  Loader<D, DQ_KEYS> kl, vl;
-  kl.init(a.k, kv);
-  vl.init(a.v, kv);
-  const float scale = a.scale * LOG2E;
   f32x16 acc[D / 32];
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) acc[c] = f32x16{};

@@ -17,7 +17,7 @@ from ._lib import check, dtype_code, load, no_tangents, once, ptr, stream_on
 
 MAX_TOKENS = (1 << 24) - 1
 DIMS = (64, 128, 256)
-PACKING_ERR_OFFSETS = 1
+SHORT = 512  # ``VH_PROMPT_SHORT``
 #: ``vh_prompt_desc``
 PROMPT = struct.Struct("@QqqQqqQqqQQQQQqqQQQqfiiiii")
 
@@ -115,8 +115,8 @@ def _desc(q, k, v, packing, o, low, lse, scale, go=None, grads=(0, 0, 0)):
 def _forward(q, k, v, packing, scale, train=False):
     q, k, v = _rows(q), _rows(k), _rows(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    # what the rounding leaves out: the backward pass takes sums over a row's result, in which it would be seen
-    low = torch.empty_like(o, dtype=torch.bfloat16) if train else None
+    # what the rounding leaves out: the backward pass takes sums over a long row's result, in which it would be seen
+    low = torch.empty_like(o, dtype=torch.bfloat16) if train and packing.tokens >= SHORT * packing.sequences else None
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     st = load().vh_prompt_attention(_desc(q, k, v, packing, o, low, lse, scale), stream_on(q.device))
     if st:
