@@ -13,6 +13,10 @@
 // is summed in a fixed order: each lane over the heads that it takes, the
 // lanes of a workgroup through LDS, the workgroups by a second kernel in
 // float64.
+//
+// Bound by memory.  8192 tokens of 32 + 8 heads of 128 in bfloat16: forward (168
+// MB) 31 us, 5.4 TB/s; back (252 MB) 50 us, 5.0 TB/s, and 3 us for the weights'
+// sums.  A single token 3.6 us, its loads' and the launch's latency.
 #include <hip/hip_runtime.h>
 
 #include "vh_device.h"
@@ -23,7 +27,9 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int MAX_DIM = 512;
 constexpr int TOKENS = 4;      // tokens of a workgroup when there are many
-constexpr int BACK_GROUPS = 1024;  // workgroups that share out the tokens of a backward pass
+// Workgroups that share out the tokens of a backward pass: four a CU, whose sums
+// of the weights' gradients are then 1 MB.
+constexpr int BACK_GROUPS = 1024;
 
 struct Tensor {
   const void* x;
@@ -300,7 +306,7 @@ Plan plan_of(const vh_norm_rope_desc* d, bool back) {
   while (p.lanes < p.units && p.lanes < 64) p.lanes *= 2;
   const int64_t rows = r.batch * r.tokens;
   const int heads = r.heads + r.kv_heads, per = THREADS / p.lanes;
-  p.many = rows >= 2048;  // as vh_rope
+  p.many = rows >= 2048;  // as vh_rope, where both sides' times are
   int64_t x = p.many ? (rows + TOKENS - 1) / TOKENS : rows;
   int64_t y = p.many ? 1 : (heads + per - 1) / per;
   if (back && x * y > BACK_GROUPS) {

