@@ -857,13 +857,15 @@ int64_t vh_norm_rope_workspace_bytes(const vh_norm_rope_desc* desc);
  * the vocabulary has the log probability NaN, in its gradient as well.
  * logprob, entropy [rows] float32, natural logarithms; top_logprob, top_token
  * [rows, top]: the largest entries in order, of equal ones the first, a NaN
- * before all others.  Entries of -inf have probability 0; a row of nothing else, or with
- * +inf or NaN, has no probabilities: NaN.  stats [rows, 2] float32 (8-byte
- * aligned; NULL: not wanted) is for the backward pass, which reads logits, tokens, entropy,
- * stats and top_token again and writes grad [rows, vocab], contiguous, for the
- * gradients g_logprob, g_entropy [rows], g_top [rows, top] (NULL: none).
- * work: vh_score_workspace_bytes(desc) bytes, 16-byte aligned. */
+ * before all others.  Entries of -inf have probability 0; a row of nothing else,
+ * or with +inf or NaN, has no probabilities: NaN.  stats [rows, 2] float32 (8-byte
+ * aligned; NULL: not wanted) is for the backward pass, which reads logits, tokens,
+ * entropy, stats and top_token again and writes grad [rows, vocab], contiguous, for
+ * the gradients g_logprob, g_entropy [rows], g_top [rows, top] (NULL: none).  Fewer
+ * than VH_SCORE_MAX_ROWS.  work: vh_score_workspace_bytes(desc) bytes, 16-byte
+ * aligned. */
 #define VH_SCORE_MAX_TOP 64
+#define VH_SCORE_MAX_ROWS 8388608
 #define VH_SCORE_MAX_VOCAB 1048576
 typedef struct vh_score_desc {
   const void* logits;
@@ -885,10 +887,12 @@ int64_t vh_score_workspace_bytes(const vh_score_desc* desc);
  * 1] - 1 of `tokens` (offsets [sequences + 1] begin at 0 and do not fall; rows
  * behind the last pad).  plan: vh_packing_ints(tokens) int32 of device memory.
  * Offsets are read on the device: where they are not as they should be, all
- * rows pad and VH_PACKING_ERR_OFFSETS is set in `flag`. */
+ * rows pad and VH_PACKING_ERR_OFFSETS is set in `flag`.  Fewer than
+ * VH_PROMPT_MAX_TOKENS and VH_PACKING_MAX_SEQUENCES. */
 #define VH_PROMPT_BLOCK 128
 #define VH_PROMPT_SHORT 512
 #define VH_PROMPT_MAX_TOKENS 16777216
+#define VH_PACKING_MAX_SEQUENCES 1048576
 #define VH_PACKING_ERR_OFFSETS 1
 int64_t vh_packing_ints(int64_t tokens);
 int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_t* plan, int32_t* flag, vh_stream_t stream);

@@ -78,6 +78,26 @@ def test_many_tokens_share_the_weights_gradient():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_more_rows_and_heads_than_workgroups():
+    """The last rows, and the last heads, beside a call of their own."""
+    for b, t, heads, dim in ((1, (1 << 26) + 5, 1, 2), (1, 2, 300000, 130)):
+        rot = rotary.Rotary(dim)
+        g = torch.Generator(device="cuda").manual_seed(t + heads)
+        q = torch.randn(b, t, heads, dim, generator=g, device="cuda", dtype=torch.bfloat16)
+        w = torch.linspace(0.5, 1.5, dim, device="cuda")
+        pos = torch.arange(t, device="cuda", dtype=torch.int32)
+        rows, of = min(t, 1000), min(heads, 100)
+        y = rot.normed(q, None, pos, w, None)[0]
+        assert torch.equal(y[:, -rows:, -of:], rot.normed(q[:, -rows:, -of:], None, pos[-rows:], w, None)[0])
+        assert torch.equal(y[:, :rows, :of], rot.normed(q[:, :rows, :of], None, pos[:rows], w, None)[0])
+        x = q.requires_grad_()
+        go = torch.ones((), device="cuda", dtype=torch.bfloat16).expand(q.shape)
+        dx, = torch.autograd.grad(rot.normed(x, None, pos, w, None)[0], x, go)
+        part = q.detach()[:, -rows:, -of:].requires_grad_()
+        dp, = torch.autograd.grad(rot.normed(part, None, pos[-rows:], w, None)[0], part, go[:, -rows:, -of:])
+        assert torch.equal(dx[:, -rows:, -of:], dp)
+
+
 def test_views():
     c = Case(2, 9, 4, 2, 64)
     fused = torch.cat((c.q, c.k, c.k), 2)

@@ -114,6 +114,23 @@ def test_views(d):
     c.check(got)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 128), (BF16, 256)])
+@pytest.mark.parametrize("lengths", [[40], [300, 7], [700]])
+def test_far_scores_of_one_key(dtype, d, lengths):
+    """Each row is its own key's alone, with a score of some thousands, whose
+    logarithm of a sum float32 holds to 2^-11 only: the scores' gradients are 0.
+    A weight's gradient and D are two sums of at most 256 products, each off by at
+    most 2^-16 of the sum of their magnitudes, and what o and its remainder leave
+    out by 2^-18: together under 2^-14."""
+    c = Case(lengths, 2, 2, d, dtype, scale=1.0)
+    c.k = (8192 ** 0.5 * torch.nn.functional.normalize(c.k.float(), dim=2)).to(dtype)
+    _, lse, dq, dk, _ = c.run(q=c.k)
+    assert 8000 < float(lse.min()) and float(lse.max()) < 8400
+    most = 2.0 ** -14 * (c.go.double() * c.v.double()).abs().sum(2, keepdim=True) * c.k.double().abs()
+    for name, y in (("dq", dq), ("dk", dk)):
+        assert bool((y.double().abs() <= most).all()), (name, float((y.double().abs() / most).max()))
+
+
 def test_a_gradient_of_one_value_for_all():
     c = Case([70, 30], 2, 1, 64, F16)
     c.go = torch.ones_like(c.go)

@@ -55,6 +55,22 @@ def test_values_and_gradients(dtype, rows, vocab, top):
     check(_logits(rows, vocab, dtype), _tokens(rows, vocab), top)
 
 
+def test_the_most_rows():
+    """The last rows, beside a call of their own."""
+    rows = (1 << 23) - 1
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(rows, 3, generator=g, device="cuda", dtype=torch.float16)
+    t = torch.randint(-1, 3, (rows,), generator=g, device="cuda")
+
+    def run(x, t):
+        x = x.detach().requires_grad_()
+        s = score.token_scores(x, t, top=2)
+        return [*(y.detach() for y in s), *torch.autograd.grad((s.logprob + s.entropy).sum(), x)]
+    for some in (slice(0, 1000), slice(-1000, None)):
+        for y, z in zip(run(x, t), run(x[some], t[some])):
+            assert torch.equal(y[some], z)
+
+
 def test_the_largest_vocabulary():
     check(_logits(1, 1 << 20, torch.float32), _tokens(1, 1 << 20), 64)
     check(_logits(2, (1 << 20) - 3, torch.bfloat16), _tokens(2, 1000), 3)

@@ -249,6 +249,25 @@ def test_packing_entry_refuses():
         assert lib.vh_packing(*args, None) == 1
 
 
+# Launches of 2^32 threads and more, and offsets that every workgroup reads.
+@pytest.mark.parametrize("kw", [dict(tokens=(1 << 24) - 1, heads=64, kv_heads=64), dict(tokens=1, heads=1 << 22, kv_heads=1)])
+def test_prompt_launches_have_a_limit(kw):
+    assert _prompt(**kw) == 1 and b"too many heads" in _lib.load().vh_last_error()
+    assert _prompt(BACK, **kw) == 1 and b"too many heads" in _lib.load().vh_last_error()
+
+
+def test_packing_sequences_have_a_limit():
+    for sequences in (1 << 20, 1 << 31, (1 << 63) - 1):
+        assert _lib.load().vh_packing(P, sequences, 10, P, P, None) == 1
+
+
+def test_score_launches_have_a_limit():
+    for entry in ("vh_score", "vh_score_backward"):
+        assert _score(entry, rows=1 << 23) == 1 and b"rows" in _lib.load().vh_last_error()
+    assert _score(rows=1 << 22, vocab=1 << 17) == 1 and b"such a vocabulary" in _lib.load().vh_last_error()
+    assert _score("vh_score_backward", rows=1 << 22, vocab=1 << 17) == 1 and b"such a vocabulary" in _lib.load().vh_last_error()
+
+
 def test_packing_refuses():
     for bad in (torch.zeros(2, dtype=torch.int32), torch.zeros(2), torch.zeros(2, 2, dtype=torch.int32)):
         with pytest.raises(ValueError, match="offsets"):

@@ -30,6 +30,8 @@ constexpr int TOKENS = 4;      // tokens of a workgroup when there are many
 // Workgroups that share out the tokens of a backward pass: four a CU, whose sums
 // of the weights' gradients are then 1 MB.
 constexpr int BACK_GROUPS = 1024;
+// At most, one way and the other, of a launch, which has fewer than 2^32 threads; they take turns beyond.
+constexpr int64_t MOST_GROUPS = 1 << 22, MOST_HEAD_GROUPS = 1 << 15;
 
 struct Tensor {
   const void* x;
@@ -312,6 +314,9 @@ Plan plan_of(const vh_norm_rope_desc* d, bool back) {
   if (back && x * y > BACK_GROUPS) {
     y = y < BACK_GROUPS ? y : BACK_GROUPS;
     x = BACK_GROUPS / y;
+  } else if (x * y > MOST_GROUPS || y > MOST_HEAD_GROUPS) {
+    y = y < MOST_HEAD_GROUPS ? y : MOST_HEAD_GROUPS;
+    x = x < MOST_GROUPS / y ? x : MOST_GROUPS / y;
   }
   p.grid = dim3((unsigned)x, (unsigned)y);
   return p;

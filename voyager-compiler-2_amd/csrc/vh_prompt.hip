@@ -96,8 +96,8 @@ int check(const vh_prompt_desc* d, const char* what) {
   VH_REQUIRE(d->dim == 64 || d->dim == 128 || d->dim == 256, "%s: heads of 64, 128 or 256 (got %d)", what, d->dim);
   VH_REQUIRE(d->tokens >= 0 && d->tokens < VH_PROMPT_MAX_TOKENS, "%s: at most %d tokens", what, VH_PROMPT_MAX_TOKENS - 1);
   VH_REQUIRE(d->kv_heads > 0 && d->heads > 0 && d->heads % d->kv_heads == 0, "%s: query heads must be a multiple of the keys'", what);
-  VH_REQUIRE((blocks_of(d->tokens) + 1) * d->heads < (1ll << 30),
-             "%s: too many heads", what);
+  // a launch has fewer than 2^32 threads
+  VH_REQUIRE((blocks_of(d->tokens) + 1) * d->heads < (1ll << 23), "%s: too many heads for as many tokens", what);
   VH_REQUIRE(d->sequences >= 0, "%s: negative size", what);
   VH_REQUIRE(d->scale > 0.0f && d->scale < __builtin_inff(), "%s: the scale must be positive", what);
   VH_REQUIRE(d->q_st < MOST_STRIDE && d->k_st < MOST_STRIDE && d->v_st < MOST_STRIDE && d->go_st < MOST_STRIDE,
@@ -176,7 +176,8 @@ extern "C" int64_t vh_packing_ints(int64_t tokens) {
 extern "C" int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_t* plan, int32_t* flag,
                           vh_stream_t stream) {
   VH_REQUIRE(tokens >= 0 && tokens < VH_PROMPT_MAX_TOKENS, "vh_packing: at most %d tokens", VH_PROMPT_MAX_TOKENS - 1);
-  VH_REQUIRE(sequences >= 0 && sequences < (1ll << 31), "vh_packing: bad number of sequences");
+  // every workgroup reads them all
+  VH_REQUIRE(sequences >= 0 && sequences < VH_PACKING_MAX_SEQUENCES, "vh_packing: at most %d sequences", VH_PACKING_MAX_SEQUENCES - 1);
   VH_REQUIRE(offsets && flag && (plan || tokens == 0), "vh_packing: null argument");
   hipStream_t s = vh::as_stream(stream);
   int32_t *first = plan, *past = plan + tokens, *order = plan + 2 * tokens;

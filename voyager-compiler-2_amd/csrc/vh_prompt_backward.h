@@ -161,9 +161,11 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   if (HALVES == 1 && short_sequences(a)) {
     // A short row's result has weights in it that are rounded and few, and of
     // that D is more wrong than a weight's own rounding makes its gradient: D as
-    // sum P dP instead, by the keys once more.  (dq's error, in that of the exact one
+    // sum P dP instead, by the keys once more, and over sum P, as the weights
+    // of far scores are off together by what lse in 32 bits is.  (dq's error, in that of the exact one
     // rounded, by o and by this: a sequence of 40 rows 1.44-1.55 and 1.39-1.49, of
     // 300 1.43-1.51 and 1.40-1.46.  For long rows it would be two thirds of this pass.)
+    float all = 0.0f;
     for (int key0 = begin; key0 < end; key0 += DQ_KEYS) {
       if (key0 > begin) __syncthreads();
       kl.load(tiles, key0, a.tokens);
@@ -181,12 +183,15 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = key + result_row(r) + 4 * half;
-          const float x = exp2_fast(__builtin_fmaf(s[r], scale, -lse)) * dp[r];
-          dot += j >= first && j <= row ? x : 0.0f;
+          const float p = j >= first && j <= row ? exp2_fast(__builtin_fmaf(s[r], scale, -lse)) : 0.0f;
+          all += p;
+          dot += p > 0.0f ? p * dp[r] : 0.0f;
         }
       }
     }
     dot = sum_halves(dot);
+    all = sum_halves(all);
+    dot = all == 0.0f ? dot : dot / all;
     __syncthreads();  // the tiles are loaded over next
   } else {
     uint4 o[D / 16];

@@ -514,7 +514,7 @@ Plan plan_of(const vh_score_desc* d) {
 int check(const vh_score_desc* d, const char* what) {
   VH_REQUIRE(d, "%s: null descriptor", what);
   VH_REQUIRE(vh::is_float_dtype(d->dtype), "%s: dtype must be bfloat16, float16 or float32", what);
-  VH_REQUIRE(d->rows >= 0 && d->rows < (1ll << 24), "%s: at most 2^24 - 1 rows", what);
+  VH_REQUIRE(d->rows >= 0 && d->rows < VH_SCORE_MAX_ROWS, "%s: at most %d rows", what, VH_SCORE_MAX_ROWS - 1);
   VH_REQUIRE(d->vocab > 0 && d->vocab <= VH_SCORE_MAX_VOCAB, "%s: a vocabulary of 1 to %d", what, VH_SCORE_MAX_VOCAB);
   VH_REQUIRE(d->top >= 0 && d->top <= MAX_TOP && d->top <= d->vocab, "%s: at most %d alternatives, and no more than the vocabulary",
              what, MAX_TOP);
@@ -573,6 +573,8 @@ extern "C" int vh_score(const vh_score_desc* d, void* work, int64_t work_bytes, 
   VH_REQUIRE(d->logits && d->tokens && d->logprob && d->entropy && (d->top == 0 || (d->top_logprob && d->top_token)),
              "vh_score: null argument");
   const Plan p = plan_of(d);
+  // a launch has fewer than 2^32 threads
+  VH_REQUIRE(d->rows * p.pieces < VH_SCORE_MAX_ROWS, "vh_score: too many rows of such a vocabulary");
   const int64_t need = part_bytes(d, p);
   VH_REQUIRE(need == 0 || (work && work_bytes >= need && (uintptr_t)work % 16 == 0),
              "vh_score: needs %lld bytes of aligned workspace", (long long)need);
@@ -599,7 +601,7 @@ extern "C" int vh_score_backward(const vh_score_desc* d, vh_stream_t stream) {
   const int64_t each = (int64_t)BACK_THREADS * BACK_VECTORS * (d->dtype == VH_F32 ? 4 : 8);
   a.chunks = (uint32_t)((d->vocab + each - 1) / each);
   const int64_t blocks = d->rows * a.chunks;
-  VH_REQUIRE(blocks < (1ll << 31), "vh_score_backward: too many workgroups");
+  VH_REQUIRE(blocks < (1ll << 24), "vh_score_backward: too many rows of such a vocabulary");  // as above
   const dim3 grid((unsigned)blocks);
   hipStream_t s = vh::as_stream(stream);
   if (d->dtype == VH_BF16) hipLaunchKernelGGL(k_score_back<__bf16>, grid, dim3(BACK_THREADS), 0, s, a);

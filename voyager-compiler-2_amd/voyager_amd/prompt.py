@@ -28,7 +28,7 @@ class Packing:
     from 0 on and not falling; equal ones are a sequence of no rows).  Rows
     behind the last sequence pad the batch.  Offsets are read on the device,
     when the packing is made: where they are not so, all rows pad, and
-    :meth:`check` raises.  Fewer than 2^24 tokens."""
+    :meth:`check` raises.  Fewer than 2^24 tokens, and 2^20 sequences."""
 
     def __init__(self, offsets: torch.Tensor, tokens: int):
         if offsets.dim() != 1 or offsets.dtype is not torch.int32 or not offsets.is_cuda or offsets.shape[0] < 1:

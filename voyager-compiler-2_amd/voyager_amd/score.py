@@ -36,8 +36,9 @@ class Scores(NamedTuple):
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Scores:
     """Scores of ``tokens [...]`` (int64) under ``logits [..., vocab]``
-    (bfloat16, float16 or float32; at most 2^20 entries), and the ``top`` best
-    alternatives, at most 64.  Rows with dense entries are read in place.
+    (bfloat16, float16 or float32; at most 2^20 entries, fewer than 2^23 rows),
+    and the ``top`` best alternatives, at most 64.  Rows with dense entries are
+    read in place.
 
     A negative token pads: its row's results are 0, its alternatives -1, and it
     has no gradient.  A token past the vocabulary, which the host does not
