@@ -104,6 +104,23 @@ VH_DEV void pack16(const f32x16& s, uint4 (&p)[2]) {
                       pack2<BF>(s[8 * i + 4], s[8 * i + 5]), pack2<BF>(s[8 * i + 6], s[8 * i + 7]));
 }
 
+// What that left out.
+template <bool BF>
+VH_DEV void rest16(const f32x16& s, const uint4 (&p)[2], uint4 (&low)[2]) {
+  f32x16 rest;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 u = unpack2<BF>(w[j]);
+      rest[8 * i + 2 * j] = s[8 * i + 2 * j] - u[0];
+      rest[8 * i + 2 * j + 1] = s[8 * i + 2 * j + 1] - u[1];
+    }
+  }
+  pack16<BF>(rest, low);
+}
+
 // float16 has no room for the gradients of weights as they come.  They are
 // multiplied by a power of two, a column's own: the largest of its gradients
 // so far lies at 2^11 to 2^15, so that a gradient goes down to 2^-36 of it.
@@ -131,10 +148,20 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
   }
 }
 
+// The rows of long sequences have many keys, whose weights' rounding averages out:
+// their gradients are off by 1.41 to 1.49 times a result's own rounding.  Those of short
+// ones have few, down to two: a weight's rounding is seen in a gradient, and twice
+// in D, which is a sum over the output, that has it as well.  They take D as a sum
+// over the weights instead, and weights and their gradients in two parts of 16
+// bits, each with a product of its own: 1.00 times the rounding.  The second
+// parts take 4 to 12% of the backward pass (us of dq, and of dk and dv, without and
+// with them: 32 sequences of 256, 32 + 8 heads of 128, 103 + 74 and 110 + 85; 20 of
+// 400, heads of 64, 78 + 61 and 82 + 76; 64 of 125, 16 + 16 heads of 64, 40 + 37 and
+// 42 + 40), and D by the keys two fifths of dq's products: too much for long rows.
 // ------------------------------------------------------------------ dq
 constexpr int DQ_KEYS = 64;  // of a tile; a wave takes 32 at a time
 
-template <int D, bool BF, int HALVES, bool CAREFUL>
+template <int D, bool BF, int HALVES, bool SHORT, bool CAREFUL>
 VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   constexpr int BYTES = DQ_KEYS * D * 2;
   const int turn = Halves<D, HALVES>::half();
@@ -158,13 +185,9 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   vl.init(a.v, kv);
   const float scale = a.scale * LOG2E;
   float dot = 0.0f;
-  if (HALVES == 1 && short_sequences(a)) {
-    // A short row's result has weights in it that are rounded and few, and of
-    // that D is more wrong than a weight's own rounding makes its gradient: D as
-    // sum P dP instead, by the keys once more, and over sum P, as the weights
-    // of far scores are off together by what lse in 32 bits is.  (dq's error, in that of the exact one
-    // rounded, by o and by this: a sequence of 40 rows 1.44-1.55 and 1.39-1.49, of
-    // 300 1.43-1.51 and 1.40-1.46.  For long rows it would be two thirds of this pass.)
+  if constexpr (SHORT) {
+    // D as sum P dP, by the keys once more, and over sum P, as the weights of far
+    // scores are off together by what lse in 32 bits is.
     float all = 0.0f;
     for (int key0 = begin; key0 < end; key0 += DQ_KEYS) {
       if (key0 > begin) __syncthreads();
@@ -259,14 +282,17 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
         }
       }
       lift<BF>(ds, up, acc);
-      uint4 p[2];
+      uint4 p[2], low[2];
       pack16<BF>(ds, p);
+      if constexpr (SHORT) rest16<BF>(ds, p, low);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-          const uint4 x = turned_operand<D>(k, sub + 16 * i, c);
-          acc[c] = mfma<BF>(CAREFUL && masked ? finite_part<BF>(x) : x, p[i], acc[c]);
+          uint4 x = turned_operand<D>(k, sub + 16 * i, c);
+          if (CAREFUL && masked) x = finite_part<BF>(x);
+          acc[c] = mfma<BF>(x, p[i], acc[c]);
+          if constexpr (SHORT) acc[c] = mfma<BF>(x, low[i], acc[c]);
         }
     }
   }
@@ -294,7 +320,7 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   return !CAREFUL && in && any_nonfinite(acc);
 }
 
-template <int D, bool BF, int HALVES>
+template <int D, bool BF, int HALVES, bool SHORT>
 __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq(Args a, int item_groups) {
   __shared__ __attribute__((aligned(16))) char s_tiles[HALVES * 4 * DQ_KEYS * D * 2];
   static_assert(sizeof(s_tiles) >= ITEM_BYTES, "the items' lists");
@@ -303,8 +329,8 @@ __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq
     prompt_items(a, blockIdx.x, item_groups, s_tiles);
     return;
   }
-  const bool apart = prompt_dq_block<D, BF, HALVES, false>(a, id, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, HALVES, true>(a, id, s_tiles);
+  const bool apart = prompt_dq_block<D, BF, HALVES, SHORT, false>(a, id, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, HALVES, SHORT, true>(a, id, s_tiles);
 }
 
 // ------------------------------------------------------------- dk and dv
@@ -312,7 +338,7 @@ __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq
 // chunk of the rows that see them.  The scores' products contract over all D: K
 // of the wave's keys stays in registers, and V where they hold both; heads of
 // 128 have the block's V in LDS.
-template <int D, int C, bool BF, bool CAREFUL>
+template <int D, int C, bool BF, bool SHORT, bool CAREFUL>
 VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
   constexpr int BYTES = DK_ROWS * D * 2, PARTS = D / C;
   constexpr bool V_LDS = D == 128;
@@ -398,7 +424,7 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
         s[r] = row >= key && row < past ? s[r] : 0.0f;
       }
     }
-    uint4 p[2];
+    uint4 p[2], low[2];
     if (CAREFUL && masked) {  // a row that holds an infinity or NaN is left out of the products: it makes the keys that it sees NaN
       f32x16 w = s;
 #pragma unroll
@@ -407,15 +433,19 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
         if ((bad_go >> result_row(r) & 1u) && row >= key && row < past) w[r] = __builtin_nanf("");
       }
       pack16<BF>(w, p);
+      if constexpr (SHORT) rest16<BF>(w, p, low);
     } else {
       pack16<BF>(s, p);
+      if constexpr (SHORT) rest16<BF>(s, p, low);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int c = 0; c < C / 32; ++c) {
-        const uint4 x = turned_operand<D>(go, 16 * i, c0 + c);
-        dv[c] = mfma<BF>(CAREFUL && masked ? finite_part<BF>(x) : x, p[i], dv[c]);
+        uint4 x = turned_operand<D>(go, 16 * i, c0 + c);
+        if (CAREFUL && masked) x = finite_part<BF>(x);
+        dv[c] = mfma<BF>(x, p[i], dv[c]);
+        if constexpr (SHORT) dv[c] = mfma<BF>(x, low[i], dv[c]);
       }
     f32x16 ds = {};
 #pragma unroll
@@ -437,12 +467,15 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
     }
     lift<BF>(ds, up, dk);
     pack16<BF>(ds, p);
+    if constexpr (SHORT) rest16<BF>(ds, p, low);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int c = 0; c < C / 32; ++c) {
-        const uint4 x = turned_operand<D>(q, 16 * i, c0 + c);
-        dk[c] = mfma<BF>(CAREFUL && masked ? finite_part<BF>(x) : x, p[i], dk[c]);
+        uint4 x = turned_operand<D>(q, 16 * i, c0 + c);
+        if (CAREFUL && masked) x = finite_part<BF>(x);
+        dk[c] = mfma<BF>(x, p[i], dk[c]);
+        if constexpr (SHORT) dk[c] = mfma<BF>(x, low[i], dk[c]);
       }
   }
   const float k_by = a.scale / up * Lift<BF>::BACK, v_by = Lift<BF>::BACK;
@@ -463,11 +496,11 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
   return !CAREFUL && in && (any_nonfinite(dk) || any_nonfinite(dv));
 }
 
-template <int D, int C, bool BF>
+template <int D, int C, bool BF, bool SHORT>
 __global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dk(Args a) {
   __shared__ __attribute__((aligned(16))) char s_tiles[4 * DK_ROWS * D * 2 + 512 + (D == 128 ? BLOCK * D * 2 : 0)];
-  const bool apart = prompt_dk_block<D, C, BF, false>(a, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dk_block<D, C, BF, true>(a, s_tiles);
+  const bool apart = prompt_dk_block<D, C, BF, SHORT, false>(a, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dk_block<D, C, BF, SHORT, true>(a, s_tiles);
 }
 
 // The sums of a block's items joined, in their order: a thread has 4 channels
@@ -497,14 +530,21 @@ void backward_of(Args a, const int32_t* q_order, const int32_t* k_order, hipStre
   const unsigned blocks = (unsigned)((a.tokens + BLOCK - 1) / BLOCK), groups = a.items ? (blocks + 63) / 64 : 0;
   a.order = q_order;
   const dim3 grid(blocks * a.heads + groups);
-  bool halves = false;
-  if constexpr (D <= 128) {
-    halves = in_halves(a, back_waves_of(D));
-    if (halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 2>), grid, dim3(2 * THREADS), 0, s, a, (int)groups);
+  const dim3 k_grid((a.items ? a.item_count : blocks) * a.kv_heads * (D / C));
+  if (short_sequences(a)) {
+    hipLaunchKernelGGL((k_prompt_dq<D, BF, 1, true>), grid, dim3(THREADS), 0, s, a, (int)groups);
+    a.order = k_order;
+    hipLaunchKernelGGL((k_prompt_dk<D, C, BF, true>), k_grid, dim3(THREADS), 0, s, a);
+  } else {
+    bool halves = false;
+    if constexpr (D <= 128) {
+      halves = in_halves(a, back_waves_of(D));
+      if (halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 2, false>), grid, dim3(2 * THREADS), 0, s, a, (int)groups);
+    }
+    if (!halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 1, false>), grid, dim3(THREADS), 0, s, a, (int)groups);
+    a.order = k_order;
+    hipLaunchKernelGGL((k_prompt_dk<D, C, BF, false>), k_grid, dim3(THREADS), 0, s, a);
   }
-  if (!halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 1>), grid, dim3(THREADS), 0, s, a, (int)groups);
-  a.order = k_order;
-  hipLaunchKernelGGL((k_prompt_dk<D, C, BF>), dim3((a.items ? a.item_count : blocks) * a.kv_heads * (D / C)), dim3(THREADS), 0, s, a);
   if (a.items) hipLaunchKernelGGL((k_prompt_join<D, BF>), dim3(blocks * a.kv_heads, 2 * BLOCK * D / 4 / THREADS), dim3(THREADS), 0, s, a);
 }
 

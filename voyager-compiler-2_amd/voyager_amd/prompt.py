@@ -67,7 +67,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     infinity or NaN may be NaN, and bfloat16 values under 2^-94 may count as 0.
     Scores, weights' sums and results are held in float32; weights, and in the
     backward pass their gradients, are rounded to the values' type for the matrix
-    instructions.  Differentiable once in q, k and v; sums are in a fixed order."""
+    instructions (for short sequences in two parts).  Differentiable once in q, k
+    and v; sums are in a fixed order."""
     given = (q.shape, q.dtype, q.device, k.shape, k.dtype, k.device, v.shape, v.dtype, v.device)
     if given != packing._checked:  # a layer's sizes are mostly those of the layer before
         _check(q, k, v, packing)
