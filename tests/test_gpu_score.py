@@ -253,3 +253,16 @@ def test_in_a_graph_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+FAR = [(d, f) for d in DTYPES for f in (-40000.0, 300.0, 65500.0, 65537.0, 1e6) if f <= torch.finfo(d).max]
+
+
+@pytest.mark.parametrize("dtype,far", FAR)
+def test_far_maxima(dtype, far):
+    """Rows about a far value: exponents are differences, on both sides of 2^16,
+    from which on they are found in another way."""
+    for vocab in (1000, 50257):
+        x = (_logits(3, vocab, torch.float32) + far).clamp(max=torch.finfo(dtype).max).to(dtype)
+        check(x, _tokens(3, vocab), 0)
+        check(x, _tokens(3, vocab), 5)

@@ -17,14 +17,14 @@
 // best are found among the registers as well: what does not reach a bound
 // that `top` entries reach is left out, and the rest is ranked.
 //
-// Bound: with alternatives, and rows for the whole card, vector instructions (4001
-// rows of 32,000 in float16 with the best one: 79 us, 3.2 TB/s); without, memory
-// (2048 rows of 128,000 in bfloat16: 121 us, 4.3 TB/s, and 5 of joining; back, read
-// and written, 162 us, 6.5 TB/s, part of it in the last cache); for few rows the
-// latency of two launches (32 rows of 128,000 with twenty: 11 + 4 us).
+// Bound: with alternatives, and rows for the whole card, what finds them beside the
+// exponentials (4001 rows of 32,000 in float16 with the best one: 62 us, 4.2 TB/s);
+// without, memory (2048 rows of 128,000 in bfloat16: 102 us, 5.1 TB/s; back, read and
+// written, 162 us, 6.5 TB/s, part of it in the last cache); for few rows the latency
+// of two launches (32 rows of 128,000 with twenty: 11 + 4 us).
 //
-// Sums are float32.  Exponents are differences x - m first, so that entries of
-// the type's lowest value, or a row of them, stay in range.
+// Sums are float32.  Exponents are differences x - m, so that entries of the
+// type's lowest value, or a row of them, stay in range.
 #include <hip/hip_runtime.h>
 
 #include "vh_device.h"
@@ -119,6 +119,22 @@ VH_DEV uint4 convert_again(uint4 v) {
   asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
   return v;
 }
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// The largest of 16 bytes' entries; float16 ones two at a time, which bfloat16 has no instruction for.
+template <typename T>
+VH_DEV float largest_entry(uint4 v) {
+  if constexpr (__is_same(T, _Float16)) {
+    const auto two = [](uint32_t w) { return __builtin_bit_cast(f16x2, w); };
+    const f16x2 a = __builtin_elementwise_maximum(__builtin_elementwise_maximum(two(v.x), two(v.y)),
+                                                  __builtin_elementwise_maximum(two(v.z), two(v.w)));
+    return maximum((float)a[0], (float)a[1]);
+  } else {
+    float m = entry<T>(v, 0);
+#pragma unroll
+    for (int j = 1; j < 16 / (int)sizeof(T); ++j) m = maximum(m, entry<T>(v, j));
+    return m;
+  }
+}
 VH_DEV float exponent(float x, float m) { return fmaxf(x - m, FAR) * LOG2E; }  // an entry of -inf has no part
 
 VH_DEV float wave_sum(float v) {
@@ -202,10 +218,11 @@ VH_DEV int count_all(int n, int* s_n) {
   return n;
 }
 
-// NV vectors of 16 bytes a thread.  TOP: with alternatives, for which 96 registers
-// are held (at 80 the compiler spills: 101 us instead of 79, 4001 rows of 32,000).
+// NV vectors of 16 bytes a thread.  TOP: with alternatives.  Three workgroups a CU, for
+// which the compiler spills some registers of these (4001 rows of 32,000 in bfloat16
+// with twenty: 102 us with two, 90 with three; in float16 with one 72 and 69).
 template <typename T, int NV, bool TOP>
-__global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
+__global__ void __launch_bounds__(THREADS, 6) k_score(Args a) {
   constexpr int VEC = 16 / sizeof(T);
   __shared__ float s_f[3][WAVES];
   __shared__ uint32_t s_bound[WAVES];
@@ -239,9 +256,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
   float m = -INF, most[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    most[i] = entry<T>(v[i], 0);
-#pragma unroll
-    for (int j = 1; j < VEC; ++j) most[i] = maximum(most[i], entry<T>(v[i], j));
+    most[i] = largest_entry<T>(v[i]);
     m = maximum(m, most[i]);
   }
   const float lane_most = m;
@@ -253,18 +268,27 @@ __global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) m = maximum(m, s_f[0][w]);
   const float ref = m > -INF && m < INF ? m : 0.0f;
+  // (x - m) log2(e) is one operation less as x log2(e) - m log2(e) (2048 rows of 128,000
+  // in bfloat16: 110 and 102 us): what the second product's rounding leaves out, `off`,
+  // is in all exponents alike, and is taken out of their sums.  Maxima that are too far for
+  // that, and could overflow, are subtracted first.
+  const bool near = __is_same(T, _Float16) || fabsf(ref) < 65536.0f;
+  const float folded = ref * LOG2E, off = near ? __builtin_fmaf(ref, LOG2E, -folded) : 0.0f;
   float l = 0.0f, e = 0.0f;
+  const auto sums = [&](auto power) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint4 w = convert_again(v[i]);
+    for (int i = 0; i < NV; ++i) {
+      const uint4 w = convert_again(v[i]);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float d = exponent(entry<T>(w, j), ref);
-      const float p = exp2_fast(d);
-      l += p;
-      e = __builtin_fmaf(p, d, e);
+      for (int j = 0; j < VEC; ++j) {
+        const float d = power(entry<T>(w, j)), p = exp2_fast(d);
+        l += p;
+        e = __builtin_fmaf(p, d, e);
+      }
     }
-  }
+  };
+  if (near) sums([&](float x) { return fmaxf(__builtin_fmaf(x, LOG2E, -folded), FAR); });
+  else sums([&](float x) { return exponent(x, ref); });
   l = wave_sum(l);
   e = wave_sum(e);
   if (lane == 0) {
@@ -284,6 +308,9 @@ __global__ void __launch_bounds__(THREADS, TOP ? 5 : 6) k_score(Args a) {
       l += s_f[1][w];
       e += s_f[2][w];
     }
+    const float by = exp2f(-off);  // d = (x - m) log2(e) + off: sums of 2^(d - off), and of its products with d - off
+    e = (e - off * l) * by;
+    l *= by;
     if (a.part) {
       float* part = a.part + (row * a.pieces + piece) * 3;
       part[0] = m;
