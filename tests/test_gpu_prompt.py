@@ -67,6 +67,12 @@ def test_long_sequences_are_cut_for_the_keys(dtype, d):
     Case([2900, 40, 3, 500], 2, 1, d, dtype, 77).check()
 
 
+@pytest.mark.parametrize("dtype,d", [(F16, 128), (BF16, 64), (BF16, 256)])
+def test_a_long_sequence_among_many_short_ones(dtype, d):
+    """By the mean they are short; the long one's blocks are cut all the same."""
+    Case([3] * 20 + [1700, 0, 9], 2, 1, d, dtype, 40).check()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_more_blocks_than_are_cut(dtype):
     c = Case([60] * 1500 + [700], 24, 12, 64, dtype, 9)
