@@ -150,8 +150,8 @@ struct Tile {
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// Operand A of 32 rows from row0 on (in bytes from `tile`), channels 16 s ...: a lane's row
-// is lane % 32, its channels 16 s + 8 (lane / 32) ... + 7.
+// Operand A of a tile's 32 rows from row0 on, channels 16 s ...: a lane's row is
+// lane % 32, its channels 16 s + 8 (lane / 32) ... + 7.
 template <int D>
 VH_DEV uint4 rows_operand(const char* tile, int row0, int s) {
   const int lane = threadIdx.x & 63;
@@ -297,7 +297,8 @@ VH_DEV uint32_t bad_rows(const char* tile, int row0) {
   return (uint32_t)all | (uint32_t)(all >> 32);
 }
 
-// Whether two halves of a workgroup share a block, which `short_sequences`, by their mean, never do: where one wave of workgroups
+// Sequences that are short by their mean: back, their few weights take more care.
+// And whether two halves of a workgroup share a block: where one wave of workgroups
 // holds all blocks, so that the longest is the pass, and sequences are long.
 // (us by one and by two, 16 + 4 heads: a prompt of 6000, heads of 64, 150 and 111,
 // of 3000, heads of 128, 85 and 64; four of 775 44 and 36; 16 of 250 22 and 27.
