@@ -189,11 +189,12 @@ VH_DEV i32x4 buffer_of(const char* p, int bytes) {
 VH_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 template <int BYTES>
 VH_DEV void load_to_lds(i32x4 buffer, int offset, uint32_t to) {
-  // a write of M0 is one wait state before the load that uses it
+  // M0 carries the LDS address, an operand, so that the compiler knows what it holds;
+  // its write is one wait state before the load that uses it
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "{m0}"(to) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "{m0}"(to) : "memory");
 }
 // All loads of the workgroup have arrived, and all reads of what is loaded over next are done.
 VH_DEV void arrived() {
