@@ -298,17 +298,40 @@ VH_DEV uint32_t bad_rows(const char* tile, int row0) {
   return (uint32_t)all | (uint32_t)(all >> 32);
 }
 
-// Sequences that are short by their mean: back, their few weights take more care.
-// And whether two halves of a workgroup share a block: where one wave of workgroups
-// holds all blocks, so that the longest is the pass, and sequences are long.
+// Whether two halves of a workgroup share a block: where one wave of workgroups
+// holds all blocks, so that the longest is the pass, and sequences are long by
+// their mean, empty ones among them, as the host knows no more of them.
 // (us by one and by two, 16 + 4 heads: a prompt of 6000, heads of 64, 150 and 111,
 // of 3000, heads of 128, 85 and 64; four of 775 44 and 36; 16 of 250 22 and 27.
 // 32 + 8 heads of 128, 4096: 164 and 176.)
-VH_DEV __host__ bool short_sequences(const Args& a) { return a.tokens < (int64_t)VH_PROMPT_SHORT * a.sequences; }
 inline bool in_halves(const Args& a, int waves) {
   const int64_t blocks = (a.tokens + BLOCK - 1) / BLOCK;
-  return blocks * a.heads <= 256 * waves && !short_sequences(a);
+  return blocks * a.heads <= 256 * waves && a.tokens >= (int64_t)VH_PROMPT_SHORT * a.sequences;
 }
+
+// The rows of the sequences of fewer than VH_PROMPT_SHORT rows that a block of rows
+// has rows of, whose gradients take more care: from the first of the first to the
+// last of the last.  Only the block's first and last sequence can be longer, so
+// they lie one after another, with rows that pad at the end at most.
+struct Run {
+  int from, to;
+  __device__ __forceinline__ bool some() const { return to > from; }
+};
+VH_DEV Run short_run(const Args& a, int row0) {
+  const int end = min(row0 + BLOCK, a.tokens);
+  const int first = a.first[row0], past = a.past[row0], last_first = a.first[end - 1], last_past = a.past[end - 1];
+  if (first > row0) return Run{0, 0};  // all pad
+  int from = first;
+  if (past - first >= VH_PROMPT_SHORT) {
+    // the next one, if there is one, is short, or long and the rest of the block
+    if (past >= end || a.first[past] > past || a.past[past] - past >= VH_PROMPT_SHORT) return Run{0, 0};
+    from = past;
+  }
+  const bool pads = last_first >= end;
+  return Run{from, pads ? end : last_past - last_first < VH_PROMPT_SHORT ? last_past : last_first};
+}
+// Whether these are all of the block's rows.
+VH_DEV bool covers(const Args& a, const Run& run, int row0) { return run.from <= row0 && run.to >= min(row0 + BLOCK, a.tokens); }
 
 template <int D>
 int forward(const Args& a, bool bf16, hipStream_t s);

@@ -209,7 +209,7 @@ extern "C" int vh_prompt_attention_backward(const vh_prompt_desc* d, void* work,
   if (int e = check(d, "vh_prompt_attention_backward")) return e;
   if (d->tokens == 0) return VH_OK;
   if (int e = check_inputs(d, "vh_prompt_attention_backward")) return e;
-  VH_REQUIRE(d->go && (d->o_low || prompt::short_sequences(args_of(d))) && d->gq && d->gk && d->gv, "vh_prompt_attention_backward: null argument");
+  VH_REQUIRE(d->go && d->o_low && d->gq && d->gk && d->gv, "vh_prompt_attention_backward: null argument");
   VH_REQUIRE(rows_aligned(d->go, d->go_st, d->go_sh) && ((uintptr_t)d->gq | (uintptr_t)d->gk | (uintptr_t)d->gv) % 16 == 0,
              "vh_prompt_attention_backward: rows must be aligned to 16 bytes");
   VH_REQUIRE(work && work_bytes >= workspace(d) && (uintptr_t)work % 16 == 0,

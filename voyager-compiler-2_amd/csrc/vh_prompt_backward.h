@@ -150,10 +150,13 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
 
 // The rows of long sequences have many keys, whose weights' rounding averages out:
 // their gradients are off by 1.41 to 1.49 times a result's own rounding.  Those of short
-// ones have few, down to two: a weight's rounding is seen in a gradient, and twice
-// in D, which is a sum over the output, that has it as well.  They take D as a sum
-// over the weights instead, and weights and their gradients in two parts of 16
-// bits, each with a product of its own: 1.00 times the rounding.  The second
+// ones (under VH_PROMPT_SHORT rows) have few, down to two: a weight's rounding is seen
+// in a gradient, and twice in D, which is a sum over the output, that has it as well.
+// They take D as a sum over the weights instead, and weights and their gradients in
+// two parts of 16 bits, each with a product of its own: 1.00 times the rounding.  A
+// block with rows of such sequences does so in the tiles in which they meet their
+// keys, whatever else it holds (two loops: a choice in the loop costs registers, and
+// spills in both cases).  The second
 // parts take 4 to 12% of the backward pass (us of dq, and of dk and dv, without and
 // with them: 32 sequences of 256, 32 + 8 heads of 128, 103 + 74 and 110 + 85; 20 of
 // 400, heads of 64, 78 + 61 and 82 + 76; 64 of 125, 16 + 16 heads of 64, 40 + 37 and
@@ -161,7 +164,7 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
 // ------------------------------------------------------------------ dq
 constexpr int DQ_KEYS = 64;  // of a tile; a wave takes 32 at a time
 
-template <int D, bool BF, int HALVES, bool SHORT, bool CAREFUL>
+template <int D, bool BF, int HALVES, bool CAREFUL>
 VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   constexpr int BYTES = DQ_KEYS * D * 2;
   const int turn = Halves<D, HALVES>::half();
@@ -184,39 +187,9 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   kl.init(a.k, kv);
   vl.init(a.v, kv);
   const float scale = a.scale * LOG2E;
+  const Run of = short_run(a, row0);
   float dot = 0.0f;
-  if constexpr (SHORT) {
-    // D as sum P dP, by the keys once more, and over sum P, as the weights of far
-    // scores are off together by what lse in 32 bits is.
-    float all = 0.0f;
-    for (int key0 = begin; key0 < end; key0 += DQ_KEYS) {
-      if (key0 > begin) __syncthreads();
-      kl.load(tiles, key0, a.tokens);
-      vl.load(tiles + 2 * BYTES, key0, a.tokens);
-      arrived();
-#pragma unroll
-      for (int sub = 0; sub < DQ_KEYS; sub += 32) {
-        const int key = key0 + sub;
-        if (key >= wave0 + 32 || key + 32 <= wave_first) continue;
-        f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(tiles, sub, i), q[i], s);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) dp = mfma<BF>(rows_operand<D>(tiles + 2 * BYTES, sub, i), go[i], dp);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = key + result_row(r) + 4 * half;
-          const float p = j >= first && j <= row ? exp2_fast(__builtin_fmaf(s[r], scale, -lse)) : 0.0f;
-          all += p;
-          dot += p > 0.0f ? p * dp[r] : 0.0f;
-        }
-      }
-    }
-    dot = sum_halves(dot);
-    all = sum_halves(all);
-    dot = all == 0.0f ? dot : dot / all;
-    __syncthreads();  // the tiles are loaded over next
-  } else {
+  if (!covers(a, of, row0)) {
     uint4 o[D / 16];
     const Tensor out{a.o, (int64_t)a.heads * D, D}, low{a.o_low, (int64_t)a.heads * D, D};
 #pragma unroll
@@ -235,6 +208,39 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
     }
     dot = sum_halves(dot);
   }
+  if (of.some()) {
+    // D as sum P dP, by the short sequences' keys once more (each half of a workgroup by
+    // all of them), and over sum P, as the weights of far scores are off together by
+    // what lse in 32 bits is.
+    float by_weights = 0.0f, all = 0.0f;
+    for (int key0 = of.from; key0 < end; key0 += DQ_KEYS) {
+      if (key0 > of.from) __syncthreads();
+      kl.load(tiles, key0, a.tokens);
+      vl.load(tiles + 2 * BYTES, key0, a.tokens);
+      arrived();
+#pragma unroll
+      for (int sub = 0; sub < DQ_KEYS; sub += 32) {
+        const int key = key0 + sub;
+        if (key >= wave0 + 32 || key + 32 <= wave_first) continue;
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(tiles, sub, i), q[i], s);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dp = mfma<BF>(rows_operand<D>(tiles + 2 * BYTES, sub, i), go[i], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = key + result_row(r) + 4 * half;
+          const float p = j >= first && j <= row ? exp2_fast(__builtin_fmaf(s[r], scale, -lse)) : 0.0f;
+          all += p;
+          by_weights += p > 0.0f ? p * dp[r] : 0.0f;
+        }
+      }
+    }
+    by_weights = sum_halves(by_weights);
+    all = sum_halves(all);
+    if (row >= of.from && row < of.to) dot = all == 0.0f ? by_weights : by_weights / all;
+    __syncthreads();  // the tiles are loaded over next
+  }
   if (in && turn == 0) {
     float* to = a.rows + (int64_t)head * 2 * a.tokens + row;
     if (half == 0) to[0] = lse;
@@ -244,56 +250,64 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) acc[c] = f32x16{};
   float up = Lift<BF>::FIRST;
-  const int first_key = begin + turn * DQ_KEYS;
-  if (first_key < end) {
-    kl.load(tiles, first_key, a.tokens);
-    vl.load(tiles + 2 * BYTES, first_key, a.tokens);
-  }
-  int at = 0;
-  for (int key0 = first_key; key0 - turn * DQ_KEYS < end; key0 += HALVES * DQ_KEYS, at ^= 1) {
-    arrived();
-    if (key0 + HALVES * DQ_KEYS < end) {
-      kl.load(tiles + (at ^ 1) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
-      vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
+  // the tiles before the short sequences' keys, and the rest, which take two parts: two loops
+  const int parted = of.some() ? begin + max(of.from - begin, 0) / DQ_KEYS * DQ_KEYS : end;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const bool two = part > 0;
+    const int from = two ? parted : begin, to = two ? end : parted;
+    if (two) __syncthreads();  // the tiles are loaded over next
+    const int first_key = from + turn * DQ_KEYS;
+    if (first_key < to) {
+      kl.load(tiles, first_key, a.tokens);
+      vl.load(tiles + 2 * BYTES, first_key, a.tokens);
     }
-    if (HALVES > 1 && key0 >= end) continue;
-    const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
-#pragma unroll
-    for (int sub = 0; sub < DQ_KEYS; sub += 32) {
-      const int key = key0 + sub;
-      if (key >= wave0 + 32 || key + 32 <= wave_first) continue;
-      const bool masked = key + 32 > wave0 + 1 || key < wave_last_first;
-      f32x16 s = {}, ds = {};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(k, sub, i), q[i], s);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) ds = mfma<BF>(rows_operand<D>(v, sub, i), go[i], ds);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(__builtin_fmaf(s[r], scale, -lse)) * (ds[r] - dot);
-      uint32_t bad = 0u;
-      if (CAREFUL && masked) bad = bad_rows<D, BF>(k, sub) >> (4 * half);
-      if (masked) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = key + result_row(r) + 4 * half;
-          // a key that holds an infinity or NaN is left out of the product: it makes its rows NaN
-          const float seen = CAREFUL && (bad >> result_row(r) & 1u) ? __builtin_nanf("") : ds[r];
-          ds[r] = j >= first && j <= row ? seen : 0.0f;
-        }
+    int at = 0;
+    for (int key0 = first_key; key0 - turn * DQ_KEYS < to; key0 += HALVES * DQ_KEYS, at ^= 1) {
+      arrived();
+      if (key0 + HALVES * DQ_KEYS < to) {
+        kl.load(tiles + (at ^ 1) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
+        vl.load(tiles + (2 + (at ^ 1)) * BYTES, key0 + HALVES * DQ_KEYS, a.tokens);
       }
-      lift<BF>(ds, up, acc);
-      uint4 p[2], low[2];
-      pack16<BF>(ds, p);
-      if constexpr (SHORT) rest16<BF>(ds, p, low);
+      if (HALVES > 1 && key0 >= to) continue;
+      const char *k = tiles + at * BYTES, *v = tiles + (2 + at) * BYTES;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int sub = 0; sub < DQ_KEYS; sub += 32) {
+        const int key = key0 + sub;
+        if (key >= wave0 + 32 || key + 32 <= wave_first) continue;
+        const bool masked = key + 32 > wave0 + 1 || key < wave_last_first;
+        f32x16 s = {}, ds = {};
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint4 x = turned_operand<D>(k, sub + 16 * i, c);
-          if (CAREFUL && masked) x = finite_part<BF>(x);
-          acc[c] = mfma<BF>(x, p[i], acc[c]);
-          if constexpr (SHORT) acc[c] = mfma<BF>(x, low[i], acc[c]);
+        for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(k, sub, i), q[i], s);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) ds = mfma<BF>(rows_operand<D>(v, sub, i), go[i], ds);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = exp2_fast(__builtin_fmaf(s[r], scale, -lse)) * (ds[r] - dot);
+        uint32_t bad = 0u;
+        if (CAREFUL && masked) bad = bad_rows<D, BF>(k, sub) >> (4 * half);
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = key + result_row(r) + 4 * half;
+            // a key that holds an infinity or NaN is left out of the product: it makes its rows NaN
+            const float seen = CAREFUL && (bad >> result_row(r) & 1u) ? __builtin_nanf("") : ds[r];
+            ds[r] = j >= first && j <= row ? seen : 0.0f;
+          }
         }
+        lift<BF>(ds, up, acc);
+        uint4 p[2], low[2];
+        pack16<BF>(ds, p);
+        if (two) rest16<BF>(ds, p, low);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint4 x = turned_operand<D>(k, sub + 16 * i, c);
+            if (CAREFUL && masked) x = finite_part<BF>(x);
+            acc[c] = mfma<BF>(x, p[i], acc[c]);
+            if (two) acc[c] = mfma<BF>(x, low[i], acc[c]);
+          }
+      }
     }
   }
   if constexpr (HALVES > 1) {
@@ -320,7 +334,7 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   return !CAREFUL && in && any_nonfinite(acc);
 }
 
-template <int D, bool BF, int HALVES, bool SHORT>
+template <int D, bool BF, int HALVES>
 __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq(Args a, int item_groups) {
   __shared__ __attribute__((aligned(16))) char s_tiles[HALVES * 4 * DQ_KEYS * D * 2];
   static_assert(sizeof(s_tiles) >= ITEM_BYTES, "the items' lists");
@@ -329,8 +343,8 @@ __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq
     prompt_items(a, blockIdx.x, item_groups, s_tiles);
     return;
   }
-  const bool apart = prompt_dq_block<D, BF, HALVES, SHORT, false>(a, id, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, HALVES, SHORT, true>(a, id, s_tiles);
+  const bool apart = prompt_dq_block<D, BF, HALVES, false>(a, id, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dq_block<D, BF, HALVES, true>(a, id, s_tiles);
 }
 
 // ------------------------------------------------------------- dk and dv
@@ -338,22 +352,13 @@ __global__ void __launch_bounds__(HALVES* THREADS, back_waves_of(D)) k_prompt_dq
 // chunk of the rows that see them.  The scores' products contract over all D: K
 // of the wave's keys stays in registers, and V where they hold both; heads of
 // 128 have the block's V in LDS.
-template <int D, int C, bool BF, bool SHORT, bool CAREFUL>
-VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
+template <int D, int C, bool BF, bool CAREFUL>
+VH_DEV bool prompt_dk_block(const Args& a, const int4& item, char* tiles) {
   constexpr int BYTES = DK_ROWS * D * 2, PARTS = D / C;
   constexpr bool V_LDS = D == 128;
-  const int rank = blockIdx.x / (a.kv_heads * PARTS), spread = blockIdx.x - rank * (a.kv_heads * PARTS);
+  const int spread = blockIdx.x % (a.kv_heads * PARTS);
   const int kv = spread % a.kv_heads, c0 = spread / a.kv_heads * (C / 32);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int4 item = make_int4(0, 0, 0, -1);
-  if (a.items) {
-    item = a.items[rank];
-    if (item.x < 0) return false;
-  } else {
-    item.x = a.order[rank];
-    item.y = item.x * BLOCK;
-    item.z = a.past[min(item.y + BLOCK, a.tokens) - 1];
-  }
   const int key0 = item.x * BLOCK, begin = item.y, end = item.z;
   const int wave0 = key0 + 32 * wave, key = wave0 + (lane & 31), half = lane >> 5;
   const bool in = key < a.tokens;
@@ -368,115 +373,125 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
 #pragma unroll
   for (int c = 0; c < C / 32; ++c) dk[c] = dv[c] = f32x16{};
   float up = Lift<BF>::FIRST;
-  Loader<D, DK_ROWS> ql, gl;
-  const int rounds = end > begin ? (end - begin + DK_ROWS - 1) / DK_ROWS : 0, all = rounds * a.group;
-  int next_head = kv * a.group, next_row = begin;
-  ql.init(a.q, next_head);
-  gl.init(a.go, next_head);
-  const auto load_next = [&](int to) {
-    ql.load(tiles + to * BYTES, next_row, a.tokens);
-    gl.load(tiles + (2 + to) * BYTES, next_row, a.tokens);
-    if (wave == 0) {
-      const i32x4 r = buffer_of((const char*)(a.rows + (int64_t)next_head * 2 * a.tokens), a.tokens * 8);
-      load_to_lds<4>(r, ((lane >> 5) * a.tokens + next_row + (lane & 31)) * 4,
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(s_rows + to * 256)));
-    }
-    next_row += DK_ROWS;
-    if (next_row >= end) {
-      next_row = begin;
-      ++next_head;
-      ql.base += a.q.sh * 2;
-      gl.base += a.go.sh * 2;
-    }
-  };
-  if (all > 0) {  // nothing is left on its way to LDS by a workgroup that ends
-    if constexpr (V_LDS) {
+  if constexpr (V_LDS) {
+    if (end > begin) {  // nothing is left on its way to LDS by a workgroup that ends
       Loader<D, BLOCK> vl;
       vl.init(a.v, kv);
       vl.load(s_v, key0, a.tokens);
     }
-    load_next(0);
   }
-  int at = 0, row0 = begin;
-  for (int n = 0; n < all; ++n, at ^= 1) {
-    arrived();
-    if (n + 1 < all) load_next(at ^ 1);
-    const int first_row = row0;
-    row0 = row0 + DK_ROWS >= end ? begin : row0 + DK_ROWS;
-    if (first_row + DK_ROWS <= wave0 || first_row >= wave_last_past) continue;
-    const bool masked = first_row < wave0 + 31 || first_row + DK_ROWS > wave_past;
-    const char *q = tiles + at * BYTES, *go = tiles + (2 + at) * BYTES;
-    const float* of = (const float*)(s_rows + at * 256) + 4 * half;
-    f32x16 s = {};
+  // the tiles of short sequences' rows, which take two parts, and the rest: two loops
+  const int parted = min(begin + (max(short_run(a, key0).to - begin, 0) + DK_ROWS - 1) / DK_ROWS * DK_ROWS, end);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(q, 0, i), k[i], s);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], scale, Lift<BF>::LOG - of[result_row(r)]));
-    uint32_t bad_go = 0u, bad_q = 0u;
-    if (CAREFUL && masked) {
-      bad_go = bad_rows<D, BF>(go, 0) >> (4 * half);
-      bad_q = bad_rows<D, BF>(q, 0) >> (4 * half);
-    }
-    if (masked) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = first_row + result_row(r) + 4 * half;
-        s[r] = row >= key && row < past ? s[r] : 0.0f;
+  for (int part = 0; part < 2; ++part) {
+    const bool two = part == 0;
+    const int from = two ? begin : parted, to = two ? parted : end;
+    if (!two) __syncthreads();  // the tiles are loaded over next
+    Loader<D, DK_ROWS> ql, gl;
+    const int rounds = to > from ? (to - from + DK_ROWS - 1) / DK_ROWS : 0, all = rounds * a.group;
+    int next_head = kv * a.group, next_row = from;
+    ql.init(a.q, next_head);
+    gl.init(a.go, next_head);
+    const auto load_next = [&](int at) __attribute__((always_inline)) {
+      ql.load(tiles + at * BYTES, next_row, a.tokens);
+      gl.load(tiles + (2 + at) * BYTES, next_row, a.tokens);
+      if (wave == 0) {
+        const i32x4 r = buffer_of((const char*)(a.rows + (int64_t)next_head * 2 * a.tokens), a.tokens * 8);
+        load_to_lds<4>(r, ((lane >> 5) * a.tokens + next_row + (lane & 31)) * 4,
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(s_rows + at * 256)));
       }
-    }
-    uint4 p[2], low[2];
-    if (CAREFUL && masked) {  // a row that holds an infinity or NaN is left out of the products: it makes the keys that it sees NaN
+      next_row += DK_ROWS;
+      if (next_row >= to) {
+        next_row = from;
+        ++next_head;
+        ql.base += a.q.sh * 2;
+        gl.base += a.go.sh * 2;
+      }
+    };
+    if (all > 0) load_next(0);
+    int at = 0, row0 = from;
+    for (int n = 0; n < all; ++n, at ^= 1) {
+      arrived();
+      if (n + 1 < all) load_next(at ^ 1);
+      const int first_row = row0;
+      row0 = row0 + DK_ROWS >= to ? from : row0 + DK_ROWS;
+      if (first_row + DK_ROWS <= wave0 || first_row >= wave_last_past) continue;
+      const bool masked = first_row < wave0 + 31 || first_row + DK_ROWS > wave_past;
+      const char *q = tiles + at * BYTES, *go = tiles + (2 + at) * BYTES;
+      const float* stats = (const float*)(s_rows + at * 256) + 4 * half;
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(q, 0, i), k[i], s);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], scale, Lift<BF>::LOG - stats[result_row(r)]));
+      uint32_t bad_go = 0u, bad_q = 0u;
+      if (CAREFUL && masked) {
+        bad_go = bad_rows<D, BF>(go, 0) >> (4 * half);
+        bad_q = bad_rows<D, BF>(q, 0) >> (4 * half);
+      }
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = first_row + result_row(r) + 4 * half;
+          s[r] = row >= key && row < past ? s[r] : 0.0f;
+        }
+      }
       f32x16 w = s;
+      if (CAREFUL && masked) {  // a row that holds an infinity or NaN is left out of the products: it makes the keys that it sees NaN
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = first_row + result_row(r) + 4 * half;
-        if ((bad_go >> result_row(r) & 1u) && row >= key && row < past) w[r] = __builtin_nanf("");
+        for (int r = 0; r < 16; ++r) {
+          const int row = first_row + result_row(r) + 4 * half;
+          if ((bad_go >> result_row(r) & 1u) && row >= key && row < past) w[r] = __builtin_nanf("");
+        }
       }
-      pack16<BF>(w, p);
-      if constexpr (SHORT) rest16<BF>(w, p, low);
-    } else {
-      pack16<BF>(s, p);
-      if constexpr (SHORT) rest16<BF>(s, p, low);
+      {
+        uint4 p[2], low[2];
+        pack16<BF>(w, p);
+        if (two) rest16<BF>(w, p, low);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < C / 32; ++c) {
+            uint4 x = turned_operand<D>(go, 16 * i, c0 + c);
+            if (CAREFUL && masked) x = finite_part<BF>(x);
+            dv[c] = mfma<BF>(x, p[i], dv[c]);
+            if (two) dv[c] = mfma<BF>(x, low[i], dv[c]);
+          }
+      }
+      f32x16 ds = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint4 of_v;
+        if constexpr (V_LDS) of_v = rows_operand<D>(s_v, 32 * wave, i);
+        else of_v = v[i];
+        ds = mfma<BF>(rows_operand<D>(go, 0, i), of_v, ds);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - stats[32 + result_row(r)]);
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = first_row + result_row(r) + 4 * half;
+          const float seen = CAREFUL && (bad_q >> result_row(r) & 1u) ? __builtin_nanf("") : ds[r];
+          ds[r] = row >= key && row < past ? seen : 0.0f;
+        }
+      }
+      lift<BF>(ds, up, dk);
+      {
+        uint4 p[2], low[2];
+        pack16<BF>(ds, p);
+        if (two) rest16<BF>(ds, p, low);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < C / 32; ++c) {
+            uint4 x = turned_operand<D>(q, 16 * i, c0 + c);
+            if (CAREFUL && masked) x = finite_part<BF>(x);
+            dk[c] = mfma<BF>(x, p[i], dk[c]);
+            if (two) dk[c] = mfma<BF>(x, low[i], dk[c]);
+          }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < C / 32; ++c) {
-        uint4 x = turned_operand<D>(go, 16 * i, c0 + c);
-        if (CAREFUL && masked) x = finite_part<BF>(x);
-        dv[c] = mfma<BF>(x, p[i], dv[c]);
-        if constexpr (SHORT) dv[c] = mfma<BF>(x, low[i], dv[c]);
-      }
-    f32x16 ds = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      uint4 of_v;
-      if constexpr (V_LDS) of_v = rows_operand<D>(s_v, 32 * wave, i);
-      else of_v = v[i];
-      ds = mfma<BF>(rows_operand<D>(go, 0, i), of_v, ds);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - of[32 + result_row(r)]);
-    if (masked) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = first_row + result_row(r) + 4 * half;
-        const float seen = CAREFUL && (bad_q >> result_row(r) & 1u) ? __builtin_nanf("") : ds[r];
-        ds[r] = row >= key && row < past ? seen : 0.0f;
-      }
-    }
-    lift<BF>(ds, up, dk);
-    pack16<BF>(ds, p);
-    if constexpr (SHORT) rest16<BF>(ds, p, low);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < C / 32; ++c) {
-        uint4 x = turned_operand<D>(q, 16 * i, c0 + c);
-        if (CAREFUL && masked) x = finite_part<BF>(x);
-        dk[c] = mfma<BF>(x, p[i], dk[c]);
-        if constexpr (SHORT) dk[c] = mfma<BF>(x, low[i], dk[c]);
-      }
   }
   const float k_by = a.scale / up * Lift<BF>::BACK, v_by = Lift<BF>::BACK;
   if (item.w < 0) {
@@ -496,11 +511,21 @@ VH_DEV bool prompt_dk_block(const Args& a, char* tiles) {
   return !CAREFUL && in && (any_nonfinite(dk) || any_nonfinite(dv));
 }
 
-template <int D, int C, bool BF, bool SHORT>
+template <int D, int C, bool BF>
 __global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dk(Args a) {
   __shared__ __attribute__((aligned(16))) char s_tiles[4 * DK_ROWS * D * 2 + 512 + (D == 128 ? BLOCK * D * 2 : 0)];
-  const bool apart = prompt_dk_block<D, C, BF, SHORT, false>(a, s_tiles);
-  if (__syncthreads_or(apart)) prompt_dk_block<D, C, BF, SHORT, true>(a, s_tiles);
+  const int rank = blockIdx.x / (a.kv_heads * (D / C));
+  int4 item = make_int4(0, 0, 0, -1);
+  if (a.items) {
+    item = a.items[rank];
+    if (item.x < 0) return;
+  } else {
+    item.x = a.order[rank];
+    item.y = item.x * BLOCK;
+    item.z = a.past[min(item.y + BLOCK, a.tokens) - 1];
+  }
+  const bool apart = prompt_dk_block<D, C, BF, false>(a, item, s_tiles);
+  if (__syncthreads_or(apart)) prompt_dk_block<D, C, BF, true>(a, item, s_tiles);
 }
 
 // The sums of a block's items joined, in their order: a thread has 4 channels
@@ -531,20 +556,14 @@ void backward_of(Args a, const int32_t* q_order, const int32_t* k_order, hipStre
   a.order = q_order;
   const dim3 grid(blocks * a.heads + groups);
   const dim3 k_grid((a.items ? a.item_count : blocks) * a.kv_heads * (D / C));
-  if (short_sequences(a)) {
-    hipLaunchKernelGGL((k_prompt_dq<D, BF, 1, true>), grid, dim3(THREADS), 0, s, a, (int)groups);
-    a.order = k_order;
-    hipLaunchKernelGGL((k_prompt_dk<D, C, BF, true>), k_grid, dim3(THREADS), 0, s, a);
-  } else {
-    bool halves = false;
-    if constexpr (D <= 128) {
-      halves = in_halves(a, back_waves_of(D));
-      if (halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 2, false>), grid, dim3(2 * THREADS), 0, s, a, (int)groups);
-    }
-    if (!halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 1, false>), grid, dim3(THREADS), 0, s, a, (int)groups);
-    a.order = k_order;
-    hipLaunchKernelGGL((k_prompt_dk<D, C, BF, false>), k_grid, dim3(THREADS), 0, s, a);
+  bool halves = false;
+  if constexpr (D <= 128) {
+    halves = in_halves(a, back_waves_of(D));
+    if (halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 2>), grid, dim3(2 * THREADS), 0, s, a, (int)groups);
   }
+  if (!halves) hipLaunchKernelGGL((k_prompt_dq<D, BF, 1>), grid, dim3(THREADS), 0, s, a, (int)groups);
+  a.order = k_order;
+  hipLaunchKernelGGL((k_prompt_dk<D, C, BF>), k_grid, dim3(THREADS), 0, s, a);
   if (a.items) hipLaunchKernelGGL((k_prompt_join<D, BF>), dim3(blocks * a.kv_heads, 2 * BLOCK * D / 4 / THREADS), dim3(THREADS), 0, s, a);
 }
 

@@ -208,7 +208,9 @@ VH_DEV bool prompt_block(const Args& a, char* lds) {
   // Divided by the sum of the rounded weights, a row whose weight is one key's has
   // none of its rounding, in its result as in the gradients' D.
   const float by = f.rounded == 0.0f ? 0.0f : 1.0f / f.rounded;
-  store_columns<D, D, BF>(a.o, a.o_low, a.heads, head, row, in, 0, f.acc, by);
+  // back, long sequences' rows read what is left out of theirs
+  void* low = a.o_low && !covers(a, short_run(a, row0), row0) ? a.o_low : nullptr;
+  store_columns<D, D, BF>(a.o, low, a.heads, head, row, in, 0, f.acc, by);
   if (in && lane < 32)
     a.lse[(int64_t)row * a.heads + head] = f.sum == 0.0f ? -__builtin_inff() : (f.ref - Range<BF>::LIFT + log2f(f.sum)) * LN2;
   // a row whose sum is not finite sees something that is not

@@ -17,7 +17,7 @@ from ._lib import check, dtype_code, load, no_tangents, once, ptr, stream_on
 
 MAX_TOKENS = (1 << 24) - 1
 DIMS = (64, 128, 256)
-SHORT = 512  # ``VH_PROMPT_SHORT``
+SHORT = 512  # ``VH_PROMPT_SHORT``: sequences of fewer rows take more care in the backward pass
 #: ``vh_prompt_desc``
 PROMPT = struct.Struct("@QqqQqqQqqQQQQQqqQQQqfiiiii")
 
@@ -67,7 +67,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     infinity or NaN may be NaN, and bfloat16 values under 2^-94 may count as 0.
     Scores, weights' sums and results are held in float32; weights, and in the
     backward pass their gradients, are rounded to the values' type for the matrix
-    instructions (for short sequences in two parts).  Differentiable once in q, k
+    instructions (for sequences of fewer than 512 rows in two parts).  Differentiable once in q, k
     and v; sums are in a fixed order."""
     given = (q.shape, q.dtype, q.device, k.shape, k.dtype, k.device, v.shape, v.dtype, v.device)
     if given != packing._checked:  # a layer's sizes are mostly those of the layer before
@@ -116,8 +116,8 @@ def _desc(q, k, v, packing, o, low, lse, scale, go=None, grads=(0, 0, 0)):
 def _forward(q, k, v, packing, scale, train=False):
     q, k, v = _rows(q), _rows(k), _rows(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    # what the rounding leaves out: the backward pass takes sums over a long row's result, in which it would be seen
-    low = torch.empty_like(o, dtype=torch.bfloat16) if train and packing.tokens >= SHORT * packing.sequences else None
+    # what the rounding leaves out: the backward pass takes sums over a long sequence's results, in which it would be seen
+    low = torch.empty_like(o, dtype=torch.bfloat16) if train else None
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     st = load().vh_prompt_attention(_desc(q, k, v, packing, o, low, lse, scale), stream_on(q.device))
     if st:
