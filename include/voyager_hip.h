@@ -905,7 +905,9 @@ int vh_packing(const int32_t* offsets, int64_t sequences, int64_t tokens, int32_
  * contiguous; lse [tokens, heads] float32, the logarithm of the sum of
  * exponentials; rows that pad give 0 and -inf.  o_low (NULL: not wanted): for the
  * backward pass, what the rounding of o left out, in bfloat16, laid out as o, of
- * sequences of VH_PROMPT_SHORT rows and more (the rest is not defined).
+ * sequences of VH_PROMPT_SHORT rows and more (the rest is not defined); lse is
+ * then twice as long, and its second half, [heads, tokens], what the weights'
+ * exponents of the backward pass take more than lse says.
  * The backward pass reads q, k, v, o, o_low, lse and the result's gradient go
  * (strides as above) and writes gq, gk, gv, contiguous, in a fixed order of sums.  work:
  * vh_prompt_attention_workspace_bytes(desc) bytes, 16-byte aligned. */

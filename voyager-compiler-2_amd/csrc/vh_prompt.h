@@ -65,6 +65,7 @@ struct Args {
   const int32_t *first, *past, *order;  // of rows, keys, and of this pass's blocks
   void *o, *o_low, *gq, *gk, *gv;
   float* lse;         // [tokens, heads]
+  float* rest;        // for the backward pass: [heads, tokens], what a weight's exponent, less lse, takes more
   float* rows;        // backward: [heads, 2, tokens], lse log2(e) and D
   // backward, where key blocks are cut into items:
   int4* items;        // [item_count]: block (-1: none), first row, row after the last, slot of its sums (-1: they are the result)
@@ -74,6 +75,15 @@ struct Args {
   float scale;
   int tokens, sequences, heads, kv_heads, group;
 };
+
+// lse in units of log2, as the backward pass takes it from the natural one.
+// Rounded in 32 bits it is off by what, for far scores, is seen in the weights
+// (2^-10 of them at 2^13): `rest` is what is missing, and the lift of weights (Lift).
+VH_DEV float log2_units(float lse) {
+#pragma clang fp contract(off)
+  return lse * LOG2E;
+}
+constexpr float weights_lift(bool bf16) { return bf16 ? 0.0f : 15.0f; }
 
 // Where blocks are few for the card, or one is long beside them, two halves of
 // a workgroup take a block's tiles in turn, and join through LDS: the longest

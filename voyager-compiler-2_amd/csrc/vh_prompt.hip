@@ -128,6 +128,7 @@ Args args_of(const vh_prompt_desc* d) {
   a.gk = d->gk;
   a.gv = d->gv;
   a.lse = d->lse;
+  a.rest = d->o_low ? d->lse + d->tokens * d->heads : nullptr;
   a.scale = d->scale;
   a.tokens = (int)d->tokens;
   a.sequences = d->sequences;

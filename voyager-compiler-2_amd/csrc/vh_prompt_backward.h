@@ -16,6 +16,7 @@
 namespace prompt {
 
 constexpr int DK_ROWS = 32;                      // of a tile of the keys' pass
+constexpr int STATS = 512;                       // bytes of its rows' numbers
 // Tiles of an item at least, but for a block's last: its sums are written and
 // read, 128 KB a head of 128.
 constexpr int LEAST = 2 * BLOCK / DK_ROWS;
@@ -127,7 +128,7 @@ VH_DEV void rest16(const f32x16& s, const uint4 (&p)[2], uint4 (&low)[2]) {
 // Weights, at most 1, are lifted by 2^15.
 template <bool BF>
 struct Lift {
-  static constexpr float LOG = BF ? 0.0f : 15.0f, BACK = BF ? 1.0f : 0x1p-15f, FIRST = BF ? 1.0f : 0x1p100f;
+  static constexpr float LOG = weights_lift(BF), BACK = BF ? 1.0f : 0x1p-15f, FIRST = BF ? 1.0f : 0x1p100f;
 };
 template <bool BF, int N>
 VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
@@ -182,7 +183,9 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
   load_columns<D>(a.go, head, wave0, a.tokens, go);
   // D, and lse log2(e), which is inf where a row sees nothing, so that its weights are 0: for the keys' pass as well
   const float natural = in ? a.lse[(int64_t)row * a.heads + head] : -__builtin_inff();
-  const float lse = natural == -__builtin_inff() ? __builtin_inff() : natural * LOG2E;
+  const float lse = natural == -__builtin_inff() ? __builtin_inff() : log2_units(natural);
+  // weights are off together by what lse leaves out, and dq is a sum over them
+  const float unit = in ? exp2_fast(a.rest[(int64_t)head * a.tokens + row] - Lift<BF>::LOG) : 1.0f;
   Loader<D, DQ_KEYS> kl, vl;
   kl.init(a.k, kv);
   vl.init(a.v, kv);
@@ -330,7 +333,7 @@ VH_DEV bool prompt_dq_block(const Args& a, int id, char* lds) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[c][r] = acc[c][r] * mine + to[(16 * c + r) * 64] * by;
   }
-  store_columns<D, D, BF>(a.gq, nullptr, a.heads, head, row, in, 0, acc, a.scale / up);
+  store_columns<D, D, BF>(a.gq, nullptr, a.heads, head, row, in, 0, acc, a.scale / up * unit);
   return !CAREFUL && in && any_nonfinite(acc);
 }
 
@@ -364,7 +367,7 @@ VH_DEV bool prompt_dk_block(const Args& a, const int4& item, char* tiles) {
   const bool in = key < a.tokens;
   const int past = in ? a.past[key] : key;  // the row after the last that sees the key
   const int wave_past = __builtin_amdgcn_readlane(past, 0), wave_last_past = __builtin_amdgcn_readlane(past, 31);
-  char *s_rows = tiles + 4 * BYTES, *s_v = s_rows + 512;  // lse and D of a tile's rows; V
+  char *s_rows = tiles + 4 * BYTES, *s_v = s_rows + 2 * STATS;  // lse, D and the rest of lse of a tile's rows; V
   uint4 k[D / 16], v[V_LDS ? 1 : D / 16];
   load_columns<D>(a.k, kv, wave0, a.tokens, k);
   if constexpr (!V_LDS) load_columns<D>(a.v, kv, wave0, a.tokens, v);
@@ -398,7 +401,11 @@ VH_DEV bool prompt_dk_block(const Args& a, const int4& item, char* tiles) {
       if (wave == 0) {
         const i32x4 r = buffer_of((const char*)(a.rows + (int64_t)next_head * 2 * a.tokens), a.tokens * 8);
         load_to_lds<4>(r, ((lane >> 5) * a.tokens + next_row + (lane & 31)) * 4,
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(s_rows + at * 256)));
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(s_rows + at * STATS)));
+      }
+      if (wave == 1) {
+        const i32x4 r = buffer_of((const char*)(a.rest + (int64_t)next_head * a.tokens), a.tokens * 4);
+        load_to_lds<4>(r, (next_row + lane) * 4, (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(s_rows + at * STATS + 256)));
       }
       next_row += DK_ROWS;
       if (next_row >= to) {
@@ -418,12 +425,12 @@ VH_DEV bool prompt_dk_block(const Args& a, const int4& item, char* tiles) {
       if (first_row + DK_ROWS <= wave0 || first_row >= wave_last_past) continue;
       const bool masked = first_row < wave0 + 31 || first_row + DK_ROWS > wave_past;
       const char *q = tiles + at * BYTES, *go = tiles + (2 + at) * BYTES;
-      const float* stats = (const float*)(s_rows + at * 256) + 4 * half;
+      const float* stats = (const float*)(s_rows + at * STATS) + 4 * half;
       f32x16 s = {};
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows_operand<D>(q, 0, i), k[i], s);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], scale, Lift<BF>::LOG - stats[result_row(r)]));
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], scale, -stats[result_row(r)]) + stats[64 + result_row(r)]);
       uint32_t bad_go = 0u, bad_q = 0u;
       if (CAREFUL && masked) {
         bad_go = bad_rows<D, BF>(go, 0) >> (4 * half);
@@ -513,7 +520,7 @@ VH_DEV bool prompt_dk_block(const Args& a, const int4& item, char* tiles) {
 
 template <int D, int C, bool BF>
 __global__ void __launch_bounds__(THREADS, back_waves_of(D)) k_prompt_dk(Args a) {
-  __shared__ __attribute__((aligned(16))) char s_tiles[4 * DK_ROWS * D * 2 + 512 + (D == 128 ? BLOCK * D * 2 : 0)];
+  __shared__ __attribute__((aligned(16))) char s_tiles[4 * DK_ROWS * D * 2 + 2 * STATS + (D == 128 ? BLOCK * D * 2 : 0)];
   const int rank = blockIdx.x / (a.kv_heads * (D / C));
   int4 item = make_int4(0, 0, 0, -1);
   if (a.items) {

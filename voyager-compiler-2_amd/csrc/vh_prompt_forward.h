@@ -211,8 +211,12 @@ VH_DEV bool prompt_block(const Args& a, char* lds) {
   // back, long sequences' rows read what is left out of theirs
   void* low = a.o_low && !covers(a, short_run(a, row0), row0) ? a.o_low : nullptr;
   store_columns<D, D, BF>(a.o, low, a.heads, head, row, in, 0, f.acc, by);
-  if (in && lane < 32)
-    a.lse[(int64_t)row * a.heads + head] = f.sum == 0.0f ? -__builtin_inff() : (f.ref - Range<BF>::LIFT + log2f(f.sum)) * LN2;
+  if (in && lane < 32) {
+    const bool none = f.sum == 0.0f;
+    const float less = f.ref - Range<BF>::LIFT, log2_sum = log2f(f.sum), lse = none ? -__builtin_inff() : (less + log2_sum) * LN2;
+    a.lse[(int64_t)row * a.heads + head] = lse;
+    if (a.rest) a.rest[(int64_t)head * a.tokens + row] = weights_lift(BF) - (none ? 0.0f : (less - log2_units(lse)) + log2_sum);
+  }
   // a row whose sum is not finite sees something that is not
   return !CAREFUL && in && f.sum < __builtin_inff() && any_nonfinite(f.acc);
 }

@@ -118,20 +118,20 @@ def _forward(q, k, v, packing, scale, train=False):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     # what the rounding leaves out: the backward pass takes sums over a long sequence's results, in which it would be seen
     low = torch.empty_like(o, dtype=torch.bfloat16) if train else None
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    lse = torch.empty((2 if train else 1, *q.shape[:2]), dtype=torch.float32, device=q.device)  # and what it leaves out
     st = load().vh_prompt_attention(_desc(q, k, v, packing, o, low, lse, scale), stream_on(q.device))
     if st:
         check(st, "vh_prompt_attention")
-    return o, lse, low
+    return o, lse[0], low, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, packing, scale):
-        o, lse, low = _forward(q, k, v, packing, scale, train=True)
+        o, lse, low, stats = _forward(q, k, v, packing, scale, train=True)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
-        ctx.save_for_backward(q, k, v, o, low, lse)
+        ctx.save_for_backward(q, k, v, o, low, stats)
         ctx.packing, ctx.scale = packing, scale
         return o, lse
 
@@ -140,10 +140,10 @@ class _Attention(torch.autograd.Function):
         once("prompt_attention")
         if go is None:
             return (None,) * 5
-        q, k, v, o, low, lse = ctx.saved_tensors
+        q, k, v, o, low, stats = ctx.saved_tensors
         q, k, v, go = _rows(q), _rows(k), _rows(v), _rows(go)
         grads = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)]
-        d = _desc(q, k, v, ctx.packing, o, low, lse, ctx.scale, go, [t.data_ptr() for t in grads])
+        d = _desc(q, k, v, ctx.packing, o, low, stats, ctx.scale, go, [t.data_ptr() for t in grads])
         lib = load()
         need = lib.vh_prompt_attention_workspace_bytes(d)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
