@@ -882,6 +882,15 @@ typedef struct vh_score_desc {
 int vh_score(const vh_score_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
 int vh_score_backward(const vh_score_desc* desc, vh_stream_t stream);
 int64_t vh_score_workspace_bytes(const vh_score_desc* desc);
+/* The same for rows in batches: row i is row i % batch_rows of batch i /
+ * batch_rows, and batches begin batch_st elements apart, as the sequences of a part
+ * of a larger batch do.  The workspace is `score`'s. */
+typedef struct vh_score_batched_desc {
+  vh_score_desc score;
+  int64_t batch_rows, batch_st;
+} vh_score_batched_desc;
+int vh_score_batched(const vh_score_batched_desc* desc, void* work, int64_t work_bytes, vh_stream_t stream);
+int vh_score_batched_backward(const vh_score_batched_desc* desc, vh_stream_t stream);
 
 /* The plan of a packed batch: sequence s is the rows offsets[s] ... offsets[s +
  * 1] - 1 of `tokens` (offsets [sequences + 1] begin at 0 and do not fall; rows

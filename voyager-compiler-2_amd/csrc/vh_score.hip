@@ -46,7 +46,8 @@ typedef unsigned long long okey;  // orders entries: by value, then the lowest i
 
 struct Args {
   const void* x;
-  int64_t x_st, vocab, rows;
+  int64_t x_st, batch_st, vocab, rows;
+  uint32_t batch_rows;  // rows of which lie x_st apart; 0: all
   const int64_t* tokens;
   int64_t piece;  // entries of a piece
   int pieces, top;
@@ -60,6 +61,13 @@ struct Args {
   void* grad;
   uint32_t chunks;
 };
+
+template <typename T>
+VH_DEV const T* logits_of(const Args& a, int64_t row) {
+  if (a.batch_rows == 0) return (const T*)a.x + row * a.x_st;
+  const uint32_t batch = (uint32_t)row / a.batch_rows;
+  return (const T*)a.x + batch * a.batch_st + ((uint32_t)row - batch * a.batch_rows) * a.x_st;
+}
 
 VH_DEV float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // keeps a NaN
 VH_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, 6) k_score(Args a) {
     if (piece == 0) write_padding<THREADS>(a, row);
     return;
   }
-  const T* x = (const T*)a.x + row * a.x_st;
+  const T* x = logits_of<T>(a, row);
   const int begin = (int)(piece * a.piece), end = (int)(begin + a.piece < a.vocab ? begin + a.piece : a.vocab);
   const int first = begin + threadIdx.x * VEC;
   uint4 v[NV];  // as they are held: converted where they are used
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_score_join(Args a) {
     const int p = threadIdx.x;
     const float* part = a.part + (row * a.pieces + (p < a.pieces ? p : 0)) * 3;
     const float mine = p < a.pieces ? part[0] : -INF;
-    const float x = token < a.vocab ? (float)((const T*)a.x + row * a.x_st)[token] : 0.0f;
+    const float x = token < a.vocab ? (float)logits_of<T>(a, row)[token] : 0.0f;
     float to = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) to = maximum(to, __shfl_xor(to, d));
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(BACK_THREADS) k_score_back(Args a) {
   const int begin = (int)(blockIdx.x - row * a.chunks) * (BACK_THREADS * BACK_VECTORS * VEC);
   const int end = begin + BACK_THREADS * BACK_VECTORS * VEC < a.vocab ? begin + BACK_THREADS * BACK_VECTORS * VEC : (int)a.vocab;
   const int64_t token = a.tokens[row];
-  const T* x = (const T*)a.x + row * a.x_st;
+  const T* x = logits_of<T>(a, row);
   T* out = (T*)a.grad + row * a.vocab;
   const float gp = token < 0 || !a.g_logprob ? 0.0f : token < a.vocab ? a.g_logprob[row] : __builtin_nanf("");
   if (threadIdx.x < 64) {
@@ -552,10 +560,12 @@ int64_t part_bytes(const vh_score_desc* d, const Plan& p) {  // of the keys: 8 b
   return p.pieces > 1 ? d->rows * p.pieces * (8ll * d->top + 12) : 0;
 }
 
-Args args_of(const vh_score_desc* d) {
+Args args_of(const vh_score_desc* d, int64_t batch_rows, int64_t batch_st) {
   Args a{};
   a.x = d->logits;
   a.x_st = d->logits_st;
+  a.batch_rows = batch_rows < d->rows ? (uint32_t)batch_rows : 0u;
+  a.batch_st = batch_st;
   a.vocab = d->vocab;
   a.rows = d->rows;
   a.tokens = d->tokens;
@@ -587,25 +597,18 @@ void launch(const Args& a, const Plan& p, hipStream_t s) {
   if (a.pieces > 1) hipLaunchKernelGGL((k_score_join<T>), dim3((unsigned)a.rows), dim3(JOIN_THREADS), 0, s, a);
 }
 
-}  // namespace
-
-extern "C" int64_t vh_score_workspace_bytes(const vh_score_desc* d) {
-  if (check(d, "vh_score_workspace_bytes")) return -1;
-  return d->rows == 0 ? 0 : part_bytes(d, plan_of(d));
-}
-
-extern "C" int vh_score(const vh_score_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
-  if (int e = check(d, "vh_score")) return e;
+int forward(const vh_score_desc* d, int64_t batch_rows, int64_t batch_st, void* work, int64_t work_bytes, vh_stream_t stream,
+            const char* what) {
   if (d->rows == 0) return VH_OK;
   VH_REQUIRE(d->logits && d->tokens && d->logprob && d->entropy && (d->top == 0 || (d->top_logprob && d->top_token)),
-             "vh_score: null argument");
+             "%s: null argument", what);
   const Plan p = plan_of(d);
   // a launch has fewer than 2^32 threads
-  VH_REQUIRE(d->rows * p.pieces < VH_SCORE_MAX_ROWS, "vh_score: too many rows of such a vocabulary");
+  VH_REQUIRE(d->rows * p.pieces < VH_SCORE_MAX_ROWS, "%s: too many rows of such a vocabulary", what);
   const int64_t need = part_bytes(d, p);
   VH_REQUIRE(need == 0 || (work && work_bytes >= need && (uintptr_t)work % 16 == 0),
-             "vh_score: needs %lld bytes of aligned workspace", (long long)need);
-  Args a = args_of(d);
+             "%s: needs %lld bytes of aligned workspace", what, (long long)need);
+  Args a = args_of(d, batch_rows, batch_st);
   a.piece = p.piece;
   a.pieces = p.pieces;
   if (need > 0) {
@@ -616,23 +619,56 @@ extern "C" int vh_score(const vh_score_desc* d, void* work, int64_t work_bytes, 
   if (d->dtype == VH_BF16) launch<__bf16>(a, p, s);
   else if (d->dtype == VH_F16) launch<_Float16>(a, p, s);
   else launch<float>(a, p, s);
-  return vh::check_launch("vh_score");
+  return vh::check_launch(what);
 }
 
-extern "C" int vh_score_backward(const vh_score_desc* d, vh_stream_t stream) {
-  if (int e = check(d, "vh_score_backward")) return e;
+int backward(const vh_score_desc* d, int64_t batch_rows, int64_t batch_st, vh_stream_t stream, const char* what) {
   if (d->rows == 0) return VH_OK;
   VH_REQUIRE(d->logits && d->tokens && d->entropy && d->stats && d->grad && (!d->g_top || d->top == 0 || d->top_token),
-             "vh_score_backward: null argument");
-  Args a = args_of(d);
+             "%s: null argument", what);
+  Args a = args_of(d, batch_rows, batch_st);
   const int64_t each = (int64_t)BACK_THREADS * BACK_VECTORS * (d->dtype == VH_F32 ? 4 : 8);
   a.chunks = (uint32_t)((d->vocab + each - 1) / each);
   const int64_t blocks = d->rows * a.chunks;
-  VH_REQUIRE(blocks < (1ll << 24), "vh_score_backward: too many rows of such a vocabulary");  // as above
+  VH_REQUIRE(blocks < (1ll << 24), "%s: too many rows of such a vocabulary", what);  // as above
   const dim3 grid((unsigned)blocks);
   hipStream_t s = vh::as_stream(stream);
   if (d->dtype == VH_BF16) hipLaunchKernelGGL(k_score_back<__bf16>, grid, dim3(BACK_THREADS), 0, s, a);
   else if (d->dtype == VH_F16) hipLaunchKernelGGL(k_score_back<_Float16>, grid, dim3(BACK_THREADS), 0, s, a);
   else hipLaunchKernelGGL(k_score_back<float>, grid, dim3(BACK_THREADS), 0, s, a);
-  return vh::check_launch("vh_score_backward");
+  return vh::check_launch(what);
+}
+
+int check_batches(const vh_score_batched_desc* d, const char* what) {
+  VH_REQUIRE(d, "%s: null descriptor", what);
+  if (int e = check(&d->score, what)) return e;
+  VH_REQUIRE(d->batch_rows > 0, "%s: batches of one row at least", what);
+  return VH_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t vh_score_workspace_bytes(const vh_score_desc* d) {
+  if (check(d, "vh_score_workspace_bytes")) return -1;
+  return d->rows == 0 ? 0 : part_bytes(d, plan_of(d));
+}
+
+extern "C" int vh_score(const vh_score_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
+  if (int e = check(d, "vh_score")) return e;
+  return forward(d, d->rows, 0, work, work_bytes, stream, "vh_score");
+}
+
+extern "C" int vh_score_backward(const vh_score_desc* d, vh_stream_t stream) {
+  if (int e = check(d, "vh_score_backward")) return e;
+  return backward(d, d->rows, 0, stream, "vh_score_backward");
+}
+
+extern "C" int vh_score_batched(const vh_score_batched_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
+  if (int e = check_batches(d, "vh_score_batched")) return e;
+  return forward(&d->score, d->batch_rows, d->batch_st, work, work_bytes, stream, "vh_score_batched");
+}
+
+extern "C" int vh_score_batched_backward(const vh_score_batched_desc* d, vh_stream_t stream) {
+  if (int e = check_batches(d, "vh_score_batched_backward")) return e;
+  return backward(&d->score, d->batch_rows, d->batch_st, stream, "vh_score_batched_backward");
 }

@@ -206,7 +206,7 @@ _SIGNATURES = {
     "vh_verify": ([_P, _P, _I64, _P], _I32),
     "vh_verify_workspace_bytes": ([_I64, _I64], _I64),
     # a pass over packed sequences: descriptors' bytes as well (rotary.NORM after vh_rope_desc's,
-    # prompt.PROMPT, score.SCORE)
+    # prompt.PROMPT, score.SCORE, and score.BATCHED after vh_score_desc's)
     "vh_norm_rope": ([_P, _P], _I32),
     "vh_norm_rope_backward": ([_P, _P, _I64, _P], _I32),
     "vh_norm_rope_workspace_bytes": ([_P], _I64),
@@ -217,6 +217,8 @@ _SIGNATURES = {
     "vh_prompt_attention_workspace_bytes": ([_P], _I64),
     "vh_score": ([_P, _P, _I64, _P], _I32),
     "vh_score_backward": ([_P, _P], _I32),
+    "vh_score_batched": ([_P, _P, _I64, _P], _I32),
+    "vh_score_batched_backward": ([_P, _P], _I32),
     "vh_score_workspace_bytes": ([_P], _I64),
 }
 

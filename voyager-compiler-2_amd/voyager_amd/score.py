@@ -19,6 +19,8 @@ MAX_TOP = 64
 MAX_VOCAB = 1 << 20
 #: ``vh_score_desc``
 SCORE = struct.Struct("@QqQqqQQQQQQQQQii")
+#: ``vh_score_batched_desc`` after its ``vh_score_desc``
+BATCHED = struct.Struct("@qq")
 _work = {}  # bytes of workspace, by a call's sizes
 
 
@@ -37,8 +39,9 @@ class Scores(NamedTuple):
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Scores:
     """Scores of ``tokens [...]`` (int64) under ``logits [..., vocab]``
     (bfloat16, float16 or float32; at most 2^20 entries, fewer than 2^23 rows),
-    and the ``top`` best alternatives, at most 64.  Rows with dense entries are
-    read in place.
+    and the ``top`` best alternatives, at most 64.  Rows with dense entries, at
+    one distance or in batches of one distance (``logits[:, :-1]``), are read in
+    place; others are copied.
 
     A negative token pads: its row's results are 0, its alternatives -1, and it
     has no gradient.  A token past the vocabulary, which the host does not
@@ -58,12 +61,11 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Sc
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_scores: 0 to {min(MAX_TOP, vocab)} alternatives (got {top})")
     no_tangents("token_scores", logits)
-    x = logits.reshape(-1, vocab)
     t = tokens.reshape(-1)
     if torch.is_grad_enabled() and logits.requires_grad:
-        out = _Scores.apply(x, t, top)
+        out = _Scores.apply(logits, t, top)
     else:
-        out = _scores(x, t, top, False)[:4 if top else 2]
+        out = _scores(logits, t, top, False)[:4 if top else 2]
     shape = tokens.shape
     if len(shape) != 1:
         out = [y.view(shape + y.shape[1:]) for y in out]
@@ -71,20 +73,38 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Sc
 
 
 def _rows(x):
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+    """``x [..., vocab]``, or a copy of it, and how its rows lie: their distance, the
+    rows of a batch, and the batches' distance."""
+    vocab = x.shape[-1]
+    if x.is_contiguous():
+        return x, vocab, 1 << 31, 0
+    if x.stride(-1) == 1 or vocab == 1:
+        dims = []  # sizes and strides, of which the inner ones go on where the outer ones' next is
+        for n, st in zip(x.shape[:-1], x.stride()):
+            if n == 1:
+                continue
+            if dims and dims[-1][1] == n * st:
+                dims[-1] = dims[-1][0] * n, st
+            else:
+                dims.append((n, st))
+        if len(dims) <= 1:
+            return x, dims[0][1] if dims else 0, 1 << 31, 0
+        if len(dims) == 2:
+            return x, dims[1][1], dims[1][0], dims[0][1]
+    return x.contiguous(), vocab, 1 << 31, 0
 
 
 def _scores(x, tokens, top, train):
-    x, tokens = _rows(x), tokens.contiguous()
-    rows, vocab = x.shape
+    (x, step, *batch), tokens = _rows(x), tokens.contiguous()
+    rows, vocab = tokens.shape[0], x.shape[-1]
     dev = x.device
     f = dict(dtype=torch.float32, device=dev)
     logprob, entropy = torch.empty(rows, **f), torch.empty(rows, **f)
     stats = torch.empty(rows, 2, **f) if train else None
     best = torch.empty(rows, top, **f) if top else None
     index = torch.empty(rows, top, dtype=torch.int64, device=dev) if top else None
-    d = SCORE.pack(x.data_ptr(), x.stride(0), tokens.data_ptr(), rows, vocab, logprob.data_ptr(), entropy.data_ptr(),
-                   ptr(stats) or 0, ptr(best) or 0, ptr(index) or 0, 0, 0, 0, 0, dtype_code(x.dtype), top)
+    d = SCORE.pack(x.data_ptr(), step, tokens.data_ptr(), rows, vocab, logprob.data_ptr(), entropy.data_ptr(),
+                   ptr(stats) or 0, ptr(best) or 0, ptr(index) or 0, 0, 0, 0, 0, dtype_code(x.dtype), top) + BATCHED.pack(*batch)
     lib = load()
     sizes = (rows, vocab, x.dtype, top)
     need = _work.get(sizes)
@@ -95,9 +115,9 @@ def _scores(x, tokens, top, train):
                 _work.clear()
             _work[sizes] = need
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    st = lib.vh_score(d, ptr(work), max(need, 0), stream_on(dev))
+    st = lib.vh_score_batched(d, ptr(work), max(need, 0), stream_on(dev))
     if st:
-        check(st, "vh_score")
+        check(st, "vh_score_batched")
     return logprob, entropy, best, index, stats
 
 
@@ -122,13 +142,13 @@ class _Scores(torch.autograd.Function):
         if g_logprob is None and g_entropy is None and g_best is None:
             return None, None, None
         x, tokens, entropy, stats, index = ctx.saved_tensors
-        x, tokens = _rows(x), tokens.contiguous()
-        rows, vocab = x.shape
+        (x, step, *batch), tokens = _rows(x), tokens.contiguous()
         g = [None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_best)]
-        grad = torch.empty(rows, vocab, dtype=x.dtype, device=x.device)
-        d = SCORE.pack(x.data_ptr(), x.stride(0), tokens.data_ptr(), rows, vocab, 0, entropy.data_ptr(), stats.data_ptr(), 0,
-                       ptr(index) or 0, *(ptr(t) or 0 for t in g), grad.data_ptr(), dtype_code(x.dtype), ctx.top)
-        st = load().vh_score_backward(d, stream_on(x.device))
+        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d = SCORE.pack(x.data_ptr(), step, tokens.data_ptr(), tokens.shape[0], x.shape[-1], 0, entropy.data_ptr(), stats.data_ptr(),
+                       0, ptr(index) or 0, *(ptr(t) or 0 for t in g), grad.data_ptr(), dtype_code(x.dtype),
+                       ctx.top) + BATCHED.pack(*batch)
+        st = load().vh_score_batched_backward(d, stream_on(x.device))
         if st:
-            check(st, "vh_score_backward")
+            check(st, "vh_score_batched_backward")
         return grad, None, None
