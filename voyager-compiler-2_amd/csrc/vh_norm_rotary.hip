@@ -10,9 +10,10 @@
 // A head's channels lie with a group of 2^n lanes, so its squares are summed
 // by exchanges inside the group and its values are read once.  Squares, sums
 // and products are float32, results are rounded once.  The weights' gradient
-// is summed in a fixed order: each lane over the heads that it takes, the
-// lanes of a workgroup through LDS, the workgroups by a second kernel in
-// float64.
+// is summed in a fixed order: each lane over the heads that it takes, in float32
+// (ten of 8192 tokens of 32 + 8 heads of 128); the lanes of a workgroup through LDS and
+// the workgroups by a second kernel in float64, as sums of many equal terms in
+// float32 are off by up to half their number.
 //
 // Bound by memory.  8192 tokens of 32 + 8 heads of 128 in bfloat16: forward (168
 // MB) 30 us, 5.5 TB/s; back (252 MB) 48 us, 5.2 TB/s, and 5 us for the weights'
@@ -28,7 +29,7 @@ constexpr int THREADS = 256;
 constexpr int MAX_DIM = 512;
 constexpr int TOKENS = 4;      // tokens of a workgroup when there are many
 // Workgroups that share out the tokens of a backward pass: four a CU, whose sums
-// of the weights' gradients are then 1 MB.
+// of the weights' gradients are then 2 MB.
 constexpr int BACK_GROUPS = 1024;
 // At most, one way and the other, of a launch, which has fewer than 2^32 threads; they take turns beyond.
 constexpr int64_t MOST_GROUPS = 1 << 22, MOST_HEAD_GROUPS = 1 << 15;
@@ -48,7 +49,7 @@ struct Args {
   const double* turns;
   int64_t tokens, rows;
   FastDiv heads_div;
-  float* part;  // backward: [workgroups, 2, dim] sums of the weights' gradients, or NULL
+  double* part;  // backward: [workgroups, 2, dim] sums of the weights' gradients, or NULL
   int nq, nk, dim, rotary, units, lanes, pos64, w32;
   float factor, eps;
 };
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(THREADS) k_norm_rope(Args a) {
     if (!a.part) return;
     // [per, dim] of one tensor at a time: 256 threads hold V values each
     __shared__ float s_sum[THREADS * V];
-    float* to = a.part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.dim;
+    double* to = a.part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.dim;
 #pragma unroll
     for (int key = 0; key < 2; ++key) {
       __syncthreads();
@@ -256,8 +257,8 @@ __global__ void __launch_bounds__(THREADS) k_norm_rope(Args a) {
       }
       __syncthreads();
       for (int c = threadIdx.x; c < a.dim; c += THREADS) {
-        float all = 0.0f;
-        for (int p = 0; p < per; ++p) all += s_sum[p * a.dim + c];
+        double all = 0.0;
+        for (int p = 0; p < per; ++p) all += (double)s_sum[p * a.dim + c];
         to[key * a.dim + c] = all;
       }
     }
@@ -266,13 +267,13 @@ __global__ void __launch_bounds__(THREADS) k_norm_rope(Args a) {
 
 // The workgroups' sums joined: 16 columns a workgroup, 16 threads a column.
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_weights(const float* part, int parts, int dim, T* gq, T* gk) {
+__global__ void __launch_bounds__(256) k_norm_weights(const double* part, int parts, int dim, T* gq, T* gk) {
   __shared__ double s_sum[16][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
   double sum = 0.0;
   if (col < 2 * dim) {
 #pragma unroll 8
-    for (int p = r; p < parts; p += 16) sum += (double)part[(int64_t)p * 2 * dim + col];
+    for (int p = r; p < parts; p += 16) sum += part[(int64_t)p * 2 * dim + col];
   }
   s_sum[r][c] = sum;
   __syncthreads();
@@ -388,7 +389,7 @@ extern "C" int vh_norm_rope(const vh_norm_rope_desc* d, vh_stream_t stream) {
 extern "C" int64_t vh_norm_rope_workspace_bytes(const vh_norm_rope_desc* d) {
   if (check(d, "vh_norm_rope_workspace_bytes")) return -1;
   if (nothing(d->rope)) return 0;
-  return (int64_t)BACK_GROUPS * 2 * d->rope.dim * (int64_t)sizeof(float);
+  return (int64_t)BACK_GROUPS * 2 * d->rope.dim * (int64_t)sizeof(double);
 }
 
 extern "C" int vh_norm_rope_backward(const vh_norm_rope_desc* d, void* work, int64_t work_bytes, vh_stream_t stream) {
@@ -399,12 +400,12 @@ extern "C" int vh_norm_rope_backward(const vh_norm_rope_desc* d, void* work, int
                  r.turns,
              "vh_norm_rope_backward: null argument");
   const bool weights = d->gq_weight || d->gk_weight;
-  const int64_t need = (int64_t)BACK_GROUPS * 2 * r.dim * (int64_t)sizeof(float);
+  const int64_t need = (int64_t)BACK_GROUPS * 2 * r.dim * (int64_t)sizeof(double);
   VH_REQUIRE(!weights || (work && work_bytes >= need && (uintptr_t)work % 16 == 0),
              "vh_norm_rope_backward: needs %lld bytes of aligned workspace", (long long)need);
   const Plan p = plan_of(d, true);
   Args a = args_of(d, p);
-  a.part = weights ? (float*)work : nullptr;
+  a.part = weights ? (double*)work : nullptr;
   hipStream_t s = vh::as_stream(stream);
   if (r.dtype == VH_BF16) dispatch<__bf16, true>(a, p, r.interleaved != 0, s);
   else if (r.dtype == VH_F16) dispatch<_Float16, true>(a, p, r.interleaved != 0, s);
