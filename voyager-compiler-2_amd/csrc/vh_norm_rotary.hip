@@ -16,7 +16,7 @@
 // float32 are off by up to half their number.
 //
 // Bound by memory.  8192 tokens of 32 + 8 heads of 128 in bfloat16: forward (168
-// MB) 30 us, 5.5 TB/s; back (252 MB) 48 us, 5.2 TB/s, and 5 us for the weights'
+// MB) 30 us, 5.5 TB/s; back (252 MB) 50 us, 5.0 TB/s, and 5 us for the weights'
 // sums.  A single token 3.6 us, its loads' and the launch's latency.
 #include <hip/hip_runtime.h>
 

@@ -5,9 +5,9 @@
 // seven, but every sum has one owner and one order, and nothing is added up in
 // memory.
 //
-// 8192 rows, 32 + 8 heads of 128 in bfloat16, one sequence: dq 740 us, dk and dv
-// 1155 us (1120 and 950 TFLOP/s of the products made); six documents of 8192 rows
-// 283, 396 and 11 us of joining.  Both are bound by the matrix units and the
+// 8192 rows, 32 + 8 heads of 128 in bfloat16, one sequence: dq 735-755 us, dk and dv
+// 1170-1240 us (1110 and 910 TFLOP/s of the products made); six documents of 8192 rows
+// 280-290, 420-455 and 12 us of joining.  Both are bound by the matrix units and the
 // vector instructions between their products, at two waves a SIMD.
 #pragma once
 
@@ -150,18 +150,18 @@ VH_DEV void lift(f32x16& ds, float& up, f32x16 (&acc)[N]) {
 }
 
 // The rows of long sequences have many keys, whose weights' rounding averages out:
-// their gradients are off by 1.41 to 1.49 times a result's own rounding.  Those of short
+// their gradients are off by 1.34 to 1.62 times a result's own rounding.  Those of short
 // ones (under VH_PROMPT_SHORT rows) have few, down to two: a weight's rounding is seen
 // in a gradient, and twice in D, which is a sum over the output, that has it as well.
 // They take D as a sum over the weights instead, and weights and their gradients in
 // two parts of 16 bits, each with a product of its own: 1.00 times the rounding.  A
 // block with rows of such sequences does so in the tiles in which they meet their
 // keys, whatever else it holds (two loops: a choice in the loop costs registers, and
-// spills in both cases).  The second
-// parts take 4 to 12% of the backward pass (us of dq, and of dk and dv, without and
-// with them: 32 sequences of 256, 32 + 8 heads of 128, 103 + 74 and 110 + 85; 20 of
-// 400, heads of 64, 78 + 61 and 82 + 76; 64 of 125, 16 + 16 heads of 64, 40 + 37 and
-// 42 + 40), and D by the keys two fifths of dq's products: too much for long rows.
+// spills in both cases).  The second parts take 6 to 12% of the two kernels' time (us of dq,
+// and of dk and dv, without and with them: 32 sequences of 256, 32 + 8 heads of 128,
+// 104 + 78 and 109 + 91; 20 of 400, heads of 64, 82 + 70 and 86 + 84; 64 of 125,
+// 16 + 16 heads of 64, 40 + 41 and 42 + 45), and D by the keys two fifths of dq's
+// products: too much for long rows.
 // ------------------------------------------------------------------ dq
 constexpr int DQ_KEYS = 64;  // of a tile; a wave takes 32 at a time
 

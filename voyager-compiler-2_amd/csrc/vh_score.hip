@@ -19,7 +19,8 @@
 //
 // Bound: with alternatives, and rows for the whole card, what finds them beside the
 // exponentials (4001 rows of 32,000 in float16 with the best one: 62 us, 4.2 TB/s);
-// without, memory (2048 rows of 128,000 in bfloat16: 102 us, 5.1 TB/s; back, read and
+// without, memory (2048 rows of 128,000 in bfloat16: 107 us, 4.9 TB/s, and 141 behind a
+// backward pass, whose writes are on their way to memory; back, read and
 // written, 162 us, 6.5 TB/s, part of it in the last cache); for few rows the latency
 // of two launches (32 rows of 128,000 with twenty: 11 + 4 us).
 //

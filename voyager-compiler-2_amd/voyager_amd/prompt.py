@@ -28,7 +28,9 @@ class Packing:
     from 0 on and not falling; equal ones are a sequence of no rows).  Rows
     behind the last sequence pad the batch.  Offsets are read on the device,
     when the packing is made: where they are not so, all rows pad, and
-    :meth:`check` raises.  Fewer than 2^24 tokens, and 2^20 sequences."""
+    :meth:`check` raises.  Empty sequences cost nothing, but where there are few rows
+    a launch is shaped, and its sums ordered, by the number of sequences.  Fewer
+    than 2^24 tokens, and 2^20 sequences."""
 
     def __init__(self, offsets: torch.Tensor, tokens: int):
         if offsets.dim() != 1 or offsets.dtype is not torch.int32 or not offsets.is_cuda or offsets.shape[0] < 1:
@@ -67,8 +69,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     infinity or NaN may be NaN, and bfloat16 values under 2^-94 may count as 0.
     Scores, weights' sums and results are held in float32; weights, and in the
     backward pass their gradients, are rounded to the values' type for the matrix
-    instructions (for sequences of fewer than 512 rows in two parts).  Differentiable once in q, k
-    and v; sums are in a fixed order."""
+    instructions (for sequences of fewer than 512 rows in two parts).  Of a score
+    of size 2^n some 2^(n - 22) is not known, nor is as much of its weight.
+    Differentiable once in q, k and v; sums are in a fixed order."""
     given = (q.shape, q.dtype, q.device, k.shape, k.dtype, k.device, v.shape, v.dtype, v.device)
     if given != packing._checked:  # a layer's sizes are mostly those of the layer before
         _check(q, k, v, packing)

@@ -119,8 +119,9 @@ class Rotary:
         or both float32; None where its tensor is) hold for all heads; the rest
         is as in a call of the embedding.  Squares are summed in float32: a
         head whose sum passes its largest value becomes 0, as one with an
-        infinity does in its finite channels.  Differentiable once in q, k and
-        the weights, whose gradients are summed in a fixed order."""
+        infinity does but in that channel and the one that it turns with, which
+        become NaN.  Differentiable once in q, k and the weights, whose gradients
+        are summed in a fixed order: of a few heads in float32, of all in float64."""
         wide = [None if t is None else (t.shape, t.dtype, t.device) for t in (q, k, positions, q_weight, k_weight)]
         given = (*wide, eps, self.turns.device)
         if given != self._normed:
