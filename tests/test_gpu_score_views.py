@@ -69,3 +69,31 @@ def test_views_are_not_copied(view):
     ones = torch.ones_like(s.logprob)
     used, (dx,) = most(lambda: torch.autograd.grad(s.logprob, part, ones))
     assert used < size + size // 4
+
+
+def test_entries_of_rows_at_one_distance():
+    """The C entries without batches, beside the call."""
+    from voyager_amd import _lib
+
+    x = _batch((6, 5003), torch.float16)
+    tokens = torch.tensor([0, 5002, -1, 7, 5003, 9]).cuda()
+    leaf = x.clone().requires_grad_()
+    want = score.token_scores(leaf, tokens, top=2)
+    g = torch.randn(6, generator=torch.Generator().manual_seed(3)).cuda()
+    (grad,) = torch.autograd.grad(want.logprob, leaf, g)
+    f = lambda *s: torch.empty(*s, device="cuda")
+    logprob, entropy, stats, best, out = f(6), f(6), f(6, 2), f(6, 2), torch.empty_like(x)
+    index = torch.empty(6, 2, dtype=torch.int64, device="cuda")
+    lib, stream = _lib.load(), _lib.stream_on(x.device)
+
+    def desc(gp):
+        return score.SCORE.pack(x.data_ptr(), 5003, tokens.data_ptr(), 6, 5003, logprob.data_ptr(), entropy.data_ptr(),
+                                stats.data_ptr(), best.data_ptr(), index.data_ptr(), gp, 0, 0, out.data_ptr(),
+                                _lib.dtype_code(x.dtype), 2)
+
+    need = lib.vh_score_workspace_bytes(desc(0))
+    work = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    assert lib.vh_score(desc(0), work.data_ptr(), need, stream) == 0
+    assert lib.vh_score_backward(desc(g.data_ptr()), stream) == 0
+    for a, b in ((logprob, want.logprob), (entropy, want.entropy), (best, want.top_logprob), (index, want.top_token), (out, grad)):
+        assert torch.equal(a.nan_to_num(7), b.detach().nan_to_num(7))
